@@ -342,6 +342,97 @@ int s1_head_norm_rope(s1_ctx* ctx, void* x, long long ldx, long long head_stride
                       const int32_t* positions, int max_positions, int rotary_dim, int total_tokens, int bf16_ops);
 
 /*
+ * ---- One new token at a time: a paged key-value cache, and the recurrent state of the linear-attention layers.
+ *
+ * The reference runs whole prompts only (`Decoder::forward`, src/archs/qwen35_text.rs:942-1005); with the calls of this section the
+ * same layers go on from where a prompt ended. None of them copies from or to the host or allocates; all can be captured into a graph.
+ * Bad contents of device arrays (a page, slot, length or position outside its range) are reported by s1_sync as S1_EKERNEL; the
+ * rows concerned are left out as each call says, and nothing outside the given buffers is read or written.
+ *
+ * The cache of a layer: k_cache and v_cache, bf16, of the same shape - page p, token i of the page, KV head h at
+ * p * page_stride + i * token_stride + h * head_stride elements (multiples of 8; head_dim values in a row). page_size is a power of
+ * two. Block tables: int32 [rows, ldt]; entry i of a row is the page that holds its tokens i * page_size ... A token's slot is
+ * page * page_size + (position mod page_size), -1: none.
+ */
+
+/*
+ * Block tables and slot maps from request lengths. Row b holds cached[b] tokens (negative: an idle row, which gets none) and is
+ * to hold added[b] more (negative counts as 0; `added` NULL: one more each). Pages are taken from the end of the stack free_pages[0 .. *free_count)
+ * in the order of the rows; the new entries of the block tables are written, others left as they are.
+ *   lengths [num_seqs]        cached + added (idle rows: unchanged); may be `cached`
+ *   free_count_out [1]        pages left; may be `free_count`
+ *   cu_seqlens [num_seqs + 1] first token of every row in the packed batch (may be NULL)
+ *   positions, slots [max_tokens]  of every token of the packed batch, row after row. `added` NULL: token b belongs to row b and
+ *                             max_tokens = num_seqs. Tokens of idle rows and those behind the last get position 0 and slot -1.
+ * A row whose tokens do not fit (its block table's width, the free pages, max_tokens) is reported and gets nothing: no page, its
+ * length unchanged, position 0 and slot -1 for its tokens (with too few pages that holds for every later row that needs one too).
+ * num_seqs <= 8192, max_tokens and free_capacity (entries of free_pages) < 2^30. The outputs must not overlap other arguments
+ * except as said.
+ */
+int s1_block_tables(s1_ctx* ctx, const int32_t* cached, const int32_t* added, int num_seqs, int page_size, const int32_t* free_pages,
+                    int free_capacity, const int32_t* free_count, int32_t* free_count_out, int32_t* tables, long long ldt, int table_width,
+                    int32_t* lengths, int32_t* cu_seqlens, int32_t* positions, int32_t* slots, int max_tokens);
+/* The pages of every row with ended[b] != 0 go back on the stack, in the order of the rows, and its length becomes -1. A row whose
+ * length is more than its block table holds, or whose pages find no room on the stack, is reported and stays as it is. */
+int s1_release_blocks(s1_ctx* ctx, const int32_t* ended, int num_seqs, int page_size, int32_t* lengths, const int32_t* tables, long long ldt,
+                      int table_width, int32_t* free_pages, int free_capacity, int32_t* free_count);
+
+/*
+ * Keys and values of `total_tokens` tokens into their slots (slot -1: left out; two tokens of a call must not have the same slot).
+ * k, v: bf16, head h of token t at k + t * ldk + h * k_head_stride. With `norm_weight` the keys are normed and rotated on the
+ * way, bit-identical to s1_head_norm_rope (whose arguments these are) before the write; k itself is not changed. NULL: they are
+ * written as they are, and the arguments down to bf16_ops are not read. head_dim 64, 128 or 256. A token whose position is
+ * outside the tables is reported and written unrotated, one whose slot is outside the cache is reported and left out.
+ */
+int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long long k_head_stride, const void* v, long long ldv, long long v_head_stride,
+                   const int32_t* slots, int total_tokens, int kv_heads, int head_dim, const void* norm_weight, float eps,
+                   const float* cos_table, const float* sin_table, const int32_t* positions, int max_positions, int rotary_dim, int bf16_ops,
+                   void* k_cache, void* v_cache, int num_pages, int page_size, long long page_stride, long long token_stride,
+                   long long head_stride);
+
+/*
+ * Attention of one new token per row over the cache, the step form of s1_attention_gqa: row b attends to its lengths[b] first
+ * tokens (the new one among them once s1_cache_write has put it there), query head h reading KV head h / (heads / kv_heads):
+ *     a = softmax(scale * q k^T) v,   out = a * sigmoid(gate) with a gate, in f32 and rounded once.
+ * A row with lengths[b] <= 0 gets zeros. lengths: DEVICE int32; tables [num_seqs, ldt], of which table_width entries a row may be
+ * used. A length beyond that is reported and its row gets zeros; a page outside the cache is reported and its keys are left out.
+ * head_dim 64, 128 or 256; any group size. q, gate: as for s1_attention_gqa; out: bf16 [num_seqs, heads * head_dim].
+ * `workspace`: device memory, 16-byte aligned, of s1_attention_paged_workspace(head_dim) bytes whatever the batch; calls that may
+ * run at the same time (graphs replayed on two streams among them) need one each.
+ */
+size_t s1_attention_paged_workspace(int head_dim);
+int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, long long q_head_stride, const void* k_cache, const void* v_cache,
+                       int num_pages, int page_size, long long page_stride, long long token_stride, long long head_stride,
+                       const int32_t* tables, long long ldt, int table_width, const int32_t* lengths, int num_seqs, int heads, int kv_heads,
+                       int head_dim, float scale, const void* gate, long long ldg, long long gate_head_stride, void* out, long long ldo,
+                       void* workspace, size_t workspace_bytes);
+
+/*
+ * The gated delta rule on a carried state. state: f32 [num_states, value_heads, 128 (key), 128 (value)]; conv_state: bf16
+ * [num_states, 4, 2 * key_heads * 128 + value_heads * 128], the projection's last rows before the conv, position p in row p mod 4.
+ * state_index: DEVICE int32 [num_seqs], the state of each row, negative: none. Two rows of a call with the same state, or one
+ * outside the states, are reported; the first of the two is carried out.
+ *   s1_gated_delta_rule_prefill  s1_gated_delta_rule_conv (bit-identical output), which also leaves every sequence's final state and
+ *                                the ring of its last rows; cu_seqlens: the offsets once more, as a DEVICE array. Sequences start
+ *                                from zero. A sequence of no tokens, or with a negative state, leaves nothing.
+ *   s1_gated_delta_rule_step     one new token of each row: conv, SiLU, the gates, the recurrence and the gated norm of
+ *                                s1_gated_delta_rule_conv as one kernel, in f32 with one rounding, updating both states in place.
+ *                                positions: DEVICE int32 [num_seqs], the token's index in its sequence; at 0 the sequence starts
+ *                                from zero whatever the state holds. Rows without a state get zeros in y. state_index NULL: row b
+ *                                has state b. b_proj, a_proj: bf16 [num_seqs, value_heads], row stride ldba.
+ */
+int s1_gated_delta_rule_prefill(s1_ctx* ctx, const void* mixed_before_conv, long long ldm, const void* conv_weight,
+                                const int32_t* positions, const void* b_proj, const void* a_proj, long long ldba, const float* dt_bias,
+                                const float* neg_exp_a, const void* z, long long ldz, const void* norm_weight, float eps,
+                                const int32_t* cu_seqlens_host, int num_seqs, int total_tokens, int key_heads, int value_heads, void* y,
+                                long long ldy, void* workspace, size_t workspace_bytes, const int32_t* cu_seqlens,
+                                const int32_t* state_index, int num_states, void* conv_state, float* state);
+int s1_gated_delta_rule_step(s1_ctx* ctx, const void* mixed, long long ldm, const void* conv_weight, const int32_t* positions,
+                             const void* b_proj, const void* a_proj, long long ldba, const float* dt_bias, const float* neg_exp_a,
+                             const void* z, long long ldz, const void* norm_weight, float eps, const int32_t* state_index, int num_states,
+                             void* conv_state, float* state, int num_seqs, int key_heads, int value_heads, void* y, long long ldy);
+
+/*
  * Tensor parallelism: the sum over ranks that follows a row-parallel projection (each rank holds a K range of the
  * weight and produces a partial [T, N]). The reference has no multi-GPU path (`device::load` opens GPU 0 only,
  * src/device.rs:43-56); these entry points exist for the sharded projections of the large hybrid model.

@@ -132,6 +132,22 @@ extern "C" int s1_sync(s1_ctx* ctx) {
         if (st[0] == 101 || st[0] == 102)
             return s1_fail(ctx, S1_EKERNEL, "%s: row %d has index %d outside the table", st[0] == 101 ? "s1_norm gather" : "s1_rope position",
                            st[2], st[3]);
+        if (st[0] >= 110 && st[0] < 130) {
+            static const char* const what[] = {
+                "s1_block_tables: row %d needs more pages than its block table holds (%d tokens)",          // 110
+                "s1_block_tables: no free pages left for row %d (%d tokens)",                               // 111
+                "s1_block_tables: row %d has tokens beyond max_tokens (%d in its sequence)",                // 112
+                "s1_block_tables: row %d was given page %d",                                                // 113
+                "s1_release_blocks: row %d has %d tokens, more than its block table holds",                 // 114
+                "s1_release_blocks: the stack of free pages has no room for those of row %d (%d tokens)",   // 115
+                "s1_cache_write: token %d has slot %d, outside the cache",                                  // 116
+                "s1_attention_paged: row %d has %d tokens, more than its block table holds",                // 117
+                "s1_attention_paged: the block table of row %d names page %d, outside the cache",           // 118
+                "s1_gated_delta_rule: row %d has state %d, outside the states or another row's",            // 119
+                "s1_gated_delta_rule_step: row %d has position %d"};                                        // 120
+            const int n = static_cast<int>(sizeof(what) / sizeof(what[0]));
+            if (st[0] - 110 < n) return s1_fail(ctx, S1_EKERNEL, what[st[0] - 110], st[2], st[3]);
+        }
         return s1_fail(ctx, S1_EKERNEL, "kernel gave up on a bounded wait: code %d block %d role %d tile %d", st[0],
                        st[1], st[2], st[3]);
     }

@@ -1,0 +1,483 @@
+// Attention of one new token per request over a paged key-value cache (grouped query heads, head dim 64, 128 or 256):
+//     a[b, h] = sum_{j < len_b} softmax_j(scale * q[b, h] . k_j) v_j,   k_j, v_j of KV head h / (heads / kv_heads)
+// and, with a gate, a * sigmoid(gate). It is the step form of the causal attention of src/archs/qwen35_text.rs:312-411, whose
+// keys and values here come from the cache instead of from the same prompt.
+//
+// What bounds it: every key and value is read once for the query heads that share it, 4 * group flops per 4 bytes - HBM, whatever
+// the group size. So the kernel is built around the loads:
+//  * work is cut into units of kUnit keys of one (row, KV head, up to 8 query heads) - a "span" is all units of one such triple -
+//    and the units of the whole batch, in order, are dealt out in equal contiguous ranges, one to each of the grid's CTAs. The
+//    CTAs find their ranges from the lengths in device memory, so that nothing of a step depends on the host and the balance holds
+//    for one long context and for many ragged ones alike. A span that crosses from one CTA to the next leaves partial results
+//    (maximum, sum, unnormalised output in f32) in the workspace, at most two per CTA, and the second kernel joins them in the order
+//    of the units: results do not depend on timing.
+//  * inside a CTA the warps take tiles of 16 keys in turn, each through a ring of its own in shared memory (cp.async, 24 KB a warp,
+//    192 KB an SM in flight or in use): no warp waits for another until its span is done.
+//  * the products run on mma.sync m16n8k16 with the operands turned round - S^T = K Q^T, O^T = V^T P^T - so that the 16 rows are
+//    keys and head dimensions, which there are enough of, and the 8 columns the query heads of the group. tcgen05 would want 64 or
+//    128 rows of queries where there are 1 to 16; at the rate that HBM delivers keys, mma.sync is a fifth busy.
+// Scores, maxima, sums and outputs are f32; the probabilities are rounded to bf16 for the second product, as in s1_attention
+// (an error of 2^-9 of each weight, averaged over the keys), while their sum is that of the unrounded ones.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "context.h"
+#include "device_guard.h"
+#include "ptx.cuh"
+
+using namespace s1;
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 16;               // keys of one warp step
+constexpr int kUnit = kWarps * kTile;   // keys of one unit of work
+constexpr int kHeads = 8;               // query heads of one span (columns of the MMAs)
+constexpr int kRingBytes = 24 * 1024;   // per warp
+
+struct PagedParams {
+    const __nv_bfloat16* q;
+    long long ldq, q_head_stride;
+    const __nv_bfloat16* k;
+    const __nv_bfloat16* v;
+    long long page_stride, token_stride, head_stride;
+    int num_pages, shift;
+    const int32_t* tables;
+    long long ldt;
+    int table_width;
+    const int32_t* lengths;
+    int num_seqs, heads, kv_heads, group, spans_per_row, blocks_per_group;
+    float scale_log2;
+    const __nv_bfloat16* gate;
+    long long ldg, gate_head_stride;
+    __nv_bfloat16* out;
+    long long ldo;
+    float* parts;   // [2 * grid][kHeads][D + 2]: first D unnormalised outputs, then maximum (in units of log2) and sum
+    int4* records;  // [grid]: row, span of the row, last CTA of the span that begins in this CTA and is cut (or -1)
+    int* status;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ void report(int* status, int code, int where, int value) {
+    if (atomicCAS(status, 0, code) == 0) {
+        status[1] = static_cast<int>(blockIdx.x);
+        status[2] = where;
+        status[3] = value;
+    }
+}
+// Keys that a row attends to; a length beyond its block table is reported and the row treated as empty.
+__device__ __forceinline__ int row_length(const PagedParams& p, int b, bool tell) {
+    const int len = max(__ldg(p.lengths + b), 0);
+    if (len > (static_cast<long long>(p.table_width) << p.shift)) {
+        if (tell) report(p.status, 117, b, len);
+        return 0;
+    }
+    return len;
+}
+template <int D>
+__device__ __forceinline__ void store_out(const PagedParams& p, int b, int h, int d, float x) {
+    if (p.gate) x /= 1.f + exp2_fast(-1.4426950408889634f * __bfloat162float(p.gate[b * p.ldg + h * p.gate_head_stride + d]));
+    p.out[b * p.ldo + h * D + d] = __float2bfloat16_rn(x);
+}
+
+// One warp's pass over its tiles of a span: keys first + 16 (warp + 8 i), below `end`.
+template <int D>
+struct WarpPass {
+    static constexpr int kSlotBytes = kTile * D * 2;
+    static constexpr int kSlots = kRingBytes / kSlotBytes;  // 3, 6 or 12
+    static constexpr int kChunks = D / 8;                   // 16-byte pieces of a key
+    static constexpr int kRowsPerCopy = 32 / kChunks;
+    static constexpr int kSteps = D / 16;
+    static constexpr int kChains = D == 256 ? 4 : 2;        // independent accumulators of S^T
+
+    const PagedParams& p;
+    const int lane;
+    const uint32_t ring;            // shared address of this warp's ring
+    volatile uint32_t* masks;       // [kSlots] which of the 16 keys a slot holds
+    float O[kSteps][4];             // O^T: dims 16 s + lane/4 (+ 8), heads 2 (lane % 4) (+ 1)
+    float m[2], l[2];
+    long long off;                  // lane k < 16: where key k of the tile whose keys were requested last begins
+    uint32_t mask;
+
+    __device__ __forceinline__ WarpPass(const PagedParams& p_, int lane_, uint32_t ring_, uint32_t* masks_) : p(p_), lane(lane_), ring(ring_), masks(masks_) {}
+
+    // request number n: the keys (even) or values (odd) of this warp's tile n / 2, into slot `slot`
+    __device__ __forceinline__ void request(int n, int slot, int b, int kvh, int first, int end) {
+        const bool values = n & 1;
+        if (!values) {
+            const int j = first + (n >> 1) * kUnit + lane;
+            const bool want = lane < kTile && j < end;
+            const int page = want ? __ldg(p.tables + b * p.ldt + (j >> p.shift)) : 0;
+            const bool ok = want && page >= 0 && page < p.num_pages;
+            if (want && !ok) report(p.status, 118, b, page);
+            off = ok ? page * p.page_stride + (j & ((1 << p.shift) - 1)) * p.token_stride + kvh * p.head_stride : 0;
+            mask = __ballot_sync(0xffffffffu, ok);
+        }
+        if (lane == 0) masks[slot] = mask;
+        const __nv_bfloat16* base = values ? p.v : p.k;
+        const uint32_t dst = ring + slot * kSlotBytes;
+#pragma unroll
+        for (int i = 0; i < kTile / kRowsPerCopy; ++i) {
+            const int row = i * kRowsPerCopy + lane / kChunks, ch = lane % kChunks;
+            const long long o = __shfl_sync(0xffffffffu, off, row);
+            // keys past the end (and those of a bad page) are zeros: what lies in the rest of a page is never multiplied
+            cp16(dst + row * (D * 2) + ((ch ^ (row & 7)) << 4), base + o + ch * 8, (mask >> row & 1u) ? 16u : 0u);
+        }
+    }
+
+    __device__ __forceinline__ void run(int b, int kvh, const uint32_t (&qf)[kSteps][2], int first, int end) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) O[s][0] = O[s][1] = O[s][2] = O[s][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+        const int requests = first < end ? 2 * ((end - first + kUnit - 1) / kUnit) : 0;
+        int wslot = 0, rslot = 0;
+#pragma unroll 1
+        for (int n = 0; n < kSlots - 1; ++n) {
+            if (n < requests) request(n, wslot, b, kvh, first, end);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ++wslot;
+        }
+        uint32_t pb0 = 0, pb1 = 0;
+#pragma unroll 1
+        for (int n = 0; n < requests; n += 2) {
+            // ---- keys: S^T = K Q^T
+            asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+            __syncwarp();  // the slot has landed for every lane, and every lane is done with the one refilled next
+            if (n + kSlots - 1 < requests) request(n + kSlots - 1, wslot, b, kvh, first, end);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            wslot = wslot + 1 == kSlots ? 0 : wslot + 1;
+            {
+                const uint32_t live = masks[rslot];
+                const uint32_t row = ring + rslot * kSlotBytes + ((lane >> 3 & 1) * 8 + (lane & 7)) * (D * 2);
+                float c[kChains][4];
+#pragma unroll
+                for (int i = 0; i < kChains; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+                    uint32_t a[4];
+                    ldsm4(a, row + (((2 * s + (lane >> 4)) ^ (lane & 7)) << 4));
+                    mma16816(c[s % kChains], a, qf[s][0], qf[s][1]);
+                }
+#pragma unroll
+                for (int i = 1; i < kChains; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[0][e] += c[i][e];
+                const bool in0 = live >> (lane >> 2) & 1u, in1 = live >> ((lane >> 2) + 8) & 1u;
+                float s[4];
+                s[0] = in0 ? c[0][0] * p.scale_log2 : -INFINITY;
+                s[1] = in0 ? c[0][1] * p.scale_log2 : -INFINITY;
+                s[2] = in1 ? c[0][2] * p.scale_log2 : -INFINITY;
+                s[3] = in1 ? c[0][3] * p.scale_log2 : -INFINITY;
+                float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+                }
+                if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+                    float scale[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float now = fmaxf(m[e], top[e]);
+                        scale[e] = now == -INFINITY ? 1.f : exp2_fast(m[e] - now);
+                        m[e] = now;
+                        l[e] *= scale[e];
+                    }
+#pragma unroll
+                    for (int t = 0; t < kSteps; ++t) O[t][0] *= scale[0], O[t][1] *= scale[1], O[t][2] *= scale[0], O[t][3] *= scale[1];
+                }
+                const float ref0 = m[0] == -INFINITY ? 0.f : m[0], ref1 = m[1] == -INFINITY ? 0.f : m[1];  // no key seen yet: all weights are 0
+                s[0] = exp2_fast(s[0] - ref0), s[1] = exp2_fast(s[1] - ref1), s[2] = exp2_fast(s[2] - ref0), s[3] = exp2_fast(s[3] - ref1);
+                l[0] += s[0] + s[2];
+                l[1] += s[1] + s[3];
+                pb0 = transpose8(pack2(s[0], s[1]));
+                pb1 = transpose8(pack2(s[2], s[3]));
+            }
+            rslot = rslot + 1 == kSlots ? 0 : rslot + 1;
+            // ---- values: O^T += V^T P^T
+            asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+            __syncwarp();
+            if (n + kSlots < requests) request(n + kSlots, wslot, b, kvh, first, end);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            wslot = wslot + 1 == kSlots ? 0 : wslot + 1;
+            {
+                const uint32_t row = ring + rslot * kSlotBytes + ((lane >> 4) * 8 + (lane & 7)) * (D * 2);
+#pragma unroll
+                for (int t = 0; t < kSteps; ++t) {
+                    uint32_t a[4];
+                    ldsm4_t(a, row + (((2 * t + (lane >> 3 & 1)) ^ (lane & 7)) << 4));
+                    mma16816(O[t], a, pb0, pb1);
+                }
+            }
+            rslot = rslot + 1 == kSlots ? 0 : rslot + 1;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+            l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+        }
+    }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const PagedParams p) {
+    using Pass = WarpPass<D>;
+    extern __shared__ __align__(128) uint8_t ring_smem[];
+    float* stage = reinterpret_cast<float*>(ring_smem);  // [warp][head][D + 4], after the rings have been read
+    constexpr int kStage = D + 4;                        // keeps the four head columns of a store on different banks
+    __shared__ uint32_t masks[kWarps][Pass::kSlots];
+    __shared__ float tops[kWarps][kHeads], sums[kWarps][kHeads], weights[kWarps][kHeads], top_all[kHeads], sum_all[kHeads];
+    __shared__ long long warp_units[kWarps + 1];
+    __shared__ long long begin_at;
+    __shared__ int begin_row;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int cta = blockIdx.x, ctas = gridDim.x;
+
+    // ---- rows without a key: zeros
+    for (int b = cta * kWarps + warp; b < p.num_seqs; b += ctas * kWarps)
+        if (row_length(p, b, lane == 0) == 0)
+            for (int i = lane * 8; i < p.heads * D; i += 256) *reinterpret_cast<uint4*>(p.out + b * p.ldo + i) = make_uint4(0, 0, 0, 0);
+
+    // ---- this CTA's range of units
+    auto units_of = [&](int b) { return static_cast<long long>((row_length(p, b, false) + kUnit - 1) / kUnit) * p.spans_per_row; };
+    const int per = (p.num_seqs + kThreads - 1) / kThreads;
+    const int rb = min(tid * per, p.num_seqs), re = min(rb + per, p.num_seqs);
+    long long mine = 0;
+    for (int b = rb; b < re; ++b) mine += units_of(b);
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += t;
+    }
+    if (lane == 31) warp_units[warp] = upto;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += warp_units[w];
+        total += warp_units[w];
+    }
+    const int workers = static_cast<int>(min(static_cast<long long>(ctas), total));  // each gets one unit at least
+    if (cta >= workers) {
+        if (tid == 0) p.records[cta] = make_int4(0, 0, -1, 0);
+        return;
+    }
+    const long long first = total * cta / workers, last = total * (cta + 1) / workers;
+    const long long at = before + upto - mine;
+    if (first >= at && first < at + mine) {
+        long long u = at;
+        int b = rb;
+        for (long long n; u + (n = units_of(b)) <= first; ++b) u += n;
+        begin_row = b;
+        begin_at = first - u;
+    }
+    __syncthreads();
+    int b = begin_row;
+    long long r = begin_at;
+    int4 record = make_int4(0, 0, -1, 0);
+    Pass pass(p, lane, smem_u32(ring_smem) + warp * kRingBytes, masks[warp]);
+
+    for (long long unit = first; unit < last;) {
+        const int len = row_length(p, b, false), units = (len + kUnit - 1) / kUnit;  // of one span of the row
+        if (r >= static_cast<long long>(units) * p.spans_per_row) {
+            ++b;
+            r = 0;
+            continue;
+        }
+        const int span = static_cast<int>(r / units), u0 = static_cast<int>(r % units);
+        const int n = static_cast<int>(min(static_cast<long long>(units - u0), last - unit));
+        const int kvh = span / p.blocks_per_group, hb = span % p.blocks_per_group;
+        const int h0 = kvh * p.group + hb * kHeads, nh = min(kHeads, p.group - hb * kHeads);
+        uint32_t qf[Pass::kSteps][2];
+        {
+            const __nv_bfloat16* q = p.q + b * p.ldq + (h0 + min(lane >> 2, nh - 1)) * p.q_head_stride + 2 * (lane & 3);
+            const bool there = (lane >> 2) < nh;
+#pragma unroll
+            for (int s = 0; s < Pass::kSteps; ++s) {
+                qf[s][0] = there ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * s)) : 0u;
+                qf[s][1] = there ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * s + 8)) : 0u;
+            }
+        }
+        pass.run(b, kvh, qf, u0 * kUnit + warp * kTile, min(len, (u0 + n) * kUnit));
+        __syncthreads();  // every ring has been read
+        {
+            float* st = stage + warp * kHeads * kStage + 2 * (lane & 3) * kStage + (lane >> 2);
+#pragma unroll
+            for (int s = 0; s < Pass::kSteps; ++s) {
+                st[16 * s] = pass.O[s][0];
+                st[kStage + 16 * s] = pass.O[s][1];
+                st[16 * s + 8] = pass.O[s][2];
+                st[kStage + 16 * s + 8] = pass.O[s][3];
+            }
+            if (lane < 4) {
+                tops[warp][2 * lane] = pass.m[0], tops[warp][2 * lane + 1] = pass.m[1];
+                sums[warp][2 * lane] = pass.l[0], sums[warp][2 * lane + 1] = pass.l[1];
+            }
+        }
+        __syncthreads();
+        if (tid < kHeads) {
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, tops[w][tid]);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = tops[w][tid] == -INFINITY ? 0.f : exp2_fast(tops[w][tid] - top);
+                weights[w][tid] = f;
+                sum += f * sums[w][tid];
+            }
+            top_all[tid] = top;
+            sum_all[tid] = sum;
+        }
+        __syncthreads();
+        const bool whole = u0 == 0 && n == units;
+        float* part = p.parts + (2ll * cta + (u0 == 0 ? 1 : 0)) * (kHeads * (D + 2));
+        for (int i = tid; i < nh * D; i += kThreads) {
+            const int h = i / D, d = i % D;
+            float x = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) x += weights[w][h] * stage[(w * kHeads + h) * kStage + d];
+            if (whole) store_out<D>(p, b, h0 + h, d, sum_all[h] == 0.f ? 0.f : x / sum_all[h]);
+            else part[h * (D + 2) + d] = x;
+        }
+        if (!whole && tid < nh) {
+            part[tid * (D + 2) + D] = top_all[tid];
+            part[tid * (D + 2) + D + 1] = sum_all[tid];
+        }
+        if (!whole && u0 == 0) record = make_int4(b, span, static_cast<int>(((unit + units) * workers - 1) / total), 0);
+        __syncthreads();  // the stage is a ring again
+        r += n;
+        unit += n;
+    }
+    if (tid == 0) p.records[cta] = record;
+}
+
+// Joins the pieces of the span that began in CTA blockIdx.x of the first kernel and went on in the CTAs after it. A thread owns
+// one head dimension of one head.
+template <int D>
+__global__ void __launch_bounds__(256) s1_attention_paged_join_kernel(const PagedParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 rec = p.records[blockIdx.x];
+    if (rec.z < 0) return;
+    const int h = threadIdx.x >> 5, d = blockIdx.y * 32 + (threadIdx.x & 31);
+    const int kvh = rec.y / p.blocks_per_group, hb = rec.y % p.blocks_per_group;
+    if (h >= min(kHeads, p.group - hb * kHeads)) return;
+    constexpr int kPart = kHeads * (D + 2);
+    const float* part = p.parts + (2ll * blockIdx.x + 1) * kPart + h * (D + 2);
+    float top = part[D], sum = part[D + 1], x = part[d];
+    part += kPart;  // piece 0 of the next CTA, then of the ones after it
+#pragma unroll 4
+    for (int c = blockIdx.x + 1; c <= rec.z; ++c, part += 2 * kPart) {
+        const float t = part[D], s = part[D + 1], y = part[d];
+        const float now = fmaxf(top, t);
+        const float f = top == -INFINITY ? 0.f : exp2_fast(top - now), g = t == -INFINITY ? 0.f : exp2_fast(t - now);
+        x = x * f + y * g;
+        sum = sum * f + s * g;
+        top = now;
+    }
+    store_out<D>(p, rec.x, kvh * p.group + hb * kHeads + h, d, sum == 0.f ? 0.f : x / sum);
+}
+
+constexpr int kMaxCtas = 256;  // the workspace's share: more than one CTA per SM of any sm_100 part
+
+size_t workspace_bytes_of(int head_dim) {
+    return sizeof(int4) * kMaxCtas + sizeof(float) * 2 * kMaxCtas * kHeads * static_cast<size_t>(head_dim + 2);
+}
+
+template <int D>
+int launch(s1_ctx* ctx, const PagedParams& p, int ctas) {
+    constexpr int smem = kWarps * kRingBytes;
+    S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    s1_attention_paged_kernel<D><<<ctas, kThreads, smem, ctx->stream>>>(p);
+    S1_CUDA_OK(ctx, cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(ctas, D / 32), cfg.blockDim = dim3(256), cfg.stream = ctx->stream;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    S1_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, s1_attention_paged_join_kernel<D>, p));
+    ctx->launches += 2;
+    return S1_OK;
+}
+
+inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+
+extern "C" size_t s1_attention_paged_workspace(int head_dim) {
+    return head_dim == 64 || head_dim == 128 || head_dim == 256 ? workspace_bytes_of(head_dim) : 0;
+}
+
+extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, long long q_head_stride, const void* k_cache, const void* v_cache,
+                                  int num_pages, int page_size, long long page_stride, long long token_stride, long long head_stride,
+                                  const int32_t* tables, long long ldt, int table_width, const int32_t* lengths, int num_seqs, int heads, int kv_heads,
+                                  int head_dim, float scale, const void* gate, long long ldg, long long gate_head_stride, void* out, long long ldo,
+                                  void* workspace, size_t workspace_bytes) {
+    if (!ctx) return S1_EINVAL;
+    const char* who = "s1_attention_paged";
+    if (!q || !k_cache || !v_cache || !tables || !lengths || !out || !workspace) return s1_fail(ctx, S1_EINVAL, "%s: null pointer", who);
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return s1_fail(ctx, S1_EINVAL, "%s: head_dim must be 64, 128 or 256 (got %d)", who, head_dim);
+    if (num_seqs < 0 || kv_heads < 1 || heads < kv_heads || heads % kv_heads) return s1_fail(ctx, S1_EINVAL, "%s: heads must be a multiple of kv_heads", who);
+    if (!(scale > 0.f) || !(scale < 3.0e38f)) return s1_fail(ctx, S1_EINVAL, "%s: scale must be positive and finite", who);
+    if (num_pages < 1 || page_size < 1 || page_size > 65536 || (page_size & (page_size - 1)))
+        return s1_fail(ctx, S1_EINVAL, "%s: page_size must be a power of two up to 65536 (got %d)", who, page_size);
+    if (static_cast<long long>(table_width) * page_size > (1ll << 30)) return s1_fail(ctx, S1_EINVAL, "%s: block tables of over 2^30 tokens a row", who);
+    if (table_width < 1 || ldt < table_width) return s1_fail(ctx, S1_EINVAL, "%s: bad block tables", who);
+    if (!al16(q) || !al16(k_cache) || !al16(v_cache) || !al16(out) || !al16(workspace) || ((ldq | q_head_stride | page_stride | token_stride | head_stride | ldo) % 8))
+        return s1_fail(ctx, S1_EINVAL, "%s: head rows and the workspace must be 16-byte aligned", who);
+    if (q_head_stride < head_dim || ldq < (heads - 1) * q_head_stride + head_dim || ldo < static_cast<long long>(heads) * head_dim)
+        return s1_fail(ctx, S1_EINVAL, "%s: heads must lie inside a row", who);
+    if (page_stride < head_dim || token_stride < head_dim || head_stride < head_dim) return s1_fail(ctx, S1_EINVAL, "%s: bad cache strides", who);
+    if (gate && (gate_head_stride < head_dim || ldg < (heads - 1) * gate_head_stride + head_dim))
+        return s1_fail(ctx, S1_EINVAL, "%s: gate heads must lie inside a row", who);
+    if (workspace_bytes < workspace_bytes_of(head_dim))
+        return s1_fail(ctx, S1_EINVAL, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, workspace_bytes_of(head_dim));
+    if (num_seqs == 0) return S1_OK;
+    S1DeviceGuard guard(ctx->device);
+    if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
+    const int group = heads / kv_heads, blocks = (group + kHeads - 1) / kHeads;
+    PagedParams p{static_cast<const __nv_bfloat16*>(q), ldq, q_head_stride, static_cast<const __nv_bfloat16*>(k_cache),
+                  static_cast<const __nv_bfloat16*>(v_cache), page_stride, token_stride, head_stride, num_pages, __builtin_ctz(page_size), tables, ldt,
+                  table_width, lengths, num_seqs, heads, kv_heads, group, kv_heads * blocks, blocks, scale * 1.4426950408889634f,
+                  static_cast<const __nv_bfloat16*>(gate), ldg, gate_head_stride, static_cast<__nv_bfloat16*>(out), ldo,
+                  reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas), static_cast<int4*>(workspace), ctx->status_dev};
+    const int ctas = std::min(ctx->sm_count, kMaxCtas);
+    if (head_dim == 64) return launch<64>(ctx, p, ctas);
+    if (head_dim == 128) return launch<128>(ctx, p, ctas);
+    return launch<256>(ctx, p, ctas);
+}

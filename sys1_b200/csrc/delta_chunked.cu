@@ -665,6 +665,11 @@ struct ScanParams {
     float* out;  // [T, H, 128]
     int num_slots, H;
     int* status;
+    // s1_gated_delta_rule_prefill only (state null otherwise): where every sequence's state goes after its last chunk
+    float* state;                  // [num_states, H, 128 (key), 128 (value)]
+    const int32_t* cu_seqlens;     // [num_seqs + 1]
+    const int32_t* state_index;    // [num_seqs], negative: not kept
+    int num_states, num_seqs;
 };
 
 constexpr int kStageBytes = 2 * kTileBytes /*WQ*/ + kTileBytes /*UT*/ + kTileBytes /*K~*/ + kTileBytes / 2 /*P*/;  // 73728
@@ -873,6 +878,31 @@ s1_delta_scan_kernel(const __grid_constant__ CUtensorMap tmWQ, const __grid_cons
             tc_fence_before();
         }
         __syncwarp();
+        if (p.state && !fail) {
+            // which sequence this is: the last one that starts at or before its first token (the tables are sorted by length)
+            const int t0 = p.slots[sq.first_slot].tok_start;
+            int lo = 0, hi = p.num_seqs;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (p.cu_seqlens[mid] <= t0) lo = mid;
+                else hi = mid;
+            }
+            const int where = p.state_index[lo];
+            // a slot that does not exist, or that a sequence before this one has: not written
+            bool bad = where >= p.num_states;
+            for (int j = lane; where >= 0 && j < lo; j += 32) bad = bad || (p.state_index[j] == where && p.cu_seqlens[j + 1] > p.cu_seqlens[j]);
+            bad = __any_sync(0xffffffffu, bad);
+            if (bad && threadIdx.x == 0 && atomicCAS(p.status, 0, 119) == 0) {
+                p.status[1] = blockIdx.x;
+                p.status[2] = lo;
+                p.status[3] = where;
+            }
+            if (where >= 0 && !bad) {
+                float* st = p.state + (static_cast<long long>(where) * p.H + head) * kD * kD + d;
+#pragma unroll
+                for (int j = 0; j < kD; ++j) st[j * kD] = S[j];
+            }
+        }
     }
     if (fail && atomicCAS(p.status, 0, 3) == 0) {
         p.status[1] = blockIdx.x;
@@ -917,8 +947,16 @@ extern "C" size_t s1_delta_rule_chunked_workspace(int num_seqs, int total_tokens
 }
 
 // Shared host path of the two entry points: chunk tables, prep (FUSED or not), scan.
+struct KeptState {  // where s1_gated_delta_rule_prefill leaves the sequences' states (all device pointers)
+    const int32_t* cu_seqlens = nullptr;
+    const int32_t* index = nullptr;
+    int num_states = 0;
+    void* conv_state = nullptr;
+    float* state = nullptr;
+};
+
 static int run_chunked(s1_ctx* ctx, const char* who, PrepParams pp, bool fused, const int32_t* cu_seqlens_host, int num_seqs,
-                       int total_tokens, int heads, float* out, void* workspace, size_t workspace_bytes) {
+                       int total_tokens, int heads, float* out, void* workspace, size_t workspace_bytes, const KeptState& kept = KeptState()) {
     if (num_seqs == 0 || total_tokens == 0) return S1_OK;
     static_assert(sizeof(SlotInfo) == sizeof(S1ChunkSlot) && sizeof(SeqInfo) == sizeof(S1SeqChunks), "the plan's chunk tables have this kernel's layout");
     const S1BatchPlan* plan = cu_seqlens_host ? nullptr : ctx->active_plan(num_seqs, total_tokens);
@@ -1000,7 +1038,9 @@ static int run_chunked(s1_ctx* ctx, const char* who, PrepParams pp, bool fused, 
     if (rc) return rc;
     rc = s1_get_tmap(ctx, pp.p, hs_rows * 64, 64, 64, 64, 64, 2, 128, &tP);
     if (rc) return rc;
-    ScanParams sp;
+    ScanParams sp = {};
+    sp.state = kept.state, sp.cu_seqlens = kept.cu_seqlens, sp.state_index = kept.index;
+    sp.num_states = kept.num_states, sp.num_seqs = num_seqs;
     sp.seqs = seqs_dev;
     sp.slots = pp.slots;
     sp.decay = pp.decay;
@@ -1045,7 +1085,7 @@ static int gated_delta_rule(s1_ctx* ctx, const char* who, const void* mixed, lon
                             const int32_t* positions, const void* b_proj, const void* a_proj, long long ldba, const float* dt_bias,
                             const float* neg_exp_a, const void* z, long long ldz, const void* norm_weight, float eps,
                             const int32_t* cu_seqlens_host, int num_seqs, int total_tokens, int key_heads, int value_heads, void* y,
-                            long long ldy, void* workspace, size_t workspace_bytes) {
+                            long long ldy, void* workspace, size_t workspace_bytes, const KeptState& kept = KeptState()) {
     if (!ctx) return S1_EINVAL;
     if (!mixed || !b_proj || !a_proj || !dt_bias || !neg_exp_a || !z || !norm_weight || !y || !workspace)
         return s1_fail(ctx, S1_EINVAL, "%s: null pointer", who);
@@ -1070,8 +1110,12 @@ static int gated_delta_rule(s1_ctx* ctx, const char* who, const void* mixed, lon
     pp.bproj = static_cast<const __nv_bfloat16*>(b_proj), pp.aproj = static_cast<const __nv_bfloat16*>(a_proj), pp.ldba = ldba;
     pp.dt_bias = dt_bias, pp.neg_exp_a = neg_exp_a, pp.Hk = key_heads;
     int rc = run_chunked(ctx, who, pp, true, cu_seqlens_host, num_seqs, total_tokens, value_heads, o,
-                         static_cast<uint8_t*>(workspace) + obytes, workspace_bytes - obytes);
+                         static_cast<uint8_t*>(workspace) + obytes, workspace_bytes - obytes, kept);
     if (rc) return rc;
+    if (kept.state) {
+        rc = s1_conv_state_launch(ctx, mixed, ldm, kept.cu_seqlens, num_seqs, kept.index, kept.num_states, static_cast<int>(width), kept.conv_state);
+        if (rc) return rc;
+    }
     return s1_delta_finish(ctx, o, z, ldz, norm_weight, eps, total_tokens, value_heads, y, ldy);
 }
 
@@ -1095,6 +1139,26 @@ extern "C" int s1_gated_delta_rule_conv(s1_ctx* ctx, const void* mixed_before_co
     return gated_delta_rule(ctx, "s1_gated_delta_rule_conv", mixed_before_conv, ldm, conv_weight, positions, b_proj, a_proj, ldba, dt_bias,
                             neg_exp_a, z, ldz, norm_weight, eps, cu_seqlens_host, num_seqs, total_tokens, key_heads, value_heads, y, ldy,
                             workspace, workspace_bytes);
+}
+
+extern "C" int s1_gated_delta_rule_prefill(s1_ctx* ctx, const void* mixed_before_conv, long long ldm, const void* conv_weight,
+                                           const int32_t* positions, const void* b_proj, const void* a_proj, long long ldba,
+                                           const float* dt_bias, const float* neg_exp_a, const void* z, long long ldz,
+                                           const void* norm_weight, float eps, const int32_t* cu_seqlens_host, int num_seqs,
+                                           int total_tokens, int key_heads, int value_heads, void* y, long long ldy, void* workspace,
+                                           size_t workspace_bytes, const int32_t* cu_seqlens, const int32_t* state_index, int num_states,
+                                           void* conv_state, float* state) {
+    const char* who = "s1_gated_delta_rule_prefill";
+    if (!ctx) return S1_EINVAL;
+    if (!conv_weight || !positions || !cu_seqlens || !state_index || !conv_state || !state) return s1_fail(ctx, S1_EINVAL, "%s: null pointer", who);
+    if (num_states < 1 || num_seqs > 65535) return s1_fail(ctx, S1_EINVAL, "%s: %d sequences, %d states", who, num_seqs, num_states);
+    if ((reinterpret_cast<uintptr_t>(conv_state) | reinterpret_cast<uintptr_t>(state)) & 15u)
+        return s1_fail(ctx, S1_EINVAL, "%s: the states must be 16-byte aligned", who);
+    KeptState kept;
+    kept.cu_seqlens = cu_seqlens, kept.index = state_index, kept.num_states = num_states, kept.conv_state = conv_state, kept.state = state;
+    return gated_delta_rule(ctx, who, mixed_before_conv, ldm, conv_weight, positions, b_proj, a_proj, ldba, dt_bias, neg_exp_a, z, ldz,
+                            norm_weight, eps, cu_seqlens_host, num_seqs, total_tokens, key_heads, value_heads, y, ldy, workspace,
+                            workspace_bytes, kept);
 }
 
 #ifdef S1_MEASURE

@@ -15,6 +15,9 @@
 #include <stdint.h>
 
 #include "context.h"
+#include "head_norm_rope.cuh"
+
+using namespace s1;
 
 namespace {
 
@@ -33,33 +36,6 @@ struct NormParams {
     int width;
     int* status;
 };
-
-__device__ __forceinline__ void unpack8(const uint4& raw, float* f) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float2 t = __bfloat1622float2(h[e]);
-        f[2 * e] = t.x;
-        f[2 * e + 1] = t.y;
-    }
-}
-
-__device__ __forceinline__ uint4 pack8(const float* f) {
-    uint4 raw;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
-    return raw;
-}
-
-__device__ __forceinline__ float bf16r(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
-
-template <int LPR>
-__device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int off = LPR / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    return v;
-}
 
 __device__ __forceinline__ const __nv_bfloat16* norm_row(const NormParams& p, long long row, bool& live) {
     long long r = row;
@@ -263,58 +239,17 @@ __global__ void __launch_bounds__(256) s1_head_norm_rope_kernel(__nv_bfloat16* _
     const bool pos_ok = pos >= 0 && pos < max_pos;
     float c[8], sn[8];
     if (rotates && pos_ok) {
-        const long long tb = static_cast<long long>(pos) * (rot / 2) + (sub % halfc) * 8;
-        *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cos_t + tb));
-        *reinterpret_cast<float4*>(c + 4) = __ldg(reinterpret_cast<const float4*>(cos_t + tb) + 1);
-        *reinterpret_cast<float4*>(sn) = __ldg(reinterpret_cast<const float4*>(sin_t + tb));
-        *reinterpret_cast<float4*>(sn + 4) = __ldg(reinterpret_cast<const float4*>(sin_t + tb) + 1);
+        load_rotation(cos_t, sin_t, pos, rot, sub, c, sn);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f;
     }
-    float f[8];
-    unpack8(raw, f);
-    float sq = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sq += f[e] * f[e];
-    const float rstd = 1.f / sqrtf(group_sum<LPR>(sq) * (1.f / static_cast<float>(8 * LPR)) + eps);
-    float g[8];
-    unpack8(__ldg(reinterpret_cast<const uint4*>(w + sub * 8)), g);
-    uint4 normed;
-    {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = f[e] * rstd * (g[e] + 1.f);
-        normed = pack8(y);
-        unpack8(normed, f);  // the bf16 values the rotation starts from
-    }
-    // the partner half of the rotated span sits rot / 16 lanes away (every lane takes part in the exchange)
-    uint4 other_raw;
-    other_raw.x = __shfl_xor_sync(0xffffffffu, normed.x, halfc);
-    other_raw.y = __shfl_xor_sync(0xffffffffu, normed.y, halfc);
-    other_raw.z = __shfl_xor_sync(0xffffffffu, normed.z, halfc);
-    other_raw.w = __shfl_xor_sync(0xffffffffu, normed.w, halfc);
+    const uint4 normed = head_norm_rope<LPR>(raw, w, eps, c, sn, rotates && pos_ok, sub, halfc, bf16_ops);
     if (!live) return;
-    if (rotates) {
-        if (!pos_ok) {
-            if (atomicCAS(status, 0, 102) == 0) {
-                status[1] = static_cast<int>(blockIdx.x);
-                status[2] = static_cast<int>(t);
-                status[3] = pos;
-            }
-        } else {
-            float o[8];
-            unpack8(other_raw, o);
-            const bool is_lo = sub < halfc;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float own_c = __fmul_rn(f[e], c[e]);
-                const float oth_s = __fmul_rn(is_lo ? -o[e] : o[e], sn[e]);  // rotate_half = [-second, first]
-                if (bf16_ops) f[e] = __fadd_rn(bf16r(own_c), bf16r(oth_s));
-                else f[e] = is_lo ? __fsub_rn(own_c, __fmul_rn(o[e], sn[e])) : __fadd_rn(__fmul_rn(o[e], sn[e]), own_c);
-            }
-            normed = pack8(f);
-        }
+    if (rotates && !pos_ok && atomicCAS(status, 0, 102) == 0) {
+        status[1] = static_cast<int>(blockIdx.x);
+        status[2] = static_cast<int>(t);
+        status[3] = pos;
     }
     *reinterpret_cast<uint4*>(ptr) = normed;
 }

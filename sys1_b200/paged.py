@@ -1,0 +1,298 @@
+"""One new token at a time: the paged key-value cache and the recurrent states that let the decoder go on from where a
+prompt ended (`s1_block_tables`, `s1_release_blocks`, `s1_cache_write`, `s1_attention_paged`, and the states of
+`s1_gated_delta_rule_prefill` / `s1_gated_delta_rule_step`).
+
+The reference keeps no cache (`Decoder::forward`, src/archs/qwen35_text.rs:942-1005, runs whole prompts). `PagedCache` holds the
+memory of a fixed number of rows (requests in flight); `qwen35.Decoder.prefill` enters prompts into it and
+`qwen35.Decoder.step` moves every row one token further. The functions are the calls of the C ABI on tensors.
+"""
+from __future__ import annotations
+
+from typing import List, NamedTuple, Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import device
+
+
+class BlockTables(NamedTuple):
+    """What `block_tables` returns (int32 CUDA tensors): tokens a row holds now `[rows]`, first token of every row
+    `[rows + 1]`, position and slot of every token `[max_tokens]` and the pages left `[1]`."""
+    lengths: torch.Tensor
+    cu_seqlens: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    free_count: torch.Tensor
+
+
+def _ints(t: torch.Tensor, dev: int, shape, name: str) -> int:
+    if t.get_device() != dev or dev < 0 or t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor on the call's GPU (no CPU fallback)")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _table(t: torch.Tensor, dev: int, rows: int) -> int:
+    if t.get_device() != dev or dev < 0 or t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.shape[0] != rows:
+        raise ValueError(f"block tables must be an int32 CUDA tensor [{rows}, pages] with contiguous rows")
+    return t.data_ptr()
+
+
+def _heads(t: torch.Tensor, dev: int, shape, name: str) -> int:
+    if t.get_device() != dev or dev < 0 or t.dtype != torch.bfloat16 or t.dim() != 3 or t.stride(2) != 1:
+        raise ValueError(f"{name} must be a bf16 CUDA tensor [tokens, heads, head_dim] with contiguous head rows (no CPU fallback)")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _caches(k: torch.Tensor, v: torch.Tensor, dev: int):
+    for name, t in (("k_cache", k), ("v_cache", v)):
+        if t.get_device() != dev or dev < 0 or t.dtype != torch.bfloat16 or t.dim() != 4 or t.stride(3) != 1:
+            raise ValueError(f"{name} must be a bf16 CUDA tensor [pages, page_size, kv_heads, head_dim] with contiguous head rows (no CPU fallback)")
+    if k.shape != v.shape or k.stride() != v.stride():
+        raise ValueError("k_cache and v_cache must have the same shape and strides")
+    return k.shape, k.stride()
+
+
+def block_tables(cached: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
+                 added: Optional[torch.Tensor] = None, max_tokens: Optional[int] = None, lengths: Optional[torch.Tensor] = None,
+                 free_count_out: Optional[torch.Tensor] = None, ctx: Optional[device.Context] = None) -> BlockTables:
+    """Pages, positions and slots for the tokens that a step adds (`s1_block_tables`): `cached` int32 `[rows]` tokens each row holds
+    (negative: idle), `added` int32 `[rows]` tokens it gets (None: one each), `free_pages` / `free_count` `[1]` the stack that new
+    pages are taken from, `tables` int32 `[rows, width]` updated in place. `max_tokens`: tokens of the packed batch, with those
+    behind the last row (needed with `added`). `lengths` may be `cached` and `free_count_out` may be `free_count`: both are then
+    advanced in place."""
+    dev, rows = cached.get_device(), cached.shape[0] if cached.dim() == 1 else -1
+    args = [_ints(cached, dev, (rows,), "cached"), 0 if added is None else _ints(added, dev, (rows,), "added"), rows, page_size,
+            _ints(free_pages, dev, (free_pages.numel(),), "free_pages"), free_pages.numel(), _ints(free_count, dev, (1,), "free_count")]
+    tp = _table(tables, dev, rows)
+    if max_tokens is None:
+        if added is not None:
+            raise ValueError("max_tokens is needed with `added`: the host knows how many tokens the batch has")
+        max_tokens = rows
+    if max_tokens < 0:
+        raise ValueError("max_tokens must not be negative")
+    out = torch.empty(2 * rows + 2 + 2 * max_tokens, dtype=torch.int32, device=cached.device)
+    new_lengths, cu, positions, slots, count = out.split_with_sizes((rows, rows + 1, max_tokens, max_tokens, 1))
+    if lengths is not None:
+        _ints(lengths, dev, (rows,), "lengths")
+        new_lengths = lengths
+    if free_count_out is not None:
+        _ints(free_count_out, dev, (1,), "free_count_out")
+        count = free_count_out
+    if ctx is None:
+        ctx = device.load(dev)
+    ctx.check(ctx._lib.s1_block_tables(ctx.handle, *args, count.data_ptr(), tp, tables.stride(0), tables.shape[1], new_lengths.data_ptr(),
+                                       cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), max_tokens))
+    return BlockTables(new_lengths, cu, positions, slots, count)
+
+
+def release_blocks(ended: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                   page_size: int, ctx: Optional[device.Context] = None) -> None:
+    """Puts the pages of every row with `ended[row] != 0` back on the stack and makes the row idle (`s1_release_blocks`)."""
+    dev, rows = lengths.get_device(), lengths.shape[0] if lengths.dim() == 1 else -1
+    args = (_ints(ended, dev, (rows,), "ended"), rows, page_size, _ints(lengths, dev, (rows,), "lengths"), _table(tables, dev, rows), tables.stride(0),
+            tables.shape[1], _ints(free_pages, dev, (free_pages.numel(),), "free_pages"), free_pages.numel(), _ints(free_count, dev, (1,), "free_count"))
+    if ctx is None:
+        ctx = device.load(dev)
+    ctx.check(ctx._lib.s1_release_blocks(ctx.handle, *args))
+
+
+def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                positions: Optional[torch.Tensor] = None, rotary_dim: int = 0, bf16_ops: bool = True, ctx: Optional[device.Context] = None) -> None:
+    """Keys and values `[T, kv_heads, head_dim]` (rows may be strided) into the slots of `k_cache`, `v_cache` `[pages, page_size,
+    kv_heads, head_dim]` (`s1_cache_write`); a token with slot -1 is left out. With `norm_weight` `[head_dim]` the keys are normed and
+    rotated on the way, as `norm.head_norm_rope_` would do in place (`cos`, `sin` f32 `[positions, rotary_dim / 2]`)."""
+    dev = k.get_device()
+    (pages, page, kv, dim), (ps, ts, hs, _) = _caches(k_cache, v_cache, dev)
+    T = k.shape[0]
+    kp, vp, sp = _heads(k, dev, (T, kv, dim), "k"), _heads(v, dev, (T, kv, dim), "v"), _ints(slots, dev, (T,), "slots")
+    wp = cp = np_ = pp = rows = 0
+    if norm_weight is not None:
+        if cos is None or sin is None or positions is None:
+            raise ValueError("keys that are normed are rotated too: cos, sin and positions are needed")
+        if norm_weight.get_device() != dev or norm_weight.dtype != torch.bfloat16 or tuple(norm_weight.shape) != (dim,) or not norm_weight.is_contiguous():
+            raise ValueError(f"norm_weight must be a contiguous bf16 CUDA tensor [{dim}]")
+        for t in (cos, sin):
+            if t.get_device() != dev or t.dtype != torch.float32 or t.shape != cos.shape or t.dim() != 2 or t.shape[1] != rotary_dim // 2 or not t.is_contiguous():
+                raise ValueError("cos and sin must be contiguous f32 CUDA tensors [positions, rotary_dim / 2]")
+        wp, cp, np_, pp, rows = norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ints(positions, dev, (T,), "positions"), cos.shape[0]
+    if T == 0:
+        return
+    if ctx is None:
+        ctx = device.load(dev)
+    ctx.check(ctx._lib.s1_cache_write(ctx.handle, kp, k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1), sp, T, kv, dim, wp, eps, cp, np_, pp,
+                                      rows, rotary_dim, 1 if bf16_ops else 0, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs))
+
+
+def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
+                    gate: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None, ctx: Optional[device.Context] = None) -> torch.Tensor:
+    """Attention of one new token per row over the first `lengths[row]` tokens of its block table (`s1_attention_paged`): q `[rows,
+    heads, head_dim]` (rows may be strided), optional gate of the same shape (pre-sigmoid). Rows of length <= 0 get zeros. Returns
+    `[rows, heads * head_dim]`. `workspace`: uint8 CUDA tensor of `attention_paged_workspace(head_dim)` bytes; by default the
+    context's own, which the calls of one stream share. Calls captured into graphs should be given one that lives as long as
+    the graph, and graphs that may run at the same time one each."""
+    dev = q.get_device()
+    (pages, page, kv, dim), (ps, ts, hs, _) = _caches(k_cache, v_cache, dev)
+    B, H = q.shape[0], q.shape[1]
+    qp, tp, lp = _heads(q, dev, (B, H, dim), "q"), _table(tables, dev, B), _ints(lengths, dev, (B,), "lengths")
+    gp = ldg = gs = 0
+    if gate is not None:
+        gp, ldg, gs = _heads(gate, dev, (B, H, dim), "gate"), gate.stride(0), gate.stride(1)
+    if out is None:
+        out = torch.empty((B, H * dim), dtype=torch.bfloat16, device=q.device)
+    elif out.get_device() != dev or out.dtype != torch.bfloat16 or tuple(out.shape) != (B, H * dim) or out.stride(1) != 1:
+        raise ValueError(f"out must be a bf16 CUDA tensor [{B}, {H * dim}] with contiguous rows")
+    if B == 0:
+        return out
+    if ctx is None:
+        ctx = device.load(dev)
+    need = ctx._lib.s1_attention_paged_workspace(dim)
+    if workspace is None:
+        workspace = ctx.workspace(need)
+    elif workspace.get_device() != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("the workspace must be a contiguous uint8 CUDA tensor")
+    ctx.check(ctx._lib.s1_attention_paged(ctx.handle, qp, q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs, tp,
+                                          tables.stride(0), tables.shape[1], lp, B, H, kv, dim, dim ** -0.5 if scale is None else scale, gp, ldg, gs,
+                                          out.data_ptr(), out.stride(0), workspace.data_ptr(), workspace.numel()))
+    return out
+
+
+def attention_paged_workspace(head_dim: int) -> int:
+    """Bytes of workspace that `attention_paged` needs, whatever the batch."""
+    from ._lib import load_library
+    return int(load_library().s1_attention_paged_workspace(int(head_dim)))
+
+
+# ------------------------------------------------------------------------------------------------ the decoder's cache
+class KvPages(NamedTuple):
+    """A full-attention layer's cache: `[pages, page_size, kv_heads, head_dim]` bf16 each."""
+    k: torch.Tensor
+    v: torch.Tensor
+
+
+class DeltaState(NamedTuple):
+    """A linear-attention layer's states: `[rows, 4, channels]` bf16 (the conv's last inputs) and `[rows, value_heads, 128, 128]` f32."""
+    conv: torch.Tensor
+    state: torch.Tensor
+
+
+class PagedCache:
+    """The memory of up to `rows` requests in flight for a decoder of configuration `cfg` (see `qwen35.Decoder`): `num_pages` pages of
+    `page_size` tokens that the rows share, at most `max_length` tokens a row, and one recurrent state a row and layer.
+
+    `admit(n)` picks idle rows, `Decoder.prefill` fills them, `Decoder.step` adds a token to every active row, `release(rows)`
+    gives their pages back. The bookkeeping lives on the GPU (`lengths`, `tables`, `free_pages`, `free_count`), so that a captured
+    step can be replayed; `held` and `pages_left` mirror it on the host, where a request that does not fit is refused before
+    anything is launched. After replaying a captured step, tell the mirror with `advanced(steps)`."""
+
+    def __init__(self, cfg, rows: int, num_pages: int, page_size: int = 64, max_length: int = 8192, dev="cuda"):
+        if rows < 1 or num_pages < 1 or max_length < 1 or page_size < 1 or page_size & (page_size - 1):
+            raise ValueError("rows, num_pages and max_length must be positive, page_size a power of two")
+        self.rows, self.num_pages, self.page_size, self.max_length = int(rows), int(num_pages), int(page_size), int(max_length)
+        dev = torch.device(dev)
+        if dev.type != "cuda":
+            raise ValueError("the cache lives on a GPU (no CPU fallback)")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.device = dev
+        i32 = dict(dtype=torch.int32, device=dev)
+        width = -(-max_length // page_size)
+        self.tables = torch.zeros((rows, width), **i32)
+        self.lengths = torch.full((rows,), -1, **i32)
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, **i32)
+        self.free_count = torch.full((1,), num_pages, **i32)
+        self.state_index = torch.full((rows,), -1, **i32)
+        self.held = np.full(rows, -1, dtype=np.int64)
+        self.pages_left = int(num_pages)
+        channels = (2 * cfg.linear_num_key_heads + cfg.linear_num_value_heads) * 128
+        self.layers: List = []
+        for i in range(cfg.num_hidden_layers):
+            if cfg.layer_type(i) == "full_attention":
+                shape = (num_pages, page_size, cfg.num_key_value_heads, cfg.head_dim)
+                self.layers.append(KvPages(*(torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))))
+            else:
+                self.layers.append(DeltaState(torch.empty((rows, 4, channels), dtype=torch.bfloat16, device=dev),
+                                              torch.empty((rows, cfg.linear_num_value_heads, 128, 128), dtype=torch.float32, device=dev)))
+        self.workspace = torch.empty(attention_paged_workspace(cfg.head_dim), dtype=torch.uint8, device=dev)
+
+    def _pages(self, tokens) -> int:
+        return -(-int(tokens) // self.page_size)
+
+    @property
+    def active(self) -> List[int]:
+        return [int(r) for r in np.flatnonzero(self.held >= 0)]
+
+    def admit(self, lengths: Sequence[int]) -> List[int]:
+        """Idle rows for prompts of these lengths, in ascending order (the order of the packed batch); refuses what does not fit."""
+        idle = np.flatnonzero(self.held < 0)
+        if len(lengths) > len(idle):
+            raise ValueError(f"{len(lengths)} prompts, {len(idle)} idle rows")
+        if any(n < 1 or n > self.max_length for n in lengths):
+            raise ValueError(f"prompts must have 1 to {self.max_length} tokens")
+        need = sum(self._pages(n) for n in lengths)
+        if need > self.pages_left:
+            raise ValueError(f"the prompts need {need} pages, {self.pages_left} are left")
+        return [int(r) for r in idle[:len(lengths)]]
+
+    def enter(self, rows: Sequence[int], lengths: Sequence[int]) -> BlockTables:
+        """Takes pages for the prompts of `rows` (from `admit`); the tokens of the packed batch follow one another in that order."""
+        if len(rows) != len(lengths) or list(rows) != sorted(set(rows)) or any(not 0 <= r < self.rows or self.held[r] >= 0 for r in rows):
+            raise ValueError("rows must be different idle rows in ascending order, one for each length")
+        if any(n < 1 or n > self.max_length for n in lengths) or sum(self._pages(n) for n in lengths) > self.pages_left:
+            raise ValueError("the prompts do not fit the cache")
+        added, index = np.zeros(self.rows, np.int32), self.held >= 0
+        added[list(rows)], index[list(rows)] = lengths, True
+        start = np.where(added > 0, 0, -1).astype(np.int32)  # lengths that change: the new rows' only
+        state = np.where(index, np.arange(self.rows), -1).astype(np.int32)
+        added_dev, start_dev, state_dev = torch.from_numpy(np.stack([added, start, state])).to(self.device)
+        self.lengths.copy_(torch.maximum(self.lengths, start_dev))
+        self.state_index.copy_(state_dev)
+        plan = block_tables(self.lengths, self.tables, self.free_pages, self.free_count, self.page_size, added=added_dev, max_tokens=int(sum(lengths)),
+                            lengths=self.lengths, free_count_out=self.free_count)
+        for r, n in zip(rows, lengths):
+            self.held[r] = n
+            self.pages_left -= self._pages(n)
+        return plan
+
+    def extend(self) -> BlockTables:
+        """One more token for every active row. Token r of the step belongs to row r; idle rows have slot -1."""
+        if not torch.cuda.is_current_stream_capturing():
+            self.advanced(1)
+        return block_tables(self.lengths, self.tables, self.free_pages, self.free_count, self.page_size, lengths=self.lengths,
+                            free_count_out=self.free_count)
+
+    def fits(self, steps: int = 1) -> bool:
+        """Whether every active row can grow by `steps` tokens."""
+        live = self.held[self.held >= 0]
+        need = sum(self._pages(n + steps) - self._pages(n) for n in live)
+        return need <= self.pages_left and (len(live) == 0 or int(live.max()) + steps <= self.max_length)
+
+    def advanced(self, steps: int = 1) -> None:
+        """Notes on the host that every active row has `steps` more tokens; refuses steps that do not fit. (`Decoder.step` calls it;
+        call it yourself before replaying a captured step.)"""
+        if not self.fits(steps):
+            raise ValueError(f"{steps} more token(s) do not fit: {self.pages_left} pages left, rows of up to {self.max_length} tokens")
+        live = self.held >= 0
+        self.pages_left -= sum(self._pages(n + steps) - self._pages(n) for n in self.held[live])
+        self.held[live] += steps
+
+    def release(self, rows: Sequence[int]) -> None:
+        """Ends the requests of `rows`: their pages go back, the rows are idle."""
+        rows = sorted(set(int(r) for r in rows))
+        if any(not 0 <= r < self.rows or self.held[r] < 0 for r in rows):
+            raise ValueError("only active rows can be released")
+        ended = np.zeros(self.rows, np.int32)
+        ended[rows] = 1
+        index = np.where((self.held >= 0) & (ended == 0), np.arange(self.rows), -1).astype(np.int32)
+        ended_dev, index_dev = torch.from_numpy(np.stack([ended, index])).to(self.device)
+        self.state_index.copy_(index_dev)
+        release_blocks(ended_dev, self.lengths, self.tables, self.free_pages, self.free_count, self.page_size)
+        for r in rows:
+            self.pages_left += self._pages(self.held[r])
+            self.held[r] = -1

@@ -7,12 +7,14 @@ names on a token-packed batch. Everything runs through the C ABI.
 from __future__ import annotations
 
 import ctypes as C
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
 
 from . import device
 from . import norm as _norm
+from . import paged
 from ._lib import EPI_SWIGLU
 from .linear import Linear, fused_linear
 
@@ -182,13 +184,23 @@ class LinearAttention:
         return tuple(outs)
 
     def forward(self, x: torch.Tensor, cu_seqlens_host, positions: torch.Tensor, residual: Optional[torch.Tensor] = None,
-                inplace: bool = False) -> torch.Tensor:
-        y = self.mix(x, cu_seqlens_host, positions)
+                inplace: bool = False, kept: Optional["Kept"] = None) -> torch.Tensor:
+        y = self.mix(x, cu_seqlens_host, positions, kept)
         return self.output.forward(y, residual=residual, out=residual if inplace else None)  # out_proj (+ the layer's residual, :938)
 
-    def mix(self, x: torch.Tensor, cu_seqlens_host, positions: torch.Tensor) -> torch.Tensor:
-        """Everything up to the input of `out_proj`: `[T, value_heads * 128]` bf16."""
+    def step(self, x: torch.Tensor, kept: "Kept", residual: Optional[torch.Tensor] = None, inplace: bool = False) -> torch.Tensor:
+        """One new token of every row (`x [rows, hidden]`) on the states in `kept.layer`, which it moves on."""
+        pre, zz, bb, aa = self._inputs(x)
+        y = gated_delta_rule_step(pre, self.conv_taps, kept.positions, bb, aa, self.dt_bias, self.decay, zz, self.norm, self.eps,
+                                  kept.layer.conv, kept.layer.state, self.key_heads, state_index=kept.state_index)
+        return self.output.forward(y, residual=residual, out=residual if inplace else None)
+
+    def mix(self, x: torch.Tensor, cu_seqlens_host, positions: torch.Tensor, kept: Optional["Kept"] = None) -> torch.Tensor:
+        """Everything up to the input of `out_proj`: `[T, value_heads * 128]` bf16. `kept`: leaves the sequences' states there
+        (`s1_gated_delta_rule_prefill`, same output)."""
         import numpy as np
+        if kept is not None and not self.fuse_conv:
+            raise ValueError("states are kept by the chunked recurrence with the conv inside (recurrence='chunked', fuse_conv, 4 taps)")
         ctx = device.load(x.device.index)
         T = x.shape[0]
         cu = np.ascontiguousarray(cu_seqlens_host, dtype=np.int32)
@@ -205,7 +217,11 @@ class LinearAttention:
         offsets = None if planned else cu.ctypes.data_as(C.POINTER(C.c_int32))
         tail = (P(bb), P(aa), bb.stride(0), P(self.dt_bias), P(self.decay), P(zz), zz.stride(0), P(self.norm), C.c_float(self.eps), offsets,
                 len(cu) - 1, T, self.key_heads, self.value_heads, P(y), y.stride(0), C.c_void_p(ptr), need)
-        if self.fuse_conv:
+        if kept is not None:
+            conv, state = kept.layer
+            rc = ctx._lib.s1_gated_delta_rule_prefill(ctx.handle, P(pre), pre.stride(0), P(self.conv_taps), P(positions), *tail, P(kept.cu_seqlens),
+                                                      P(kept.state_index), state.shape[0], P(conv), P(state))
+        elif self.fuse_conv:
             pos = positions if positions.dtype == torch.int32 and positions.is_contiguous() else positions.to(torch.int32).contiguous()
             rc = ctx._lib.s1_gated_delta_rule_conv(ctx.handle, P(pre), pre.stride(0), P(self.conv_taps), P(pos), *tail)
         else:
@@ -228,6 +244,53 @@ class LinearAttention:
         o = delta_rule_packed(q, k, v, g, beta, cu_dev, ctx)
         ctx.check(ctx._lib.s1_delta_finish(ctx.handle, P(o), P(zz), zz.stride(0), P(self.norm), C.c_float(self.eps), T, Hv,
                                            P(y), y.stride(0)))
+
+
+def gated_delta_rule_step(mixed: torch.Tensor, conv_weight: torch.Tensor, positions: torch.Tensor, b: torch.Tensor, a: torch.Tensor,
+                          dt_bias: torch.Tensor, neg_exp_a: torch.Tensor, z: torch.Tensor, norm_weight: torch.Tensor, eps: float,
+                          conv_state: torch.Tensor, state: torch.Tensor, key_heads: int, state_index: Optional[torch.Tensor] = None,
+                          out: Optional[torch.Tensor] = None, ctx: Optional[device.Context] = None) -> torch.Tensor:
+    """The linear-attention layer between its projections for one new token of each row (`s1_gated_delta_rule_step`): mixed
+    `[rows, C]` bf16 before the conv, conv_weight `[C, 4]` (or `[C, 1, 4]`), b, a `[rows, value_heads]`, z `[rows, value_heads * 128]`,
+    positions int32 `[rows]`, dt_bias, neg_exp_a f32 `[value_heads]`. `conv_state` bf16 `[states, 4, C]` and `state` f32 `[states,
+    value_heads, 128, 128]` are updated in place; row r has state `state_index[r]` (int32, -1: none, its output is zero; None: r).
+    Returns `[rows, value_heads * 128]`."""
+    dev, (rows, C_), Hv = mixed.get_device(), mixed.shape, state.shape[1]
+    if C_ != (2 * key_heads + Hv) * 128:
+        raise ValueError(f"mixed must have {(2 * key_heads + Hv) * 128} columns for {key_heads} key and {Hv} value heads, not {C_}")
+    for name, t, shape in (("mixed", mixed, (rows, C_)), ("b", b, (rows, Hv)), ("a", a, (rows, Hv)), ("z", z, (rows, Hv * 128)),
+                           ("norm_weight", norm_weight, (128,))):
+        if t.get_device() != dev or dev < 0 or t.dtype != torch.bfloat16 or t.stride(-1) != 1 or tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be a bf16 CUDA tensor {list(shape)} with contiguous rows (no CPU fallback)")
+    if conv_weight.get_device() != dev or conv_weight.dtype != torch.bfloat16 or conv_weight.numel() != C_ * 4 or conv_weight.shape[-1] != 4 or not conv_weight.is_contiguous():
+        raise ValueError(f"conv_weight must be a contiguous bf16 CUDA tensor [{C_}, 4]")
+    for name, t in (("dt_bias", dt_bias), ("neg_exp_a", neg_exp_a)):
+        if t.get_device() != dev or t.dtype != torch.float32 or t.numel() != Hv or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous f32 CUDA tensor [{Hv}]")
+    states = state.shape[0]
+    if state.get_device() != dev or state.dtype != torch.float32 or tuple(state.shape) != (states, Hv, 128, 128) or not state.is_contiguous():
+        raise ValueError("state must be a contiguous f32 CUDA tensor [states, value_heads, 128, 128]")
+    if conv_state.get_device() != dev or conv_state.dtype != torch.bfloat16 or tuple(conv_state.shape) != (states, 4, C_) or not conv_state.is_contiguous():
+        raise ValueError(f"conv_state must be a contiguous bf16 CUDA tensor [{states}, 4, {C_}]")
+    for name, t in (("positions", positions), ("state_index", state_index)):
+        if t is not None and (t.get_device() != dev or t.dtype != torch.int32 or tuple(t.shape) != (rows,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 CUDA tensor [{rows}]")
+    if rows > 1 and b.stride(0) != a.stride(0):
+        raise ValueError("b and a must have the same row stride (column ranges of one projection, or contiguous)")
+    if out is None:
+        out = torch.empty((rows, Hv * 128), dtype=torch.bfloat16, device=mixed.device)
+    elif out.get_device() != dev or out.dtype != torch.bfloat16 or tuple(out.shape) != (rows, Hv * 128) or out.stride(1) != 1:
+        raise ValueError(f"out must be a bf16 CUDA tensor [{rows}, {Hv * 128}] with contiguous rows")
+    if rows == 0:
+        return out
+    if ctx is None:
+        ctx = device.load(dev)
+    ctx.check(ctx._lib.s1_gated_delta_rule_step(
+        ctx.handle, mixed.data_ptr(), mixed.stride(0), conv_weight.data_ptr(), positions.data_ptr(), b.data_ptr(), a.data_ptr(), b.stride(0),
+        dt_bias.data_ptr(), neg_exp_a.data_ptr(), z.data_ptr(), z.stride(0), norm_weight.data_ptr(), eps,
+        0 if state_index is None else state_index.data_ptr(), states, conv_state.data_ptr(), state.data_ptr(), rows, key_heads, Hv, out.data_ptr(),
+        out.stride(0)))
+    return out
 
 
 class RopeParams:
@@ -288,22 +351,42 @@ class FullAttention:
             self.merged = Linear(torch.cat([q.weight, k.weight, v.weight], dim=0).contiguous())
 
     def forward(self, x: torch.Tensor, cu_seqlens_host, positions: torch.Tensor, residual: Optional[torch.Tensor] = None,
-                inplace: bool = False) -> torch.Tensor:
-        gated = self.mix(x, cu_seqlens_host, positions)
+                inplace: bool = False, kept: Optional["Kept"] = None) -> torch.Tensor:
+        gated = self.mix(x, cu_seqlens_host, positions, kept)
         return self.output.forward(gated, residual=residual, out=residual if inplace else None)
 
-    def mix(self, x: torch.Tensor, cu_seqlens_host, positions: torch.Tensor) -> torch.Tensor:
-        """Everything up to the input of `o_proj`: the gated attention output `[T, heads * head_dim]` bf16."""
-        T, H, KV, D = x.shape[0], self.heads, self.kv_heads, self.head_dim
-        if self.merged is not None:
-            qkv = self.merged.forward(x)                        # [T, H * 2 * D + 2 * KV * D]
-            qg, k, v = qkv[:, :2 * H * D], qkv[:, 2 * H * D:2 * H * D + KV * D], qkv[:, 2 * H * D + KV * D:]
-        else:
-            qg, k, v = self.q.forward(x), self.k.forward(x), self.v.forward(x)
+    def _inputs(self, x: torch.Tensor):
+        """Query and gate of every head side by side, keys, values: the three input projections of `x`."""
+        H, KV, D = self.heads, self.kv_heads, self.head_dim
+        if self.merged is None:
+            return self.q.forward(x), self.k.forward(x), self.v.forward(x)
+        qkv = self.merged.forward(x)                        # [T, H * 2 * D + 2 * KV * D]
+        return qkv[:, :2 * H * D], qkv[:, 2 * H * D:2 * H * D + KV * D], qkv[:, 2 * H * D + KV * D:]
+
+    def step(self, x: torch.Tensor, kept: "Kept", residual: Optional[torch.Tensor] = None, inplace: bool = False) -> torch.Tensor:
+        """One new token of every row (`x [rows, hidden]`): its key, normed and rotated on the way, and its value go into the pages of
+        `kept.layer`, and its queries attend to them."""
+        H, KV, D, r = self.heads, self.kv_heads, self.head_dim, self.rope
+        qg, k, v = self._inputs(x)
+        _norm.head_norm_rope_(qg, H, 2 * D, D, self.q_norm.weight, self.q_norm.eps, r.cos, r.sin, kept.positions, r.rotary_dim)
+        pages = kept.layer
+        paged.cache_write(k.unflatten(1, (KV, D)), v.unflatten(1, (KV, D)), pages.k, pages.v, kept.slots, norm_weight=self.k_norm.weight,
+                          eps=self.k_norm.eps, cos=r.cos, sin=r.sin, positions=kept.positions, rotary_dim=r.rotary_dim)
+        q4 = qg.unflatten(1, (H, 2, D))
+        gated = paged.attention_paged(q4[:, :, 0], pages.k, pages.v, kept.tables, kept.lengths, gate=q4[:, :, 1], workspace=kept.workspace)
+        return self.output.forward(gated, residual=residual, out=residual if inplace else None)
+
+    def mix(self, x: torch.Tensor, cu_seqlens_host, positions: torch.Tensor, kept: Optional["Kept"] = None) -> torch.Tensor:
+        """Everything up to the input of `o_proj`: the gated attention output `[T, heads * head_dim]` bf16. `kept`: the keys (normed
+        and rotated) and values also go into its pages."""
+        H, KV, D = self.heads, self.kv_heads, self.head_dim
+        qg, k, v = self._inputs(x)
         r = self.rope
         # per head [query | gate]: norm + rotation of the query halves, then of the key heads, each where it lies
         _norm.head_norm_rope_(qg, H, 2 * D, D, self.q_norm.weight, self.q_norm.eps, r.cos, r.sin, positions, r.rotary_dim)
         _norm.head_norm_rope_(k, KV, D, D, self.k_norm.weight, self.k_norm.eps, r.cos, r.sin, positions, r.rotary_dim)
+        if kept is not None:
+            paged.cache_write(k.unflatten(1, (KV, D)), v.unflatten(1, (KV, D)), kept.layer.k, kept.layer.v, kept.slots)
         q4 = qg.unflatten(1, (H, 2, D))
         return attention_causal_gqa(q4[:, :, 0], k.unflatten(1, (KV, D)), v.unflatten(1, (KV, D)), cu_seqlens_host, gate=q4[:, :, 1])
 
@@ -315,10 +398,29 @@ class Layer:
     def __init__(self, input_norm: RmsNorm, mixer, post_norm: RmsNorm, mlp: Mlp):
         self.input_norm, self.mixer, self.post_norm, self.mlp = input_norm, mixer, post_norm, mlp
 
-    def forward(self, x: torch.Tensor, cu_seqlens_host, positions: torch.Tensor, inplace: bool = False) -> torch.Tensor:
-        """`inplace`: update the residual stream `x` in memory (both adds become part of the projections' stores)."""
-        x = self.mixer.forward(self.input_norm(x), cu_seqlens_host, positions, residual=x, inplace=inplace)
+    def forward(self, x: torch.Tensor, cu_seqlens_host, positions: torch.Tensor, inplace: bool = False, kept: Optional["Kept"] = None) -> torch.Tensor:
+        """`inplace`: update the residual stream `x` in memory (both adds become part of the projections' stores). `kept`: what the
+        mixer leaves for `step`."""
+        x = self.mixer.forward(self.input_norm(x), cu_seqlens_host, positions, residual=x, inplace=inplace, **({} if kept is None else {"kept": kept}))
         return self.mlp.forward(self.post_norm(x), residual=x, inplace=inplace)
+
+    def step(self, x: torch.Tensor, kept: "Kept", inplace: bool = False) -> torch.Tensor:
+        """The layer for one new token of every row of a cache."""
+        x = self.mixer.step(self.input_norm(x), kept, residual=x, inplace=inplace)
+        return self.mlp.forward(self.post_norm(x), residual=x, inplace=inplace)
+
+
+@dataclass
+class Kept:
+    """One layer's part of a `PagedCache` and where the tokens of this call belong in it."""
+    layer: object                           # paged.KvPages or paged.DeltaState
+    positions: torch.Tensor                 # int32 [tokens]
+    slots: torch.Tensor                     # int32 [tokens]
+    state_index: torch.Tensor               # int32 [sequences of the call]
+    cu_seqlens: Optional[torch.Tensor] = None   # prompts: int32 [sequences + 1] on the GPU
+    tables: Optional[torch.Tensor] = None       # steps
+    lengths: Optional[torch.Tensor] = None
+    workspace: Optional[torch.Tensor] = None
 
 
 class Decoder:
@@ -338,7 +440,7 @@ class Decoder:
     linear-attention layers, see `LinearAttention`."""
 
     def __init__(self, weights, cfg, max_positions: int = 8192, recurrence: str = "chunked"):
-        self.cfg, self.w = cfg, weights
+        self.cfg, self.w, self.max_positions = cfg, weights, int(max_positions)
         dev = weights["embed_tokens"].device
         lin = lambda name: Linear(weights[name])
         rope = RopeParams(cfg.rope_theta, cfg.rotary_dim, max_positions, dev)
@@ -378,6 +480,59 @@ class Decoder:
             ctx.use_plan(previous)
         y = self.norm(x)
         return (y, states) if collect else y
+
+
+    def prefill(self, ids: torch.Tensor, lengths, cache: "paged.PagedCache"):
+        """Enters prompts into a cache: `ids` the packed prompts (CUDA, one after the other), `lengths` their lengths (host). Same
+        result as `forward` on that batch, `[T, hidden]`, and the rows they got, in the prompts' order."""
+        lengths = [int(n) for n in lengths]
+        total = sum(lengths)
+        if ids.dim() != 1 or not ids.is_cuda or ids.shape[0] != total or not lengths:
+            raise ValueError(f"ids must be a CUDA tensor of the prompts' {total} tokens (no CPU fallback)")
+        self._check(cache, ids)
+        if max(lengths) > self.max_positions:
+            raise ValueError(f"a prompt of {max(lengths)} tokens, positions up to {self.max_positions}")
+        for layer in self.layers:
+            if isinstance(layer.mixer, LinearAttention) and not layer.mixer.fuse_conv:
+                raise ValueError("states are kept by the chunked recurrence with the conv inside (recurrence='chunked', 4 taps)")
+        rows = cache.admit(lengths)
+        ctx = device.load(ids.device.index)
+        bounds = [0]
+        for n in lengths:
+            bounds.append(bounds[-1] + n)
+        plan = cache.enter(rows, lengths)
+        cu, index = torch.tensor([bounds, rows + [0]], dtype=torch.int32).to(ids.device)
+        x = _norm.embedding(self.w["embed_tokens"], ids.to(torch.int32).contiguous())
+        previous = getattr(ctx, "_plan", None)
+        ctx.use_plan(batch_plan_cached(self, ctx, bounds))
+        try:
+            for layer, part in zip(self.layers, cache.layers):
+                x = layer.forward(x, bounds, plan.positions, inplace=True, kept=Kept(part, plan.positions, plan.slots, index, cu_seqlens=cu))
+        finally:
+            ctx.use_plan(previous)
+        return self.norm(x), rows
+
+    def step(self, ids: torch.Tensor, cache: "paged.PagedCache") -> torch.Tensor:
+        """One new token of every active row of the cache: `ids [cache.rows]` (CUDA; those of idle rows are not looked at further than
+        the embedding). Returns the hidden states `[cache.rows, hidden]` after the final norm; the rows of idle requests mean nothing.
+        Can be captured into a CUDA graph and replayed (`cache.advanced` tells the host's mirror)."""
+        if ids.dim() != 1 or not ids.is_cuda or ids.shape[0] != cache.rows:
+            raise ValueError(f"ids must be a CUDA tensor [{cache.rows}], a token for every row of the cache (no CPU fallback)")
+        self._check(cache, ids)
+        if not torch.cuda.is_current_stream_capturing() and cache.held.max() >= self.max_positions:
+            raise ValueError(f"a row has reached the decoder's {self.max_positions} positions")
+        plan = cache.extend()
+        x = _norm.embedding(self.w["embed_tokens"], ids.to(torch.int32).contiguous())
+        for layer, part in zip(self.layers, cache.layers):
+            x = layer.step(x, Kept(part, plan.positions, plan.slots, cache.state_index, tables=cache.tables, lengths=cache.lengths,
+                                   workspace=cache.workspace), inplace=True)
+        return self.norm(x)
+
+    def _check(self, cache, ids) -> None:
+        if cache.device != ids.device or cache.device != self.w["embed_tokens"].device:
+            raise ValueError("the cache, the ids and the weights must be on one GPU")
+        if len(cache.layers) != len(self.layers):
+            raise ValueError(f"the cache was made for {len(cache.layers)} layers, the decoder has {len(self.layers)}")
 
 
 def batch_plan_cached(owner, ctx, bounds):
