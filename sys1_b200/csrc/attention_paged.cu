@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "context.h"
 #include "device_guard.h"
@@ -56,7 +57,8 @@ struct PagedParams {
     long long ldg, gate_head_stride;
     __nv_bfloat16* out;
     long long ldo;
-    float* parts;   // [2 * grid][kHeads][D + 2]: first D unnormalised outputs, then maximum (in units of log2) and sum
+    float* parts;   // [2 * grid][kHeads][D]: unnormalised outputs of the cut spans' pieces
+    float2* marks;  // [2 * grid][kHeads]: maximum (in units of log2) and sum of the same pieces
     int4* records;  // [grid]: row, span of the row, last CTA of the span that begins in this CTA and is cut (or -1)
     int* status;
 };
@@ -266,6 +268,8 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x, ctas = gridDim.x;
 
+    griddep_launch_dependents();  // the join's blocks may take the SMs that run out of work first (they wait for the whole grid)
+
     // ---- rows without a key: zeros
     for (int b = cta * kWarps + warp; b < p.num_seqs; b += ctas * kWarps)
         if (row_length(p, b, lane == 0) == 0)
@@ -364,19 +368,17 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
         }
         __syncthreads();
         const bool whole = u0 == 0 && n == units;
-        float* part = p.parts + (2ll * cta + (u0 == 0 ? 1 : 0)) * (kHeads * (D + 2));
+        const int piece = 2 * cta + (u0 == 0 ? 1 : 0);
+        float* part = p.parts + static_cast<long long>(piece) * kHeads * D;
         for (int i = tid; i < nh * D; i += kThreads) {
             const int h = i / D, d = i % D;
             float x = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) x += weights[w][h] * stage[(w * kHeads + h) * kStage + d];
             if (whole) store_out<D>(p, b, h0 + h, d, sum_all[h] == 0.f ? 0.f : x / sum_all[h]);
-            else part[h * (D + 2) + d] = x;
+            else part[i] = x;
         }
-        if (!whole && tid < nh) {
-            part[tid * (D + 2) + D] = top_all[tid];
-            part[tid * (D + 2) + D + 1] = sum_all[tid];
-        }
+        if (!whole && tid < nh) p.marks[piece * kHeads + tid] = make_float2(top_all[tid], sum_all[tid]);
         if (!whole && u0 == 0) record = make_int4(b, span, static_cast<int>(((unit + units) * workers - 1) / total), 0);
         __syncthreads();  // the stage is a ring again
         r += n;
@@ -385,49 +387,73 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     if (tid == 0) p.records[cta] = record;
 }
 
-// Joins the pieces of the span that began in CTA blockIdx.x of the first kernel and went on in the CTAs after it. A thread owns
-// one head dimension of one head.
+// Joins the pieces of the span that began in CTA blockIdx.x of the first kernel and went on in the CTAs after it, for one of its
+// heads (blockIdx.y). There may be over a hundred pieces when one context is alone, so the warps share them and request
+// theirs independently of one another: the common maximum comes from the marks first.
 template <int D>
 __global__ void __launch_bounds__(256) s1_attention_paged_join_kernel(const PagedParams p) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int kVec = D / 32;  // dims of a lane
+    __shared__ float sums[kWarps][D];
+    griddep_wait();
     const int4 rec = p.records[blockIdx.x];
     if (rec.z < 0) return;
-    const int h = threadIdx.x >> 5, d = blockIdx.y * 32 + (threadIdx.x & 31);
-    const int kvh = rec.y / p.blocks_per_group, hb = rec.y % p.blocks_per_group;
+    const int h = blockIdx.y, kvh = rec.y / p.blocks_per_group, hb = rec.y % p.blocks_per_group;
     if (h >= min(kHeads, p.group - hb * kHeads)) return;
-    constexpr int kPart = kHeads * (D + 2);
-    const float* part = p.parts + (2ll * blockIdx.x + 1) * kPart + h * (D + 2);
-    float top = part[D], sum = part[D + 1], x = part[d];
-    part += kPart;  // piece 0 of the next CTA, then of the ones after it
-#pragma unroll 4
-    for (int c = blockIdx.x + 1; c <= rec.z; ++c, part += 2 * kPart) {
-        const float t = part[D], s = part[D + 1], y = part[d];
-        const float now = fmaxf(top, t);
-        const float f = top == -INFINITY ? 0.f : exp2_fast(top - now), g = t == -INFINITY ? 0.f : exp2_fast(t - now);
-        x = x * f + y * g;
-        sum = sum * f + s * g;
-        top = now;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int first = blockIdx.x, pieces = rec.z - first + 1;  // piece i: of CTA first + i, its second (i = 0) or its first
+    auto place = [&](int i) { return (2 * (first + i) + (i == 0 ? 1 : 0)) * kHeads + h; };
+    float top = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.marks[place(i)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    auto weight = [&](float t) { return t == -INFINITY ? 0.f : exp2_fast(t - top); };
+    float sum = 0.f;
+    for (int i = lane; i < pieces; i += 32) {
+        const float2 m = p.marks[place(i)];
+        sum += m.y * weight(m.x);
     }
-    store_out<D>(p, rec.x, kvh * p.group + hb * kHeads + h, d, sum == 0.f ? 0.f : x / sum);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    float x[kVec] = {};
+#pragma unroll 4
+    for (int i = warp; i < pieces; i += kWarps) {
+        const float f = weight(p.marks[place(i)].x);
+        const float* part = p.parts + static_cast<long long>(place(i)) * D + lane;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) x[e] = fmaf(f, part[32 * e], x[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sums[warp][lane + 32 * e] = x[e];
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += 256) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) y += sums[w][d];
+        store_out<D>(p, rec.x, kvh * p.group + hb * kHeads + h, d, sum == 0.f ? 0.f : y / sum);
+    }
 }
 
 constexpr int kMaxCtas = 256;  // the workspace's share: more than one CTA per SM of any sm_100 part
 
 size_t workspace_bytes_of(int head_dim) {
-    return sizeof(int4) * kMaxCtas + sizeof(float) * 2 * kMaxCtas * kHeads * static_cast<size_t>(head_dim + 2);
+    return sizeof(int4) * kMaxCtas + 2 * kMaxCtas * kHeads * (sizeof(float2) + sizeof(float) * static_cast<size_t>(head_dim));
 }
 
 template <int D>
 int launch(s1_ctx* ctx, const PagedParams& p, int ctas) {
     constexpr int smem = kWarps * kRingBytes;
-    S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<unsigned long long> told{0};  // one bit per device
+    if (!(told.load(std::memory_order_relaxed) >> (ctx->device & 63) & 1)) {
+        S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        told.fetch_or(1ull << (ctx->device & 63), std::memory_order_relaxed);
+    }
     s1_attention_paged_kernel<D><<<ctas, kThreads, smem, ctx->stream>>>(p);
     S1_CUDA_OK(ctx, cudaGetLastError());
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(ctas, D / 32), cfg.blockDim = dim3(256), cfg.stream = ctx->stream;
+    cfg.gridDim = dim3(ctas, std::min(kHeads, p.group)), cfg.blockDim = dim3(256), cfg.stream = ctx->stream;
     cfg.attrs = attr, cfg.numAttrs = 1;
     S1_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, s1_attention_paged_join_kernel<D>, p));
     ctx->launches += 2;
@@ -471,11 +497,12 @@ extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, lon
     S1DeviceGuard guard(ctx->device);
     if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
     const int group = heads / kv_heads, blocks = (group + kHeads - 1) / kHeads;
+    float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas);
     PagedParams p{static_cast<const __nv_bfloat16*>(q), ldq, q_head_stride, static_cast<const __nv_bfloat16*>(k_cache),
                   static_cast<const __nv_bfloat16*>(v_cache), page_stride, token_stride, head_stride, num_pages, __builtin_ctz(page_size), tables, ldt,
                   table_width, lengths, num_seqs, heads, kv_heads, group, kv_heads * blocks, blocks, scale * 1.4426950408889634f,
                   static_cast<const __nv_bfloat16*>(gate), ldg, gate_head_stride, static_cast<__nv_bfloat16*>(out), ldo,
-                  reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas), static_cast<int4*>(workspace), ctx->status_dev};
+                  reinterpret_cast<float*>(marks + 2 * kMaxCtas * kHeads), marks, static_cast<int4*>(workspace), ctx->status_dev};
     const int ctas = std::min(ctx->sm_count, kMaxCtas);
     if (head_dim == 64) return launch<64>(ctx, p, ctas);
     if (head_dim == 128) return launch<128>(ctx, p, ctas);
