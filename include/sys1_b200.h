@@ -397,8 +397,9 @@ int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long long k_head_s
  * A row with lengths[b] <= 0 gets zeros. lengths: DEVICE int32; tables [num_seqs, ldt], of which table_width entries a row may be
  * used. A length beyond that is reported and its row gets zeros; a page outside the cache is reported and its keys are left out.
  * head_dim 64, 128 or 256; any group size. q, gate: as for s1_attention_gqa; out: bf16 [num_seqs, heads * head_dim].
- * `workspace`: device memory, 16-byte aligned, of s1_attention_paged_workspace(head_dim) bytes whatever the batch; calls that may
- * run at the same time (graphs replayed on two streams among them) need one each.
+ * `workspace`: device memory, 16-byte aligned, of s1_attention_paged_workspace(head_dim) bytes whatever the batch, zeroed by the
+ * caller before its first use (every call leaves it ready for the next) and used for nothing else. Calls that may run at the same
+ * time (graphs replayed on two streams among them) need one each.
  */
 size_t s1_attention_paged_workspace(int head_dim);
 int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, long long q_head_stride, const void* k_cache, const void* v_cache,

@@ -40,6 +40,10 @@ constexpr int kUnit = kWarps * kTile;   // keys of one unit of work
 constexpr int kHeads = 8;               // query heads of one span (columns of the MMAs)
 constexpr int kRingBytes = 24 * 1024;   // per warp
 
+// What a span costs beyond its units (its queries, the first keys' way, the warps' results put together), in units of its head dim.
+template <int D>
+constexpr int kStart = 256 / D;
+
 struct PagedParams {
     const __nv_bfloat16* q;
     long long ldq, q_head_stride;
@@ -107,10 +111,9 @@ __device__ __forceinline__ int row_length(const PagedParams& p, int b, bool tell
     }
     return len;
 }
-template <int D>
-__device__ __forceinline__ void store_out(const PagedParams& p, int b, int h, int d, float x) {
-    if (p.gate) x /= 1.f + exp2_fast(-1.4426950408889634f * __bfloat162float(p.gate[b * p.ldg + h * p.gate_head_stride + d]));
-    p.out[b * p.ldo + h * D + d] = __float2bfloat16_rn(x);
+__device__ __forceinline__ float sigmoid_fast(float x) { return 1.f / (1.f + exp2_fast(-1.4426950408889634f * x)); }
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 // One warp's pass over its tiles of a span: keys first + 16 (warp + 8 i), below `end`.
@@ -254,6 +257,17 @@ struct WarpPass {
     }
 };
 
+struct Walk {        // a run over a range of the batch's costs
+    long long at, last;
+    long long r;     // cost inside the row
+    int b;
+};
+struct Segment {     // the part of one span that lies in the range
+    int b, kvh, hb;      // row, KV head, which eight query heads of its group
+    int u0, n, units;    // units u0 .. u0 + n - 1 of `units`
+    int end;             // keys u0 * kUnit .. end - 1
+};
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const PagedParams p) {
     using Pass = WarpPass<D>;
@@ -261,10 +275,10 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     float* stage = reinterpret_cast<float*>(ring_smem);  // [warp][head][D + 4], after the rings have been read
     constexpr int kStage = D + 4;                        // keeps the four head columns of a store on different banks
     __shared__ uint32_t masks[kWarps][Pass::kSlots];
-    __shared__ float tops[kWarps][kHeads], sums[kWarps][kHeads], weights[kWarps][kHeads], top_all[kHeads], sum_all[kHeads];
-    __shared__ long long warp_units[kWarps + 1];
-    __shared__ long long begin_at;
-    __shared__ int begin_row;
+    __shared__ float2 marks[kWarps][kHeads];             // maximum and sum of every warp
+    __shared__ float2 marks_all[kHeads];
+    __shared__ long long warp_costs[kWarps];
+    __shared__ Walk begin_sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x, ctas = gridDim.x;
 
@@ -275,60 +289,73 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
         if (row_length(p, b, lane == 0) == 0)
             for (int i = lane * 8; i < p.heads * D; i += 256) *reinterpret_cast<uint4*>(p.out + b * p.ldo + i) = make_uint4(0, 0, 0, 0);
 
-    // ---- this CTA's range of units
-    auto units_of = [&](int b) { return static_cast<long long>((row_length(p, b, false) + kUnit - 1) / kUnit) * p.spans_per_row; };
+    // ---- this CTA's range
+    auto cost_of = [&](int b) {
+        const int units = (row_length(p, b, false) + kUnit - 1) / kUnit;
+        return units ? static_cast<long long>(units + kStart<D>) * p.spans_per_row : 0ll;
+    };
     const int per = (p.num_seqs + kThreads - 1) / kThreads;
     const int rb = min(tid * per, p.num_seqs), re = min(rb + per, p.num_seqs);
     long long mine = 0;
-    for (int b = rb; b < re; ++b) mine += units_of(b);
+    for (int b = rb; b < re; ++b) mine += cost_of(b);
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += t;
     }
-    if (lane == 31) warp_units[warp] = upto;
+    if (lane == 31) warp_costs[warp] = upto;
     __syncthreads();
     long long before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += warp_units[w];
-        total += warp_units[w];
+        if (w < warp) before += warp_costs[w];
+        total += warp_costs[w];
     }
-    const int workers = static_cast<int>(min(static_cast<long long>(ctas), total));  // each gets one unit at least
+    const int workers = static_cast<int>(min(static_cast<long long>(ctas), total));
     if (cta >= workers) {
         if (tid == 0) p.records[cta] = make_int4(0, 0, -1, 0);
         return;
     }
-    const long long first = total * cta / workers, last = total * (cta + 1) / workers;
-    const long long at = before + upto - mine;
-    if (first >= at && first < at + mine) {
-        long long u = at;
-        int b = rb;
-        for (long long n; u + (n = units_of(b)) <= first; ++b) u += n;
-        begin_row = b;
-        begin_at = first - u;
+    {
+        const long long first = total * cta / workers, at = before + upto - mine;
+        if (first >= at && first < at + mine) {
+            long long u = at;
+            int b = rb;
+            for (long long n; b + 1 < re && u + (n = cost_of(b)) <= first; ++b) u += n;
+            begin_sh = Walk{first, total * (cta + 1) / workers, first - u, b};
+        }
     }
     __syncthreads();
-    int b = begin_row;
-    long long r = begin_at;
+    Walk walk = begin_sh;
+    auto advance = [&](Segment& s) {
+        while (walk.at < walk.last && walk.b < p.num_seqs) {
+            const int len = row_length(p, walk.b, false), units = (len + kUnit - 1) / kUnit, cost = units + kStart<D>;
+            if (units == 0 || walk.r >= static_cast<long long>(cost) * p.spans_per_row) {
+                ++walk.b;
+                walk.r = 0;
+                continue;
+            }
+            const int span = static_cast<int>(walk.r / cost), at = static_cast<int>(walk.r - static_cast<long long>(span) * cost);
+            const int step = static_cast<int>(min(static_cast<long long>(cost - at), walk.last - walk.at));
+            s.b = walk.b, s.units = units;
+            s.kvh = span / p.blocks_per_group, s.hb = span - s.kvh * p.blocks_per_group;
+            s.u0 = max(0, at - kStart<D>), s.n = max(0, at + step - kStart<D>) - s.u0;
+            s.end = min(len, (s.u0 + s.n) * kUnit);
+            walk.at += step, walk.r += step;
+            if (s.n) return true;
+        }
+        return false;
+    };
     int4 record = make_int4(0, 0, -1, 0);
     Pass pass(p, lane, smem_u32(ring_smem) + warp * kRingBytes, masks[warp]);
 
-    for (long long unit = first; unit < last;) {
-        const int len = row_length(p, b, false), units = (len + kUnit - 1) / kUnit;  // of one span of the row
-        if (r >= static_cast<long long>(units) * p.spans_per_row) {
-            ++b;
-            r = 0;
-            continue;
-        }
-        const int span = static_cast<int>(r / units), u0 = static_cast<int>(r % units);
-        const int n = static_cast<int>(min(static_cast<long long>(units - u0), last - unit));
-        const int kvh = span / p.blocks_per_group, hb = span % p.blocks_per_group;
-        const int h0 = kvh * p.group + hb * kHeads, nh = min(kHeads, p.group - hb * kHeads);
+    Segment now = {}, next = {};
+    for (bool more = advance(now); more; now = next) {
+        const int h0 = now.kvh * p.group + now.hb * kHeads, nh = min(kHeads, p.group - now.hb * kHeads);
         uint32_t qf[Pass::kSteps][2];
         {
-            const __nv_bfloat16* q = p.q + b * p.ldq + (h0 + min(lane >> 2, nh - 1)) * p.q_head_stride + 2 * (lane & 3);
+            const __nv_bfloat16* q = p.q + now.b * p.ldq + (h0 + min(lane >> 2, nh - 1)) * p.q_head_stride + 2 * (lane & 3);
             const bool there = (lane >> 2) < nh;
 #pragma unroll
             for (int s = 0; s < Pass::kSteps; ++s) {
@@ -336,53 +363,80 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
                 qf[s][1] = there ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * s + 8)) : 0u;
             }
         }
-        pass.run(b, kvh, qf, u0 * kUnit + warp * kTile, min(len, (u0 + n) * kUnit));
+        pass.run(now.b, now.kvh, qf, now.u0 * kUnit + warp * kTile, now.end);
+        // ---- the next span's first tile is fetched into L2, and this one's gates, while the warps' results are put together
+        const bool whole = now.u0 == 0 && now.n == now.units;
+        const long long stop = walk.at;  // where this segment ends
+        more = advance(next);
+        if (more) {
+            const int j = next.u0 * kUnit + warp * kTile + lane;
+            if (lane < kTile && j < next.end) {
+                const int page = __ldg(p.tables + next.b * p.ldt + (j >> p.shift));
+                if (page >= 0 && page < p.num_pages) {
+                    const long long o = page * p.page_stride + (j & ((1 << p.shift) - 1)) * p.token_stride + next.kvh * p.head_stride;
+                    prefetch_l2(p.k + o, D * 2);
+                    prefetch_l2(p.v + o, D * 2);
+                }
+            }
+        }
+        constexpr int kPairs = kHeads * D / 2 / kThreads;  // pairs of outputs of a thread
+        uint32_t gates[kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            const int h = (tid + i * kThreads) / (D / 2), d = 2 * ((tid + i * kThreads) % (D / 2));
+            gates[i] = whole && p.gate && h < nh ? __ldg(reinterpret_cast<const uint32_t*>(p.gate + now.b * p.ldg + (h0 + h) * p.gate_head_stride + d)) : 0u;
+        }
+        if (lane < 4) marks[warp][2 * lane] = make_float2(pass.m[0], pass.l[0]), marks[warp][2 * lane + 1] = make_float2(pass.m[1], pass.l[1]);
         __syncthreads();  // every ring has been read
         {
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top[0] = fmaxf(top[0], marks[w][2 * (lane & 3)].x), top[1] = fmaxf(top[1], marks[w][2 * (lane & 3) + 1].x);
+            const float f0 = pass.m[0] == -INFINITY ? 0.f : exp2_fast(pass.m[0] - top[0]), f1 = pass.m[1] == -INFINITY ? 0.f : exp2_fast(pass.m[1] - top[1]);
             float* st = stage + warp * kHeads * kStage + 2 * (lane & 3) * kStage + (lane >> 2);
 #pragma unroll
             for (int s = 0; s < Pass::kSteps; ++s) {
-                st[16 * s] = pass.O[s][0];
-                st[kStage + 16 * s] = pass.O[s][1];
-                st[16 * s + 8] = pass.O[s][2];
-                st[kStage + 16 * s + 8] = pass.O[s][3];
+                st[16 * s] = pass.O[s][0] * f0;
+                st[kStage + 16 * s] = pass.O[s][1] * f1;
+                st[16 * s + 8] = pass.O[s][2] * f0;
+                st[kStage + 16 * s + 8] = pass.O[s][3] * f1;
             }
-            if (lane < 4) {
-                tops[warp][2 * lane] = pass.m[0], tops[warp][2 * lane + 1] = pass.m[1];
-                sums[warp][2 * lane] = pass.l[0], sums[warp][2 * lane + 1] = pass.l[1];
+            if (tid < kHeads) {
+                float high = -INFINITY, sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) high = fmaxf(high, marks[w][tid].x);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) sum += marks[w][tid].x == -INFINITY ? 0.f : marks[w][tid].y * exp2_fast(marks[w][tid].x - high);
+                marks_all[tid] = make_float2(high, sum);
             }
         }
         __syncthreads();
-        if (tid < kHeads) {
-            float top = -INFINITY, sum = 0.f;
+        const int piece = 2 * cta + (now.u0 == 0 ? 1 : 0);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, tops[w][tid]);
+        for (int i = 0; i < kPairs; ++i) {
+            const int h = (tid + i * kThreads) / (D / 2), d = 2 * ((tid + i * kThreads) % (D / 2));
+            if (h >= nh) break;
+            float2 x = make_float2(0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float f = tops[w][tid] == -INFINITY ? 0.f : exp2_fast(tops[w][tid] - top);
-                weights[w][tid] = f;
-                sum += f * sums[w][tid];
+                const float2 y = *reinterpret_cast<const float2*>(&stage[(w * kHeads + h) * kStage + d]);
+                x.x += y.x, x.y += y.y;
             }
-            top_all[tid] = top;
-            sum_all[tid] = sum;
+            if (whole) {
+                const float inv = marks_all[h].y == 0.f ? 0.f : 1.f / marks_all[h].y;
+                x.x *= inv, x.y *= inv;
+                if (p.gate) x.x *= sigmoid_fast(__uint_as_float(gates[i] << 16)), x.y *= sigmoid_fast(__uint_as_float(gates[i] & 0xffff0000u));
+                *reinterpret_cast<uint32_t*>(p.out + now.b * p.ldo + (h0 + h) * D + d) = pack2(x.x, x.y);
+            } else {
+                *reinterpret_cast<float2*>(p.parts + (static_cast<long long>(piece) * kHeads + h) * D + d) = x;
+            }
         }
-        __syncthreads();
-        const bool whole = u0 == 0 && n == units;
-        const int piece = 2 * cta + (u0 == 0 ? 1 : 0);
-        float* part = p.parts + static_cast<long long>(piece) * kHeads * D;
-        for (int i = tid; i < nh * D; i += kThreads) {
-            const int h = i / D, d = i % D;
-            float x = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) x += weights[w][h] * stage[(w * kHeads + h) * kStage + d];
-            if (whole) store_out<D>(p, b, h0 + h, d, sum_all[h] == 0.f ? 0.f : x / sum_all[h]);
-            else part[i] = x;
+        if (!whole) {
+            if (tid < nh) p.marks[piece * kHeads + tid] = marks_all[tid];
+            // a span that begins here and is cut at the end of this CTA's range: the CTA that has its last unit
+            if (now.u0 == 0) record = make_int4(now.b, now.kvh * p.blocks_per_group + now.hb, static_cast<int>(((stop - now.n + now.units) * workers - 1) / total), 0);
         }
-        if (!whole && tid < nh) p.marks[piece * kHeads + tid] = make_float2(top_all[tid], sum_all[tid]);
-        if (!whole && u0 == 0) record = make_int4(b, span, static_cast<int>(((unit + units) * workers - 1) / total), 0);
         __syncthreads();  // the stage is a ring again
-        r += n;
-        unit += n;
     }
     if (tid == 0) p.records[cta] = record;
 }
@@ -400,6 +454,9 @@ __global__ void __launch_bounds__(256) s1_attention_paged_join_kernel(const Page
     const int h = blockIdx.y, kvh = rec.y / p.blocks_per_group, hb = rec.y % p.blocks_per_group;
     if (h >= min(kHeads, p.group - hb * kHeads)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = kvh * p.group + hb * kHeads + h;
+    float gate = 0.f;
+    if (p.gate && threadIdx.x < D) gate = __bfloat162float(p.gate[rec.x * p.ldg + head * p.gate_head_stride + threadIdx.x]);
     const int first = blockIdx.x, pieces = rec.z - first + 1;  // piece i: of CTA first + i, its second (i = 0) or its first
     auto place = [&](int i) { return (2 * (first + i) + (i == 0 ? 1 : 0)) * kHeads + h; };
     float top = -INFINITY;
@@ -425,11 +482,13 @@ __global__ void __launch_bounds__(256) s1_attention_paged_join_kernel(const Page
 #pragma unroll
     for (int e = 0; e < kVec; ++e) sums[warp][lane + 32 * e] = x[e];
     __syncthreads();
-    for (int d = threadIdx.x; d < D; d += 256) {
+    if (threadIdx.x < D) {
         float y = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) y += sums[w][d];
-        store_out<D>(p, rec.x, kvh * p.group + hb * kHeads + h, d, sum == 0.f ? 0.f : y / sum);
+        for (int w = 0; w < kWarps; ++w) y += sums[w][threadIdx.x];
+        y = sum == 0.f ? 0.f : y / sum;
+        if (p.gate) y *= sigmoid_fast(gate);
+        p.out[rec.x * p.ldo + head * D + threadIdx.x] = __float2bfloat16_rn(y);
     }
 }
 
@@ -489,6 +548,7 @@ extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, lon
     if (q_head_stride < head_dim || ldq < (heads - 1) * q_head_stride + head_dim || ldo < static_cast<long long>(heads) * head_dim)
         return s1_fail(ctx, S1_EINVAL, "%s: heads must lie inside a row", who);
     if (page_stride < head_dim || token_stride < head_dim || head_stride < head_dim) return s1_fail(ctx, S1_EINVAL, "%s: bad cache strides", who);
+    if (gate && ((reinterpret_cast<uintptr_t>(gate) & 3u) || ((ldg | gate_head_stride) % 2))) return s1_fail(ctx, S1_EINVAL, "%s: gate rows must be 4-byte aligned", who);
     if (gate && (gate_head_stride < head_dim || ldg < (heads - 1) * gate_head_stride + head_dim))
         return s1_fail(ctx, S1_EINVAL, "%s: gate heads must lie inside a row", who);
     if (workspace_bytes < workspace_bytes_of(head_dim))

@@ -71,6 +71,17 @@ class Context:
         off = (-ws.data_ptr()) % 1024
         return ws[off:]
 
+    def attention_workspace(self) -> torch.Tensor:
+        """The workspace of this context's `s1_attention_paged` calls: zeroed once, large enough for every head size, kept for good
+        (captured calls hold its address)."""
+        ws = getattr(self, "_paged_ws", None)
+        if ws is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("this context has no workspace for paged attention yet: make one call before the capture starts, or pass a workspace")
+            ws = torch.zeros(int(self._lib.s1_attention_paged_workspace(256)), dtype=torch.uint8, device=torch.device("cuda", self.ordinal))
+            self._paged_ws = ws
+        return ws
+
     # -- batch plans ------------------------------------------------------------------------------
     def batch_plan(self, cu_seqlens_host, total_tokens: int) -> torch.Tensor:
         """Builds the per-batch tables of the attention / delta-rule kernels once (`s1_batch_plan`) and returns the

@@ -134,9 +134,8 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     workspace: Optional[torch.Tensor] = None, ctx: Optional[device.Context] = None) -> torch.Tensor:
     """Attention of one new token per row over the first `lengths[row]` tokens of its block table (`s1_attention_paged`): q `[rows,
     heads, head_dim]` (rows may be strided), optional gate of the same shape (pre-sigmoid). Rows of length <= 0 get zeros. Returns
-    `[rows, heads * head_dim]`. `workspace`: uint8 CUDA tensor of `attention_paged_workspace(head_dim)` bytes; by default the
-    context's own, which the calls of one stream share. Calls captured into graphs should be given one that lives as long as
-    the graph, and graphs that may run at the same time one each."""
+    `[rows, heads * head_dim]`. `workspace`: uint8 CUDA tensor of `attention_paged_workspace(head_dim)` bytes, zeroed before its first use;
+    by default the context's own, which the calls of one stream share. Graphs that may run at the same time need one each."""
     dev = q.get_device()
     (pages, page, kv, dim), (ps, ts, hs, _) = _caches(k_cache, v_cache, dev)
     B, H = q.shape[0], q.shape[1]
@@ -154,7 +153,7 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         ctx = device.load(dev)
     need = ctx._lib.s1_attention_paged_workspace(dim)
     if workspace is None:
-        workspace = ctx.workspace(need)
+        workspace = ctx.attention_workspace()
     elif workspace.get_device() != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("the workspace must be a contiguous uint8 CUDA tensor")
     ctx.check(ctx._lib.s1_attention_paged(ctx.handle, qp, q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs, tp,
@@ -219,7 +218,7 @@ class PagedCache:
             else:
                 self.layers.append(DeltaState(torch.empty((rows, 4, channels), dtype=torch.bfloat16, device=dev),
                                               torch.empty((rows, cfg.linear_num_value_heads, 128, 128), dtype=torch.float32, device=dev)))
-        self.workspace = torch.empty(attention_paged_workspace(cfg.head_dim), dtype=torch.uint8, device=dev)
+        self.workspace = torch.zeros(attention_paged_workspace(cfg.head_dim), dtype=torch.uint8, device=dev)
 
     def _pages(self, tokens) -> int:
         return -(-int(tokens) // self.page_size)
