@@ -132,67 +132,101 @@ struct WarpPass {
     volatile uint32_t* masks;       // [kSlots] which of the 16 keys a slot holds
     float O[kSteps][4];             // O^T: dims 16 s + lane/4 (+ 8), heads 2 (lane % 4) (+ 1)
     float m[2], l[2];
-    long long off;                  // lane k < 16: where key k of the tile whose keys were requested last begins
-    uint32_t mask;
+    const bool one_page;            // pages of 16 tokens and more: a tile never leaves its page
+    long long off;                  // where the tile whose keys were requested last begins (one_page), or lane j's key of it
+    uint32_t mask;                  // which of its keys there are
 
-    __device__ __forceinline__ WarpPass(const PagedParams& p_, int lane_, uint32_t ring_, uint32_t* masks_) : p(p_), lane(lane_), ring(ring_), masks(masks_) {}
+    __device__ __forceinline__ WarpPass(const PagedParams& p_, int lane_, uint32_t ring_, uint32_t* masks_)
+        : p(p_), lane(lane_), ring(ring_), masks(masks_), one_page(p_.shift >= 4) {}
 
-    // request number n: the keys (even) or values (odd) of this warp's tile n / 2, into slot `slot`
-    __device__ __forceinline__ void request(int n, int slot, int b, int kvh, int first, int end) {
-        const bool values = n & 1;
+    // the keys (or, with `values`, the values) of the tile that begins at key j0, into slot `slot`
+    __device__ __forceinline__ void request(bool values, int slot, int b, int kvh, int j0, int end) {
         if (!values) {
-            const int j = first + (n >> 1) * kUnit + lane;
-            const bool want = lane < kTile && j < end;
-            const int page = want ? __ldg(p.tables + b * p.ldt + (j >> p.shift)) : 0;
-            const bool ok = want && page >= 0 && page < p.num_pages;
-            if (want && !ok) report(p.status, 118, b, page);
-            off = ok ? page * p.page_stride + (j & ((1 << p.shift) - 1)) * p.token_stride + kvh * p.head_stride : 0;
-            mask = __ballot_sync(0xffffffffu, ok);
+            if (one_page) {
+                const int page = __ldg(p.tables + b * p.ldt + (j0 >> p.shift));
+                const bool ok = page >= 0 && page < p.num_pages;
+                if (!ok && lane == 0) report(p.status, 118, b, page);
+                off = page * p.page_stride + (j0 & ((1 << p.shift) - 1)) * p.token_stride + kvh * p.head_stride;
+                mask = ok ? (1u << min(kTile, end - j0)) - 1u : 0u;
+            } else {
+                const int j = j0 + lane;
+                const bool want = lane < kTile && j < end;
+                const int page = want ? __ldg(p.tables + b * p.ldt + (j >> p.shift)) : 0;
+                const bool ok = want && page >= 0 && page < p.num_pages;
+                if (want && !ok) report(p.status, 118, b, page);
+                off = ok ? page * p.page_stride + (j & ((1 << p.shift) - 1)) * p.token_stride + kvh * p.head_stride : 0;
+                mask = __ballot_sync(0xffffffffu, ok);
+            }
+            if (lane == 0) masks[slot] = mask;
         }
-        if (lane == 0) masks[slot] = mask;
         const __nv_bfloat16* base = values ? p.v : p.k;
         const uint32_t dst = ring + slot * kSlotBytes;
+        const int row0 = lane / kChunks, ch = lane % kChunks;
+        // keys past the end (and those of a bad page) are zeros: what lies in the rest of a page is never multiplied
+        if (one_page && mask == (1u << kTile) - 1u) {
+            const __nv_bfloat16* src = base + off + row0 * p.token_stride + ch * 8;
 #pragma unroll
-        for (int i = 0; i < kTile / kRowsPerCopy; ++i) {
-            const int row = i * kRowsPerCopy + lane / kChunks, ch = lane % kChunks;
-            const long long o = __shfl_sync(0xffffffffu, off, row);
-            // keys past the end (and those of a bad page) are zeros: what lies in the rest of a page is never multiplied
-            cp16(dst + row * (D * 2) + ((ch ^ (row & 7)) << 4), base + o + ch * 8, (mask >> row & 1u) ? 16u : 0u);
+            for (int i = 0; i < kTile / kRowsPerCopy; ++i, src += kRowsPerCopy * p.token_stride)
+                cp16(dst + (i * kRowsPerCopy + row0) * (D * 2) + ((ch ^ ((i * kRowsPerCopy + row0) & 7)) << 4), src, 16u);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < kTile / kRowsPerCopy; ++i) {
+                const int row = i * kRowsPerCopy + row0;
+                const bool there = mask >> row & 1u;
+                const long long o = one_page ? off + row * p.token_stride : __shfl_sync(0xffffffffu, off, row);
+                cp16(dst + row * (D * 2) + ((ch ^ (row & 7)) << 4), base + (there ? o : 0) + ch * 8, there ? 16u : 0u);
+            }
         }
     }
 
-    __device__ __forceinline__ void run(int b, int kvh, const uint32_t (&qf)[kSteps][2], int first, int end) {
+    int b, kvh, first, end, requests, wslot;
+
+    // requests of a span's first tiles
+    __device__ __forceinline__ void start(int b_, int kvh_, int first_, int end_) {
+        b = b_, kvh = kvh_, first = first_, end = end_;
+        requests = first < end ? 2 * ((end - first + kUnit - 1) / kUnit) : 0;
+        wslot = 0;
+#pragma unroll 1
+        for (int n = 0; n < kSlots - 1; ++n) {
+            if (n < requests) load(n);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ++wslot;
+        }
+    }
+    __device__ __forceinline__ void load(int n) { request(n & 1, wslot, b, kvh, first + (n >> 1) * kUnit, end); }  // request number n
+
+    __device__ __forceinline__ void run(const uint32_t (&qf)[kSteps][2]) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) O[s][0] = O[s][1] = O[s][2] = O[s][3] = 0.f;
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.f;
-        const int requests = first < end ? 2 * ((end - first + kUnit - 1) / kUnit) : 0;
-        int wslot = 0, rslot = 0;
-#pragma unroll 1
-        for (int n = 0; n < kSlots - 1; ++n) {
-            if (n < requests) request(n, wslot, b, kvh, first, end);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            ++wslot;
+        int rslot = 0;
+        // this lane's rows of the ldmatrix tiles: the 16-byte pieces 2 s + h of row r lie at r * 2 D + ((2 s + h) ^ (r & 7)) * 16, which is
+        // one of four places and a multiple of 128 bytes
+        uint32_t kat[4], vat[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            kat[i] = ((lane >> 3 & 1) * 8 + (lane & 7)) * (D * 2) + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4);
+            vat[i] = ((lane >> 4) * 8 + (lane & 7)) * (D * 2) + (((2 * i + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
         }
-        uint32_t pb0 = 0, pb1 = 0;
 #pragma unroll 1
         for (int n = 0; n < requests; n += 2) {
+            uint32_t pb0, pb1;
             // ---- keys: S^T = K Q^T
             asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
             __syncwarp();  // the slot has landed for every lane, and every lane is done with the one refilled next
-            if (n + kSlots - 1 < requests) request(n + kSlots - 1, wslot, b, kvh, first, end);
+            if (n + kSlots - 1 < requests) load(n + kSlots - 1);
             asm volatile("cp.async.commit_group;" ::: "memory");
             wslot = wslot + 1 == kSlots ? 0 : wslot + 1;
             {
-                const uint32_t live = masks[rslot];
-                const uint32_t row = ring + rslot * kSlotBytes + ((lane >> 3 & 1) * 8 + (lane & 7)) * (D * 2);
+                const uint32_t live = masks[rslot], slot = ring + rslot * kSlotBytes;
                 float c[kChains][4];
 #pragma unroll
                 for (int i = 0; i < kChains; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
                     uint32_t a[4];
-                    ldsm4(a, row + (((2 * s + (lane >> 4)) ^ (lane & 7)) << 4));
+                    ldsm4(a, slot + kat[s & 3] + (s >> 2) * 128);
                     mma16816(c[s % kChains], a, qf[s][0], qf[s][1]);
                 }
 #pragma unroll
@@ -211,7 +245,9 @@ struct WarpPass {
                     top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
                     top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
                 }
-                if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+                if (n == 0) {
+                    m[0] = top[0], m[1] = top[1];
+                } else if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
                     float scale[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -234,15 +270,15 @@ struct WarpPass {
             // ---- values: O^T += V^T P^T
             asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
             __syncwarp();
-            if (n + kSlots < requests) request(n + kSlots, wslot, b, kvh, first, end);
+            if (n + kSlots < requests) load(n + kSlots);
             asm volatile("cp.async.commit_group;" ::: "memory");
             wslot = wslot + 1 == kSlots ? 0 : wslot + 1;
             {
-                const uint32_t row = ring + rslot * kSlotBytes + ((lane >> 4) * 8 + (lane & 7)) * (D * 2);
+                const uint32_t slot = ring + rslot * kSlotBytes;
 #pragma unroll
                 for (int t = 0; t < kSteps; ++t) {
                     uint32_t a[4];
-                    ldsm4_t(a, row + (((2 * t + (lane >> 3 & 1)) ^ (lane & 7)) << 4));
+                    ldsm4_t(a, slot + vat[t & 3] + (t >> 2) * 128);
                     mma16816(O[t], a, pb0, pb1);
                 }
             }
@@ -259,8 +295,8 @@ struct WarpPass {
 
 struct Walk {        // a run over a range of the batch's costs
     long long at, last;
-    long long r;     // cost inside the row
-    int b;
+    int b, kvh, hb;  // row, KV head, which eight query heads of its group
+    int inside;      // cost inside that span
 };
 struct Segment {     // the part of one span that lies in the range
     int b, kvh, hb;      // row, KV head, which eight query heads of its group
@@ -277,6 +313,8 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     __shared__ uint32_t masks[kWarps][Pass::kSlots];
     __shared__ float2 marks[kWarps][kHeads];             // maximum and sum of every warp
     __shared__ float2 marks_all[kHeads];
+    constexpr int kQueryRow = D + 8;                     // eight rows that a warp reads by columns without bank conflicts
+    __shared__ __align__(16) __nv_bfloat16 queries[kHeads][kQueryRow];
     __shared__ long long warp_costs[kWarps];
     __shared__ Walk begin_sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -323,7 +361,10 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
             long long u = at;
             int b = rb;
             for (long long n; b + 1 < re && u + (n = cost_of(b)) <= first; ++b) u += n;
-            begin_sh = Walk{first, total * (cta + 1) / workers, first - u, b};
+            const long long cost = cost_of(b) / p.spans_per_row;
+            const int span = static_cast<int>((first - u) / cost);
+            begin_sh = Walk{first, total * (cta + 1) / workers, b, span / p.blocks_per_group, span % p.blocks_per_group,
+                            static_cast<int>((first - u) % cost)};
         }
     }
     __syncthreads();
@@ -331,18 +372,20 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     auto advance = [&](Segment& s) {
         while (walk.at < walk.last && walk.b < p.num_seqs) {
             const int len = row_length(p, walk.b, false), units = (len + kUnit - 1) / kUnit, cost = units + kStart<D>;
-            if (units == 0 || walk.r >= static_cast<long long>(cost) * p.spans_per_row) {
+            if (units == 0) {
                 ++walk.b;
-                walk.r = 0;
                 continue;
             }
-            const int span = static_cast<int>(walk.r / cost), at = static_cast<int>(walk.r - static_cast<long long>(span) * cost);
-            const int step = static_cast<int>(min(static_cast<long long>(cost - at), walk.last - walk.at));
-            s.b = walk.b, s.units = units;
-            s.kvh = span / p.blocks_per_group, s.hb = span - s.kvh * p.blocks_per_group;
+            const int at = walk.inside, step = static_cast<int>(min(static_cast<long long>(cost - at), walk.last - walk.at));
+            s.b = walk.b, s.kvh = walk.kvh, s.hb = walk.hb, s.units = units;
             s.u0 = max(0, at - kStart<D>), s.n = max(0, at + step - kStart<D>) - s.u0;
             s.end = min(len, (s.u0 + s.n) * kUnit);
-            walk.at += step, walk.r += step;
+            walk.at += step, walk.inside += step;
+            if (walk.inside == cost) {  // on to the next span
+                walk.inside = 0;
+                if (++walk.hb == p.blocks_per_group) walk.hb = 0, ++walk.kvh;
+                if (walk.kvh == p.kv_heads) walk.kvh = 0, ++walk.b;
+            }
             if (s.n) return true;
         }
         return false;
@@ -350,35 +393,51 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     int4 record = make_int4(0, 0, -1, 0);
     Pass pass(p, lane, smem_u32(ring_smem) + warp * kRingBytes, masks[warp]);
 
+    // the queries of a span: 16 bytes a thread, fetched a span ahead (rows past the group's last head repeat it and are not written out)
+    constexpr int kQueryThreads = kHeads * D / 8;
+    const int qrow = tid / (D / 8), qcol = tid % (D / 8) * 8;
+    auto fetch_q = [&](const Segment& s) {
+        const int h = s.kvh * p.group + min(s.hb * kHeads + qrow, p.group - 1);
+        return tid < kQueryThreads ? __ldg(reinterpret_cast<const uint4*>(p.q + s.b * p.ldq + h * p.q_head_stride + qcol)) : make_uint4(0, 0, 0, 0);
+    };
+    auto hand_q = [&](const uint4& q) {
+        if (tid < kQueryThreads) *reinterpret_cast<uint4*>(&queries[qrow][qcol]) = q;
+    };
+
     Segment now = {}, next = {};
-    for (bool more = advance(now); more; now = next) {
+    bool more = advance(now);
+    if (more) {
+        const uint4 q = fetch_q(now);
+        pass.start(now.b, now.kvh, now.u0 * kUnit + warp * kTile, now.end);
+        hand_q(q);
+    }
+    __syncthreads();
+    while (more) {
         const int h0 = now.kvh * p.group + now.hb * kHeads, nh = min(kHeads, p.group - now.hb * kHeads);
-        uint32_t qf[Pass::kSteps][2];
-        {
-            const __nv_bfloat16* q = p.q + now.b * p.ldq + (h0 + min(lane >> 2, nh - 1)) * p.q_head_stride + 2 * (lane & 3);
-            const bool there = (lane >> 2) < nh;
-#pragma unroll
-            for (int s = 0; s < Pass::kSteps; ++s) {
-                qf[s][0] = there ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * s)) : 0u;
-                qf[s][1] = there ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * s + 8)) : 0u;
-            }
-        }
-        pass.run(now.b, now.kvh, qf, now.u0 * kUnit + warp * kTile, now.end);
-        // ---- the next span's first tile is fetched into L2, and this one's gates, while the warps' results are put together
         const bool whole = now.u0 == 0 && now.n == now.units;
         const long long stop = walk.at;  // where this segment ends
         more = advance(next);
-        if (more) {
-            const int j = next.u0 * kUnit + warp * kTile + lane;
-            if (lane < kTile && j < next.end) {
-                const int page = __ldg(p.tables + next.b * p.ldt + (j >> p.shift));
-                if (page >= 0 && page < p.num_pages) {
-                    const long long o = page * p.page_stride + (j & ((1 << p.shift) - 1)) * p.token_stride + next.kvh * p.head_stride;
-                    prefetch_l2(p.k + o, D * 2);
-                    prefetch_l2(p.v + o, D * 2);
-                }
+        // where the next span's keys begin for this warp: looked up now, wanted when this span is done
+        int next_j = next.u0 * kUnit + warp * kTile + lane;
+        const bool fetch = more && lane < kTile && next_j < next.end;
+        const int next_page = fetch ? __ldg(p.tables + next.b * p.ldt + (next_j >> p.shift)) : -1;
+        {
+            uint32_t qf[Pass::kSteps][2];
+#pragma unroll
+            for (int s = 0; s < Pass::kSteps; ++s) {
+                qf[s][0] = *reinterpret_cast<const uint32_t*>(&queries[lane >> 2][16 * s + 2 * (lane & 3)]);
+                qf[s][1] = *reinterpret_cast<const uint32_t*>(&queries[lane >> 2][16 * s + 8 + 2 * (lane & 3)]);
             }
+            pass.run(qf);
         }
+        // ---- the next span's first tile is fetched into L2, its queries and this one's gates into registers, while the warps' results
+        //      are put together
+        if (next_page >= 0 && next_page < p.num_pages) {
+            const long long o = next_page * p.page_stride + (next_j & ((1 << p.shift) - 1)) * p.token_stride + next.kvh * p.head_stride;
+            prefetch_l2(p.k + o, D * 2);
+            prefetch_l2(p.v + o, D * 2);
+        }
+        const uint4 next_q = more ? fetch_q(next) : make_uint4(0, 0, 0, 0);
         constexpr int kPairs = kHeads * D / 2 / kThreads;  // pairs of outputs of a thread
         uint32_t gates[kPairs];
 #pragma unroll
@@ -388,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
         }
         if (lane < 4) marks[warp][2 * lane] = make_float2(pass.m[0], pass.l[0]), marks[warp][2 * lane + 1] = make_float2(pass.m[1], pass.l[1]);
         __syncthreads();  // every ring has been read
-        {
+        const int parts = min(kWarps, (now.end - now.u0 * kUnit + kTile - 1) / kTile);  // warps that had a tile
+        if (warp < parts) {
             float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) top[0] = fmaxf(top[0], marks[w][2 * (lane & 3)].x), top[1] = fmaxf(top[1], marks[w][2 * (lane & 3) + 1].x);
@@ -420,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float2 y = *reinterpret_cast<const float2*>(&stage[(w * kHeads + h) * kStage + d]);
-                x.x += y.x, x.y += y.y;
+                x.x += w < parts ? y.x : 0.f, x.y += w < parts ? y.y : 0.f;
             }
             if (whole) {
                 const float inv = marks_all[h].y == 0.f ? 0.f : 1.f / marks_all[h].y;
@@ -436,7 +496,10 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
             // a span that begins here and is cut at the end of this CTA's range: the CTA that has its last unit
             if (now.u0 == 0) record = make_int4(now.b, now.kvh * p.blocks_per_group + now.hb, static_cast<int>(((stop - now.n + now.units) * workers - 1) / total), 0);
         }
+        hand_q(next_q);
         __syncthreads();  // the stage is a ring again
+        now = next;
+        if (more) pass.start(now.b, now.kvh, now.u0 * kUnit + warp * kTile, now.end);
     }
     if (tid == 0) p.records[cta] = record;
 }
