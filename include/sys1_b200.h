@@ -397,9 +397,8 @@ int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long long k_head_s
  * A row with lengths[b] <= 0 gets zeros. lengths: DEVICE int32; tables [num_seqs, ldt], of which table_width entries a row may be
  * used. A length beyond that is reported and its row gets zeros; a page outside the cache is reported and its keys are left out.
  * head_dim 64, 128 or 256; any group size. q, gate: as for s1_attention_gqa; out: bf16 [num_seqs, heads * head_dim].
- * `workspace`: device memory, 16-byte aligned, of s1_attention_paged_workspace(head_dim) bytes whatever the batch, zeroed by the
- * caller before its first use (every call leaves it ready for the next) and used for nothing else. Calls that may run at the same
- * time (graphs replayed on two streams among them) need one each.
+ * `workspace`: device memory, 16-byte aligned, of s1_attention_paged_workspace(head_dim) bytes whatever the batch. Calls that may
+ * run at the same time (graphs replayed on two streams among them) need one each. q, gate and out rows: 16-byte aligned (gate: 4).
  */
 size_t s1_attention_paged_workspace(int head_dim);
 int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, long long q_head_stride, const void* k_cache, const void* v_cache,
@@ -420,7 +419,8 @@ int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, long long q_he
  *                                s1_gated_delta_rule_conv as one kernel, in f32 with one rounding, updating both states in place.
  *                                positions: DEVICE int32 [num_seqs], the token's index in its sequence; at 0 the sequence starts
  *                                from zero whatever the state holds. Rows without a state get zeros in y. state_index NULL: row b
- *                                has state b. b_proj, a_proj: bf16 [num_seqs, value_heads], row stride ldba.
+ *                                has state b. b_proj, a_proj: bf16 [num_seqs, value_heads], row stride ldba. Alignment: mixed
+ *                                rows 4 bytes; z, y rows and norm_weight 8; conv_weight and the states 16.
  */
 int s1_gated_delta_rule_prefill(s1_ctx* ctx, const void* mixed_before_conv, long long ldm, const void* conv_weight,
                                 const int32_t* positions, const void* b_proj, const void* a_proj, long long ldba, const float* dt_bias,

@@ -144,8 +144,7 @@ extern "C" int s1_sync(s1_ctx* ctx) {
                 "s1_attention_paged: row %d has %d tokens, more than its block table holds",                // 117
                 "s1_attention_paged: the block table of row %d names page %d, outside the cache",           // 118
                 "s1_gated_delta_rule: row %d has state %d, outside the states or another row's",            // 119
-                "s1_gated_delta_rule_step: row %d has position %d",                                         // 120
-                "s1_attention_paged: the workspace was not zeroed before its first use (word %d holds %d)"};   // 121
+                "s1_gated_delta_rule_step: row %d has position %d"};                                        // 120
             const int n = static_cast<int>(sizeof(what) / sizeof(what[0]));
             if (st[0] - 110 < n) return s1_fail(ctx, S1_EKERNEL, what[st[0] - 110], st[2], st[3]);
         }

@@ -72,13 +72,11 @@ class Context:
         return ws[off:]
 
     def attention_workspace(self) -> torch.Tensor:
-        """The workspace of this context's `s1_attention_paged` calls: zeroed once, large enough for every head size, kept for good
-        (captured calls hold its address)."""
+        """The workspace of this context's `s1_attention_paged` calls: large enough for every head size, and kept for good, so that
+        a captured call never finds its address given to something else."""
         ws = getattr(self, "_paged_ws", None)
         if ws is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("this context has no workspace for paged attention yet: make one call before the capture starts, or pass a workspace")
-            ws = torch.zeros(int(self._lib.s1_attention_paged_workspace(256)), dtype=torch.uint8, device=torch.device("cuda", self.ordinal))
+            ws = torch.empty(int(self._lib.s1_attention_paged_workspace(256)), dtype=torch.uint8, device=torch.device("cuda", self.ordinal))
             self._paged_ws = ws
         return ws
 
@@ -192,14 +190,19 @@ def comm_unique_id() -> bytes:
     return buf.raw
 
 
+# The current stream's handle without the stream object around it (1.2 us a call, which every operator makes); PyTorch builds
+# without that function get the handle from the object.
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda ordinal: torch.cuda.current_stream(ordinal).cuda_stream)
+
+
 def load(ordinal: Optional[int] = None) -> Context:
     """Context for GPU `ordinal` (default: PyTorch's current device) on PyTorch's current stream."""
     if ordinal is None:
         ordinal = torch.cuda.current_device()
-    stream = torch.cuda.current_stream(ordinal)
-    key = (ordinal, stream.cuda_stream)
+    key = (ordinal, _current_stream(ordinal))
     ctx = _contexts.get(key)
     if ctx is None:
+        stream = torch.cuda.current_stream(ordinal)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("no context exists for the capturing stream yet: call device.load() on that stream once "
                                "before the capture starts (creating a context allocates)")

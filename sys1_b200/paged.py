@@ -26,35 +26,46 @@ class BlockTables(NamedTuple):
     free_count: torch.Tensor
 
 
-def _ints(t: torch.Tensor, dev: int, shape, name: str) -> int:
-    if t.get_device() != dev or dev < 0 or t.dtype != torch.int32 or not t.is_contiguous():
+_I32, _BF16 = torch.int32, torch.bfloat16
+
+
+def _ints(t: torch.Tensor, dev: int, n: int, name: str) -> int:
+    if t.dtype is not _I32 or t.get_device() != dev or dev < 0 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor on the call's GPU (no CPU fallback)")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
+    if t.shape != (n,):
+        raise ValueError(f"{name} must have shape [{n}], not {list(t.shape)}")
     return t.data_ptr()
 
 
-def _table(t: torch.Tensor, dev: int, rows: int) -> int:
-    if t.get_device() != dev or dev < 0 or t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.shape[0] != rows:
+def _table(t: torch.Tensor, dev: int, rows: int):
+    """Address, row stride and width of the block tables."""
+    if t.dtype is not _I32 or t.get_device() != dev or dev < 0 or t.dim() != 2 or t.shape[0] != rows or t.stride(1) != 1:
         raise ValueError(f"block tables must be an int32 CUDA tensor [{rows}, pages] with contiguous rows")
-    return t.data_ptr()
+    return t.data_ptr(), t.stride(0), t.shape[1]
 
 
-def _heads(t: torch.Tensor, dev: int, shape, name: str) -> int:
-    if t.get_device() != dev or dev < 0 or t.dtype != torch.bfloat16 or t.dim() != 3 or t.stride(2) != 1:
+def _heads(t: torch.Tensor, dev: int, shape, name: str):
+    """Address, token stride and head stride of a tensor of head rows."""
+    if t.dtype is not _BF16 or t.get_device() != dev or dev < 0 or t.dim() != 3:
         raise ValueError(f"{name} must be a bf16 CUDA tensor [tokens, heads, head_dim] with contiguous head rows (no CPU fallback)")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
-    return t.data_ptr()
+    token, head, one = t.stride()
+    if one != 1:
+        raise ValueError(f"{name} must have contiguous head rows")
+    return t.data_ptr(), token, head
 
 
 def _caches(k: torch.Tensor, v: torch.Tensor, dev: int):
-    for name, t in (("k_cache", k), ("v_cache", v)):
-        if t.get_device() != dev or dev < 0 or t.dtype != torch.bfloat16 or t.dim() != 4 or t.stride(3) != 1:
-            raise ValueError(f"{name} must be a bf16 CUDA tensor [pages, page_size, kv_heads, head_dim] with contiguous head rows (no CPU fallback)")
-    if k.shape != v.shape or k.stride() != v.stride():
-        raise ValueError("k_cache and v_cache must have the same shape and strides")
-    return k.shape, k.stride()
+    """The caches' shape and strides."""
+    for t in (k, v):
+        if t.dtype is not _BF16 or t.get_device() != dev or dev < 0 or t.dim() != 4:
+            raise ValueError("k_cache and v_cache must be bf16 CUDA tensors [pages, page_size, kv_heads, head_dim] with contiguous head rows "
+                             "(no CPU fallback)")
+    shape, strides = k.shape, k.stride()
+    if v.shape != shape or v.stride() != strides or strides[3] != 1:
+        raise ValueError("k_cache and v_cache must have the same shape and strides, and contiguous head rows")
+    return shape, strides
 
 
 def block_tables(cached: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
@@ -65,40 +76,43 @@ def block_tables(cached: torch.Tensor, tables: torch.Tensor, free_pages: torch.T
     pages are taken from, `tables` int32 `[rows, width]` updated in place. `max_tokens`: tokens of the packed batch, with those
     behind the last row (needed with `added`). `lengths` may be `cached` and `free_count_out` may be `free_count`: both are then
     advanced in place."""
-    dev, rows = cached.get_device(), cached.shape[0] if cached.dim() == 1 else -1
-    args = [_ints(cached, dev, (rows,), "cached"), 0 if added is None else _ints(added, dev, (rows,), "added"), rows, page_size,
-            _ints(free_pages, dev, (free_pages.numel(),), "free_pages"), free_pages.numel(), _ints(free_count, dev, (1,), "free_count")]
-    tp = _table(tables, dev, rows)
+    dev, rows, pool = cached.get_device(), cached.numel(), free_pages.numel()
     if max_tokens is None:
         if added is not None:
             raise ValueError("max_tokens is needed with `added`: the host knows how many tokens the batch has")
         max_tokens = rows
     if max_tokens < 0:
         raise ValueError("max_tokens must not be negative")
-    out = torch.empty(2 * rows + 2 + 2 * max_tokens, dtype=torch.int32, device=cached.device)
+    cp, fp, np_ = _ints(cached, dev, rows, "cached"), _ints(free_pages, dev, pool, "free_pages"), _ints(free_count, dev, 1, "free_count")
+    ap = 0 if added is None else _ints(added, dev, rows, "added")
+    tp, ldt, width = _table(tables, dev, rows)
+    # one buffer for what is new: lengths, first tokens, positions, slots, pages left
+    out = cached.new_empty(2 * rows + 2 + 2 * max_tokens)
+    at = out.data_ptr()
+    lp, up, pp, sp, op = at, at + 4 * rows, at + 4 * (2 * rows + 1), at + 4 * (2 * rows + 1 + max_tokens), at + 4 * (2 * rows + 1 + 2 * max_tokens)
     new_lengths, cu, positions, slots, count = out.split_with_sizes((rows, rows + 1, max_tokens, max_tokens, 1))
     if lengths is not None:
-        _ints(lengths, dev, (rows,), "lengths")
-        new_lengths = lengths
+        lp, new_lengths = _ints(lengths, dev, rows, "lengths"), lengths
     if free_count_out is not None:
-        _ints(free_count_out, dev, (1,), "free_count_out")
-        count = free_count_out
+        op, count = _ints(free_count_out, dev, 1, "free_count_out"), free_count_out
     if ctx is None:
         ctx = device.load(dev)
-    ctx.check(ctx._lib.s1_block_tables(ctx.handle, *args, count.data_ptr(), tp, tables.stride(0), tables.shape[1], new_lengths.data_ptr(),
-                                       cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), max_tokens))
+    rc = ctx._lib.s1_block_tables(ctx._h, cp, ap, rows, page_size, fp, pool, np_, op, tp, ldt, width, lp, up, pp, sp, max_tokens)
+    if rc:
+        ctx.check(rc)
     return BlockTables(new_lengths, cu, positions, slots, count)
 
 
 def release_blocks(ended: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
                    page_size: int, ctx: Optional[device.Context] = None) -> None:
     """Puts the pages of every row with `ended[row] != 0` back on the stack and makes the row idle (`s1_release_blocks`)."""
-    dev, rows = lengths.get_device(), lengths.shape[0] if lengths.dim() == 1 else -1
-    args = (_ints(ended, dev, (rows,), "ended"), rows, page_size, _ints(lengths, dev, (rows,), "lengths"), _table(tables, dev, rows), tables.stride(0),
-            tables.shape[1], _ints(free_pages, dev, (free_pages.numel(),), "free_pages"), free_pages.numel(), _ints(free_count, dev, (1,), "free_count"))
+    dev, rows, pool = lengths.get_device(), lengths.numel(), free_pages.numel()
+    ep, lp, fp, np_ = (_ints(ended, dev, rows, "ended"), _ints(lengths, dev, rows, "lengths"), _ints(free_pages, dev, pool, "free_pages"),
+                       _ints(free_count, dev, 1, "free_count"))
+    tp, ldt, width = _table(tables, dev, rows)
     if ctx is None:
         ctx = device.load(dev)
-    ctx.check(ctx._lib.s1_release_blocks(ctx.handle, *args))
+    ctx.check(ctx._lib.s1_release_blocks(ctx._h, ep, rows, page_size, lp, tp, ldt, width, fp, pool, np_))
 
 
 def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
@@ -110,23 +124,28 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     dev = k.get_device()
     (pages, page, kv, dim), (ps, ts, hs, _) = _caches(k_cache, v_cache, dev)
     T = k.shape[0]
-    kp, vp, sp = _heads(k, dev, (T, kv, dim), "k"), _heads(v, dev, (T, kv, dim), "v"), _ints(slots, dev, (T,), "slots")
+    kp, ldk, khs = _heads(k, dev, (T, kv, dim), "k")
+    vp, ldv, vhs = _heads(v, dev, (T, kv, dim), "v")
+    sp = _ints(slots, dev, T, "slots")
     wp = cp = np_ = pp = rows = 0
     if norm_weight is not None:
         if cos is None or sin is None or positions is None:
             raise ValueError("keys that are normed are rotated too: cos, sin and positions are needed")
-        if norm_weight.get_device() != dev or norm_weight.dtype != torch.bfloat16 or tuple(norm_weight.shape) != (dim,) or not norm_weight.is_contiguous():
+        if norm_weight.get_device() != dev or norm_weight.dtype is not _BF16 or norm_weight.shape != (dim,) or not norm_weight.is_contiguous():
             raise ValueError(f"norm_weight must be a contiguous bf16 CUDA tensor [{dim}]")
+        rows = cos.shape[0]
         for t in (cos, sin):
-            if t.get_device() != dev or t.dtype != torch.float32 or t.shape != cos.shape or t.dim() != 2 or t.shape[1] != rotary_dim // 2 or not t.is_contiguous():
+            if t.get_device() != dev or t.dtype is not torch.float32 or t.shape != (rows, rotary_dim // 2) or not t.is_contiguous():
                 raise ValueError("cos and sin must be contiguous f32 CUDA tensors [positions, rotary_dim / 2]")
-        wp, cp, np_, pp, rows = norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ints(positions, dev, (T,), "positions"), cos.shape[0]
+        wp, cp, np_, pp = norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ints(positions, dev, T, "positions")
     if T == 0:
         return
     if ctx is None:
         ctx = device.load(dev)
-    ctx.check(ctx._lib.s1_cache_write(ctx.handle, kp, k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1), sp, T, kv, dim, wp, eps, cp, np_, pp,
-                                      rows, rotary_dim, 1 if bf16_ops else 0, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs))
+    rc = ctx._lib.s1_cache_write(ctx._h, kp, ldk, khs, vp, ldv, vhs, sp, T, kv, dim, wp, eps, cp, np_, pp, rows, rotary_dim, 1 if bf16_ops else 0,
+                                 k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs)
+    if rc:
+        ctx.check(rc)
 
 
 def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
@@ -134,31 +153,35 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     workspace: Optional[torch.Tensor] = None, ctx: Optional[device.Context] = None) -> torch.Tensor:
     """Attention of one new token per row over the first `lengths[row]` tokens of its block table (`s1_attention_paged`): q `[rows,
     heads, head_dim]` (rows may be strided), optional gate of the same shape (pre-sigmoid). Rows of length <= 0 get zeros. Returns
-    `[rows, heads * head_dim]`. `workspace`: uint8 CUDA tensor of `attention_paged_workspace(head_dim)` bytes, zeroed before its first use;
-    by default the context's own, which the calls of one stream share. Graphs that may run at the same time need one each."""
+    `[rows, heads * head_dim]`. `workspace`: uint8 CUDA tensor of `attention_paged_workspace(head_dim)` bytes; by default
+    the context's own, which the calls of one stream share. Graphs that may run at the same time need one each."""
     dev = q.get_device()
     (pages, page, kv, dim), (ps, ts, hs, _) = _caches(k_cache, v_cache, dev)
-    B, H = q.shape[0], q.shape[1]
-    qp, tp, lp = _heads(q, dev, (B, H, dim), "q"), _table(tables, dev, B), _ints(lengths, dev, (B,), "lengths")
-    gp = ldg = gs = 0
+    shape = q.shape
+    B, H = shape[0], shape[1]
+    qp, ldq, qhs = _heads(q, dev, (B, H, dim), "q")
+    tp, ldt, width = _table(tables, dev, B)
+    lp = _ints(lengths, dev, B, "lengths")
+    gp = ldg = ghs = 0
     if gate is not None:
-        gp, ldg, gs = _heads(gate, dev, (B, H, dim), "gate"), gate.stride(0), gate.stride(1)
+        gp, ldg, ghs = _heads(gate, dev, (B, H, dim), "gate")
     if out is None:
-        out = torch.empty((B, H * dim), dtype=torch.bfloat16, device=q.device)
-    elif out.get_device() != dev or out.dtype != torch.bfloat16 or tuple(out.shape) != (B, H * dim) or out.stride(1) != 1:
+        out = q.new_empty((B, H * dim))
+    elif out.get_device() != dev or out.dtype is not _BF16 or out.shape != (B, H * dim) or out.stride(1) != 1:
         raise ValueError(f"out must be a bf16 CUDA tensor [{B}, {H * dim}] with contiguous rows")
     if B == 0:
         return out
     if ctx is None:
         ctx = device.load(dev)
-    need = ctx._lib.s1_attention_paged_workspace(dim)
     if workspace is None:
         workspace = ctx.attention_workspace()
-    elif workspace.get_device() != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+    elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
         raise ValueError("the workspace must be a contiguous uint8 CUDA tensor")
-    ctx.check(ctx._lib.s1_attention_paged(ctx.handle, qp, q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs, tp,
-                                          tables.stride(0), tables.shape[1], lp, B, H, kv, dim, dim ** -0.5 if scale is None else scale, gp, ldg, gs,
-                                          out.data_ptr(), out.stride(0), workspace.data_ptr(), workspace.numel()))
+    rc = ctx._lib.s1_attention_paged(ctx._h, qp, ldq, qhs, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs, tp, ldt, width, lp, B, H, kv, dim,
+                                     dim ** -0.5 if scale is None else scale, gp, ldg, ghs, out.data_ptr(), out.stride(0), workspace.data_ptr(),
+                                     workspace.numel())
+    if rc:
+        ctx.check(rc)
     return out
 
 
@@ -218,7 +241,7 @@ class PagedCache:
             else:
                 self.layers.append(DeltaState(torch.empty((rows, 4, channels), dtype=torch.bfloat16, device=dev),
                                               torch.empty((rows, cfg.linear_num_value_heads, 128, 128), dtype=torch.float32, device=dev)))
-        self.workspace = torch.zeros(attention_paged_workspace(cfg.head_dim), dtype=torch.uint8, device=dev)
+        self.workspace = torch.empty(attention_paged_workspace(cfg.head_dim), dtype=torch.uint8, device=dev)
 
     def _pages(self, tokens) -> int:
         return -(-int(tokens) // self.page_size)

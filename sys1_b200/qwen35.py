@@ -255,41 +255,37 @@ def gated_delta_rule_step(mixed: torch.Tensor, conv_weight: torch.Tensor, positi
     positions int32 `[rows]`, dt_bias, neg_exp_a f32 `[value_heads]`. `conv_state` bf16 `[states, 4, C]` and `state` f32 `[states,
     value_heads, 128, 128]` are updated in place; row r has state `state_index[r]` (int32, -1: none, its output is zero; None: r).
     Returns `[rows, value_heads * 128]`."""
-    dev, (rows, C_), Hv = mixed.get_device(), mixed.shape, state.shape[1]
+    dev, (rows, C_), (states, Hv, _, _) = mixed.get_device(), mixed.shape, state.shape
+    bf16, f32 = torch.bfloat16, torch.float32
     if C_ != (2 * key_heads + Hv) * 128:
         raise ValueError(f"mixed must have {(2 * key_heads + Hv) * 128} columns for {key_heads} key and {Hv} value heads, not {C_}")
-    for name, t, shape in (("mixed", mixed, (rows, C_)), ("b", b, (rows, Hv)), ("a", a, (rows, Hv)), ("z", z, (rows, Hv * 128)),
-                           ("norm_weight", norm_weight, (128,))):
-        if t.get_device() != dev or dev < 0 or t.dtype != torch.bfloat16 or t.stride(-1) != 1 or tuple(t.shape) != shape:
-            raise ValueError(f"{name} must be a bf16 CUDA tensor {list(shape)} with contiguous rows (no CPU fallback)")
-    if conv_weight.get_device() != dev or conv_weight.dtype != torch.bfloat16 or conv_weight.numel() != C_ * 4 or conv_weight.shape[-1] != 4 or not conv_weight.is_contiguous():
-        raise ValueError(f"conv_weight must be a contiguous bf16 CUDA tensor [{C_}, 4]")
-    for name, t in (("dt_bias", dt_bias), ("neg_exp_a", neg_exp_a)):
-        if t.get_device() != dev or t.dtype != torch.float32 or t.numel() != Hv or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous f32 CUDA tensor [{Hv}]")
-    states = state.shape[0]
-    if state.get_device() != dev or state.dtype != torch.float32 or tuple(state.shape) != (states, Hv, 128, 128) or not state.is_contiguous():
-        raise ValueError("state must be a contiguous f32 CUDA tensor [states, value_heads, 128, 128]")
-    if conv_state.get_device() != dev or conv_state.dtype != torch.bfloat16 or tuple(conv_state.shape) != (states, 4, C_) or not conv_state.is_contiguous():
-        raise ValueError(f"conv_state must be a contiguous bf16 CUDA tensor [{states}, 4, {C_}]")
-    for name, t in (("positions", positions), ("state_index", state_index)):
-        if t is not None and (t.get_device() != dev or t.dtype != torch.int32 or tuple(t.shape) != (rows,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous int32 CUDA tensor [{rows}]")
-    if rows > 1 and b.stride(0) != a.stride(0):
+
+    def check(name, t, dtype, shape, whole=True):
+        if t.dtype is not dtype or t.get_device() != dev or dev < 0 or t.shape != shape or (not t.is_contiguous() if whole else t.stride(-1) != 1):
+            raise ValueError(f"{name} must be a {'contiguous ' if whole else ''}{str(dtype)[6:]} CUDA tensor {list(shape)}"
+                             f"{'' if whole else ' with contiguous rows'} (no CPU fallback)")
+        return t.data_ptr()
+
+    mp, bp, ap = check("mixed", mixed, bf16, (rows, C_), False), check("b", b, bf16, (rows, Hv), False), check("a", a, bf16, (rows, Hv), False)
+    zp, np_, pp = check("z", z, bf16, (rows, Hv * 128), False), check("norm_weight", norm_weight, bf16, (128,)), check("positions", positions, torch.int32, (rows,))
+    wp = check("conv_weight", conv_weight, bf16, (C_, 4) if conv_weight.dim() == 2 else (C_, 1, 4))
+    tp, dp = check("dt_bias", dt_bias, f32, (Hv,)), check("neg_exp_a", neg_exp_a, f32, (Hv,))
+    sp, cp = check("state", state, f32, (states, Hv, 128, 128)), check("conv_state", conv_state, bf16, (states, 4, C_))
+    ip = 0 if state_index is None else check("state_index", state_index, torch.int32, (rows,))
+    ldba = b.stride(0)
+    if ldba != a.stride(0) and rows > 1:
         raise ValueError("b and a must have the same row stride (column ranges of one projection, or contiguous)")
     if out is None:
-        out = torch.empty((rows, Hv * 128), dtype=torch.bfloat16, device=mixed.device)
-    elif out.get_device() != dev or out.dtype != torch.bfloat16 or tuple(out.shape) != (rows, Hv * 128) or out.stride(1) != 1:
-        raise ValueError(f"out must be a bf16 CUDA tensor [{rows}, {Hv * 128}] with contiguous rows")
+        out = mixed.new_empty((rows, Hv * 128))
+    op = check("out", out, bf16, (rows, Hv * 128), False)
     if rows == 0:
         return out
     if ctx is None:
         ctx = device.load(dev)
-    ctx.check(ctx._lib.s1_gated_delta_rule_step(
-        ctx.handle, mixed.data_ptr(), mixed.stride(0), conv_weight.data_ptr(), positions.data_ptr(), b.data_ptr(), a.data_ptr(), b.stride(0),
-        dt_bias.data_ptr(), neg_exp_a.data_ptr(), z.data_ptr(), z.stride(0), norm_weight.data_ptr(), eps,
-        0 if state_index is None else state_index.data_ptr(), states, conv_state.data_ptr(), state.data_ptr(), rows, key_heads, Hv, out.data_ptr(),
-        out.stride(0)))
+    rc = ctx._lib.s1_gated_delta_rule_step(ctx._h, mp, mixed.stride(0), wp, pp, bp, ap, ldba, tp, dp, zp, z.stride(0), np_, eps, ip, states, cp, sp, rows,
+                                           key_heads, Hv, op, out.stride(0))
+    if rc:
+        ctx.check(rc)
     return out
 
 
