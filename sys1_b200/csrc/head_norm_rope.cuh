@@ -36,7 +36,7 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // The cosines and sines of lane `sub` of a head (its 8 columns of the rotated span, `rot / 16` lanes to each half).
 __device__ __forceinline__ void load_rotation(const float* cos_t, const float* sin_t, int pos, int rot, int sub, float (&c)[8], float (&sn)[8]) {
-    const long long tb = static_cast<long long>(pos) * (rot / 2) + (sub % (rot / 16)) * 8;
+    const long long tb = static_cast<long long>(pos) * (rot / 2) + (sub & (rot / 16 - 1)) * 8;  // rot / 16 is a power of two
     *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cos_t + tb));
     *reinterpret_cast<float4*>(c + 4) = __ldg(reinterpret_cast<const float4*>(cos_t + tb) + 1);
     *reinterpret_cast<float4*>(sn) = __ldg(reinterpret_cast<const float4*>(sin_t + tb));

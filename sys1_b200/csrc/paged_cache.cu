@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "context.h"
 #include "device_guard.h"
@@ -250,46 +251,59 @@ struct WriteParams {
 };
 
 // LPR lanes hold one head row (16 bytes each); the first half of the rows are keys, the second values. Streaming: every value is
-// read and written once.
-template <int LPR, bool NORM>
+// read and written once. A warp that only copies takes U = 2 groups of rows where there are rows enough to fill the GPU that way and
+// requests both before it writes the first (16384 tokens x 4 heads of 256: 23.2 us = 5.8 TB/s, with U = 1 27.2, with U = 4 23.5; 64
+// tokens x 2 heads: 1.8 us, with U = 1 1.6). Norm and rotation leave U = 1 the faster at every size: registers for the other row's
+// cosines cost the warps that hide their latency.
+template <int LPR, bool NORM, int U>
 __global__ void __launch_bounds__(256) s1_cache_write_kernel(const WriteParams p) {
     constexpr int RPW = 32 / LPR;
     const int lane = threadIdx.x & 31, sub = lane % LPR;
-    const long long warp = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5;
-    const long long rows = static_cast<long long>(p.T) * p.kv_heads;
-    long long row = warp * RPW + lane / LPR;
-    const bool value = row >= rows;
-    if (value) row -= rows;
-    bool live = row < rows;
-    const int t = live ? static_cast<int>(row / p.kv_heads) : 0, h = live ? static_cast<int>(row % p.kv_heads) : 0;
-    const long long slot = live ? __ldg(p.slots + t) : -1;
-    const __nv_bfloat16* src = value ? p.v + t * p.ldv + h * p.v_head_stride : p.k + t * p.ldk + h * p.k_head_stride;
-    uint4 raw = live ? __ldg(reinterpret_cast<const uint4*>(src + sub * 8)) : make_uint4(0, 0, 0, 0);
-    live = live && slot >= 0;  // tokens without a slot are left out
-    if (live && slot >= p.num_slots) {
-        report(p.status, 116, t, static_cast<int>(slot));
-        live = false;
-    }
-    if constexpr (NORM) {
-        const int halfc = p.rot / 16;
-        const bool rotates = live && !value && sub < 2 * halfc;
-        const int pos = rotates ? __ldg(p.positions + t) : 0;
-        const bool pos_ok = pos >= 0 && pos < p.max_pos;
-        float c[8], sn[8];
-        if (rotates && pos_ok) {
-            load_rotation(p.cos_t, p.sin_t, pos, p.rot, sub, c, sn);
-        } else {
+    const unsigned rows = static_cast<unsigned>(p.T) * static_cast<unsigned>(p.kv_heads);  // of keys; as many of values behind them
+    const unsigned first = ((blockIdx.x * 256u + threadIdx.x) >> 5) * (RPW * U) + lane / LPR;
+    uint4 raw[U];
+    long long slot[U];
+    int t[U], h[U], pos[U];
+    bool value[U], live[U];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f;
-        }
-        const uint4 normed = head_norm_rope<LPR>(raw, p.norm_w, p.eps, c, sn, rotates && pos_ok, sub, halfc, p.bf16_ops);
-        if (!value) raw = normed;
-        if (rotates && !pos_ok) report(p.status, 102, t, pos);
+    for (int u = 0; u < U; ++u) {
+        unsigned row = first + u * RPW;
+        value[u] = row >= rows;
+        if (value[u]) row -= rows;
+        live[u] = row < rows;
+        t[u] = live[u] ? static_cast<int>(row / static_cast<unsigned>(p.kv_heads)) : 0, h[u] = live[u] ? static_cast<int>(row) - t[u] * p.kv_heads : 0;
+        slot[u] = live[u] ? __ldg(p.slots + t[u]) : -1;
+        pos[u] = NORM && live[u] && !value[u] ? __ldg(p.positions + t[u]) : 0;
+        const __nv_bfloat16* src = value[u] ? p.v + t[u] * p.ldv + h[u] * p.v_head_stride : p.k + t[u] * p.ldk + h[u] * p.k_head_stride;
+        raw[u] = live[u] ? __ldg(reinterpret_cast<const uint4*>(src + sub * 8)) : make_uint4(0, 0, 0, 0);
     }
-    if (!live) return;
-    __nv_bfloat16* dst = (value ? p.v_cache : p.k_cache) + (slot >> p.shift) * p.page_stride + (slot & ((1ll << p.shift) - 1)) * p.token_stride +
-                         h * p.head_stride;
-    *reinterpret_cast<uint4*>(dst + sub * 8) = raw;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        live[u] = live[u] && slot[u] >= 0;  // tokens without a slot are left out
+        if (live[u] && slot[u] >= p.num_slots) {
+            report(p.status, 116, t[u], static_cast<int>(slot[u]));
+            live[u] = false;
+        }
+        if (NORM && !__all_sync(0xffffffffu, value[u])) {  // a warp of values alone has nothing to norm
+            const int halfc = p.rot / 16;
+            const bool rotates = live[u] && !value[u] && sub < 2 * halfc;
+            const bool pos_ok = pos[u] >= 0 && pos[u] < p.max_pos;
+            float c[8], sn[8];
+            if (!value[u] && sub < 2 * halfc && pos_ok) {  // (whatever the slot says, which may still be on its way)
+                load_rotation(p.cos_t, p.sin_t, pos[u], p.rot, sub, c, sn);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f;
+            }
+            const uint4 normed = head_norm_rope<LPR>(raw[u], p.norm_w, p.eps, c, sn, rotates && pos_ok, sub, halfc, p.bf16_ops);
+            if (!value[u]) raw[u] = normed;
+            if (rotates && !pos_ok) report(p.status, 102, t[u], pos[u]);
+        }
+        if (!live[u]) continue;
+        __nv_bfloat16* dst = (value[u] ? p.v_cache : p.k_cache) + (slot[u] >> p.shift) * p.page_stride +
+                             (slot[u] & ((1ll << p.shift) - 1)) * p.token_stride + h[u] * p.head_stride;
+        *reinterpret_cast<uint4*>(dst + sub * 8) = raw[u];
+    }
 }
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -317,7 +331,11 @@ extern "C" int s1_block_tables(s1_ctx* ctx, const int32_t* cached, const int32_t
     TableParams p{cached, added, num_seqs, __builtin_ctz(page_size), free_pages, free_capacity, free_count, free_count_out, tables, ldt, table_width,
                   lengths, cu_seqlens, positions, slots, max_tokens, ctx->status_dev};
     const int smem = static_cast<int>(sizeof(int32_t)) * (3 * num_seqs + 1);
-    S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (3 * kMaxTableRows + 1)));
+    static std::atomic<unsigned long long> told{0};  // one bit per device
+    if (!(told.load(std::memory_order_relaxed) >> (ctx->device & 63) & 1)) {
+        S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (3 * kMaxTableRows + 1)));
+        told.fetch_or(1ull << (ctx->device & 63), std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     // one block up to four tokens a thread, then more blocks, up to the eight of a portable cluster
@@ -380,8 +398,11 @@ extern "C" int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long lo
     }
     if (total_tokens == 0) return S1_OK;
     const int lpr = head_dim / 8;
-    const long long rows = 2LL * total_tokens * kv_heads, per_block = 8 * (32 / lpr), blocks = (rows + per_block - 1) / per_block;
-    if (blocks > 2147483647LL) return s1_fail(ctx, S1_EINVAL, "%s: too many rows", who);
+    // two groups of rows a warp from where that gives every scheduler four warps (see the kernel)
+    const long long rows = 2LL * total_tokens * kv_heads, groups = (rows * lpr + 31) / 32;
+    const int unroll = !norm_weight && groups >= 2LL * 16 * ctx->sm_count ? 2 : 1;
+    const long long per_block = 8LL * unroll * (32 / lpr), blocks = (rows + per_block - 1) / per_block;
+    if (rows > (1LL << 30)) return s1_fail(ctx, S1_EINVAL, "%s: too many rows", who);
     S1DeviceGuard guard(ctx->device);
     if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
     WriteParams p{static_cast<const __nv_bfloat16*>(k), ldk, k_head_stride, static_cast<const __nv_bfloat16*>(v), ldv, v_head_stride, slots, total_tokens,
@@ -389,10 +410,11 @@ extern "C" int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long lo
                   static_cast<__nv_bfloat16*>(k_cache), static_cast<__nv_bfloat16*>(v_cache), static_cast<long long>(num_pages) * page_size,
                   __builtin_ctz(page_size), page_stride, token_stride, head_stride, ctx->status_dev};
     const unsigned grid = static_cast<unsigned>(blocks);
-#define S1_WRITE(LPR_)                                                                       \
-    do {                                                                                     \
-        if (norm_weight) s1_cache_write_kernel<LPR_, true><<<grid, 256, 0, ctx->stream>>>(p); \
-        else s1_cache_write_kernel<LPR_, false><<<grid, 256, 0, ctx->stream>>>(p);            \
+#define S1_WRITE(LPR_)                                                                                              \
+    do {                                                                                                            \
+        if (norm_weight) s1_cache_write_kernel<LPR_, true, 1><<<grid, 256, 0, ctx->stream>>>(p);                     \
+        else if (unroll == 2) s1_cache_write_kernel<LPR_, false, 2><<<grid, 256, 0, ctx->stream>>>(p);              \
+        else s1_cache_write_kernel<LPR_, false, 1><<<grid, 256, 0, ctx->stream>>>(p);                               \
     } while (0)
     if (lpr == 8) S1_WRITE(8);
     else if (lpr == 16) S1_WRITE(16);
