@@ -505,57 +505,64 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
 }
 
 // Joins the pieces of the span that began in CTA blockIdx.x of the first kernel and went on in the CTAs after it, for one of its
-// heads (blockIdx.y). There may be over a hundred pieces when one context is alone, so the warps share them and request
-// theirs independently of one another: the common maximum comes from the marks first.
+// heads (blockIdx.y). There may be over a hundred pieces when one context is alone: a thread looks at one mark each, and the warps
+// share the pieces, so that the block waits for the record, the marks and the pieces once each.
+constexpr int kJoinThreads = 512;
 template <int D>
-__global__ void __launch_bounds__(256) s1_attention_paged_join_kernel(const PagedParams p) {
-    constexpr int kVec = D / 32;  // dims of a lane
-    __shared__ float sums[kWarps][D];
+__global__ void __launch_bounds__(kJoinThreads) s1_attention_paged_join_kernel(const PagedParams p) {
+    constexpr int kVec = D / 32, kJoinWarps = kJoinThreads / 32;
+    __shared__ float sums[kJoinWarps][D];
+    __shared__ float weights[kJoinThreads];
+    __shared__ float tops[kJoinWarps], totals[kJoinWarps];
     griddep_wait();
     const int4 rec = p.records[blockIdx.x];
     if (rec.z < 0) return;
     const int h = blockIdx.y, kvh = rec.y / p.blocks_per_group, hb = rec.y % p.blocks_per_group;
     if (h >= min(kHeads, p.group - hb * kHeads)) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int head = kvh * p.group + hb * kHeads + h;
     float gate = 0.f;
-    if (p.gate && threadIdx.x < D) gate = __bfloat162float(p.gate[rec.x * p.ldg + head * p.gate_head_stride + threadIdx.x]);
+    if (p.gate && tid < D) gate = __bfloat162float(p.gate[rec.x * p.ldg + head * p.gate_head_stride + tid]);
     const int first = blockIdx.x, pieces = rec.z - first + 1;  // piece i: of CTA first + i, its second (i = 0) or its first
     auto place = [&](int i) { return (2 * (first + i) + (i == 0 ? 1 : 0)) * kHeads + h; };
-    float top = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.marks[place(i)].x);
+    const float2 mark = tid < pieces ? p.marks[place(tid)] : make_float2(-INFINITY, 0.f);
+    float top = mark.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    auto weight = [&](float t) { return t == -INFINITY ? 0.f : exp2_fast(t - top); };
-    float sum = 0.f;
-    for (int i = lane; i < pieces; i += 32) {
-        const float2 m = p.marks[place(i)];
-        sum += m.y * weight(m.x);
-    }
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
+    const float weight = mark.x == -INFINITY ? 0.f : exp2_fast(mark.x - top);
+    weights[tid] = weight;
+    float sum = mark.y * weight;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) totals[warp] = sum;
+    __syncthreads();
     float x[kVec] = {};
 #pragma unroll 4
-    for (int i = warp; i < pieces; i += kWarps) {
-        const float f = weight(p.marks[place(i)].x);
+    for (int i = warp; i < pieces; i += kJoinWarps) {
+        const float f = weights[i];
         const float* part = p.parts + static_cast<long long>(place(i)) * D + lane;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) x[e] = fmaf(f, part[32 * e], x[e]);
+        for (int e = 0; e < kVec; ++e) x[e] = fmaf(f, __ldcg(part + 32 * e), x[e]);
     }
 #pragma unroll
     for (int e = 0; e < kVec; ++e) sums[warp][lane + 32 * e] = x[e];
     __syncthreads();
-    if (threadIdx.x < D) {
-        float y = 0.f;
+    if (tid < D) {
+        float y = 0.f, total = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) y += sums[w][threadIdx.x];
-        y = sum == 0.f ? 0.f : y / sum;
+        for (int w = 0; w < kJoinWarps; ++w) y += sums[w][tid], total += totals[w];
+        y = total == 0.f ? 0.f : y / total;
         if (p.gate) y *= sigmoid_fast(gate);
-        p.out[rec.x * p.ldo + head * D + threadIdx.x] = __float2bfloat16_rn(y);
+        p.out[rec.x * p.ldo + head * D + tid] = __float2bfloat16_rn(y);
     }
 }
 
 constexpr int kMaxCtas = 256;  // the workspace's share: more than one CTA per SM of any sm_100 part
+static_assert(kMaxCtas <= kJoinThreads, "the join looks at one piece a thread");
 
 size_t workspace_bytes_of(int head_dim) {
     return sizeof(int4) * kMaxCtas + 2 * kMaxCtas * kHeads * (sizeof(float2) + sizeof(float) * static_cast<size_t>(head_dim));
@@ -575,7 +582,7 @@ int launch(s1_ctx* ctx, const PagedParams& p, int ctas) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(ctas, std::min(kHeads, p.group)), cfg.blockDim = dim3(256), cfg.stream = ctx->stream;
+    cfg.gridDim = dim3(ctas, std::min(kHeads, p.group)), cfg.blockDim = dim3(kJoinThreads), cfg.stream = ctx->stream;
     cfg.attrs = attr, cfg.numAttrs = 1;
     S1_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, s1_attention_paged_join_kernel<D>, p));
     ctx->launches += 2;
