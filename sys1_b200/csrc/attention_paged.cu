@@ -6,13 +6,16 @@
 // What bounds it: every key and value is read once for the query heads that share it, 4 * group flops per 4 bytes - HBM, whatever
 // the group size. So the kernel is built around the loads:
 //  * work is cut into units of kUnit keys of one (row, KV head, up to 8 query heads) - a "span" is all units of one such triple -
-//    and the units of the whole batch, in order, are dealt out in equal contiguous ranges, one to each of the grid's CTAs. The
-//    CTAs find their ranges from the lengths in device memory, so that nothing of a step depends on the host and the balance holds
-//    for one long context and for many ragged ones alike. A span that crosses from one CTA to the next leaves partial results
-//    (maximum, sum, unnormalised output in f32) in the workspace, at most two per CTA, and the second kernel joins them in the order
-//    of the units: results do not depend on timing.
+//    and the units of the whole batch, in order, are dealt out in contiguous ranges of equal cost, one to each CTA of the grid; a
+//    span's beginning is counted too, as so many units (kStart; without it 32 short contexts beside 30 of 8192 tokens took 340 us,
+//    with it 209). The CTAs find their ranges from the lengths in device memory, so that nothing of a step depends on the host and
+//    the balance holds for one long context and for many ragged ones alike. A span that crosses from one CTA to the next leaves
+//    partial results (maximum, sum, unnormalised output in f32) in the workspace, at most two per CTA; and a second
+//    kernel joins them, in the order of the units: results do not depend on timing. (Joined by the CTA that finds all pieces of a
+//    span there, without the second kernel, the pieces were one CTA's work: 32 contexts up to 2048 took 27 us instead of 21.)
 //  * inside a CTA the warps take tiles of 16 keys in turn, each through a ring of its own in shared memory (cp.async, 24 KB a warp,
-//    192 KB an SM in flight or in use): no warp waits for another until its span is done.
+//    192 KB an SM in flight or in use): no warp waits for another until its span is done. The next span's first keys are fetched into
+//    L2 and its queries into registers while the warps' results are put together.
 //  * the products run on mma.sync m16n8k16 with the operands turned round - S^T = K Q^T, O^T = V^T P^T - so that the 16 rows are
 //    keys and head dimensions, which there are enough of, and the 8 columns the query heads of the group. tcgen05 would want 64 or
 //    128 rows of queries where there are 1 to 16; at the rate that HBM delivers keys, mma.sync is a fifth busy.
@@ -111,7 +114,12 @@ __device__ __forceinline__ int row_length(const PagedParams& p, int b, bool tell
     }
     return len;
 }
-__device__ __forceinline__ float sigmoid_fast(float x) { return 1.f / (1.f + exp2_fast(-1.4426950408889634f * x)); }
+__device__ __forceinline__ float rcp_fast(float x) {  // relative error 2^-23, before a rounding to bf16
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.f + exp2_fast(-1.4426950408889634f * x)); }
 __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
@@ -294,7 +302,7 @@ struct WarpPass {
 };
 
 struct Walk {        // a run over a range of the batch's costs
-    long long at, last;
+    int at, last;
     int b, kvh, hb;  // row, KV head, which eight query heads of its group
     int inside;      // cost inside that span
 };
@@ -315,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     __shared__ float2 marks_all[kHeads];
     constexpr int kQueryRow = D + 8;                     // eight rows that a warp reads by columns without bank conflicts
     __shared__ __align__(16) __nv_bfloat16 queries[kHeads][kQueryRow];
-    __shared__ long long warp_costs[kWarps];
+    __shared__ int warp_costs[kWarps];
     __shared__ Walk begin_sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x, ctas = gridDim.x;
@@ -327,44 +335,43 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
         if (row_length(p, b, lane == 0) == 0)
             for (int i = lane * 8; i < p.heads * D; i += 256) *reinterpret_cast<uint4*>(p.out + b * p.ldo + i) = make_uint4(0, 0, 0, 0);
 
-    // ---- this CTA's range
+    // ---- this CTA's range (the host has seen to it that all costs together fit 31 bits)
     auto cost_of = [&](int b) {
         const int units = (row_length(p, b, false) + kUnit - 1) / kUnit;
-        return units ? static_cast<long long>(units + kStart<D>) * p.spans_per_row : 0ll;
+        return units ? (units + kStart<D>) * p.spans_per_row : 0;
     };
     const int per = (p.num_seqs + kThreads - 1) / kThreads;
     const int rb = min(tid * per, p.num_seqs), re = min(rb + per, p.num_seqs);
-    long long mine = 0;
+    int mine = 0;
     for (int b = rb; b < re; ++b) mine += cost_of(b);
-    long long upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+        const int t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += t;
     }
     if (lane == 31) warp_costs[warp] = upto;
     __syncthreads();
-    long long before = 0, total = 0;
+    int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         if (w < warp) before += warp_costs[w];
         total += warp_costs[w];
     }
-    const int workers = static_cast<int>(min(static_cast<long long>(ctas), total));
+    const int workers = min(ctas, total);
     if (cta >= workers) {
         if (tid == 0) p.records[cta] = make_int4(0, 0, -1, 0);
         return;
     }
+    const int share = total / workers, longer = total - share * workers;  // the first `longer` CTAs have one more
     {
-        const long long first = total * cta / workers, at = before + upto - mine;
+        const int first = share * cta + min(cta, longer), at = before + upto - mine;
         if (first >= at && first < at + mine) {
-            long long u = at;
-            int b = rb;
-            for (long long n; b + 1 < re && u + (n = cost_of(b)) <= first; ++b) u += n;
-            const long long cost = cost_of(b) / p.spans_per_row;
-            const int span = static_cast<int>((first - u) / cost);
-            begin_sh = Walk{first, total * (cta + 1) / workers, b, span / p.blocks_per_group, span % p.blocks_per_group,
-                            static_cast<int>((first - u) % cost)};
+            int u = at, b = rb;
+            for (int n; b + 1 < re && u + (n = cost_of(b)) <= first; ++b) u += n;
+            const int cost = (row_length(p, b, false) + kUnit - 1) / kUnit + kStart<D>;
+            const int span = (first - u) / cost, kvh = span / p.blocks_per_group;
+            begin_sh = Walk{first, first + share + (cta < longer ? 1 : 0), b, kvh, span - kvh * p.blocks_per_group, first - u - span * cost};
         }
     }
     __syncthreads();
@@ -376,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
                 ++walk.b;
                 continue;
             }
-            const int at = walk.inside, step = static_cast<int>(min(static_cast<long long>(cost - at), walk.last - walk.at));
+            const int at = walk.inside, step = min(cost - at, walk.last - walk.at);
             s.b = walk.b, s.kvh = walk.kvh, s.hb = walk.hb, s.units = units;
             s.u0 = max(0, at - kStart<D>), s.n = max(0, at + step - kStart<D>) - s.u0;
             s.end = min(len, (s.u0 + s.n) * kUnit);
@@ -415,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     while (more) {
         const int h0 = now.kvh * p.group + now.hb * kHeads, nh = min(kHeads, p.group - now.hb * kHeads);
         const bool whole = now.u0 == 0 && now.n == now.units;
-        const long long stop = walk.at;  // where this segment ends
+        const int stop = walk.at;  // where this segment ends
         more = advance(next);
         // where the next span's keys begin for this warp: looked up now, wanted when this span is done
         int next_j = next.u0 * kUnit + warp * kTile + lane;
@@ -483,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
                 x.x += w < parts ? y.x : 0.f, x.y += w < parts ? y.y : 0.f;
             }
             if (whole) {
-                const float inv = marks_all[h].y == 0.f ? 0.f : 1.f / marks_all[h].y;
+                const float inv = marks_all[h].y == 0.f ? 0.f : rcp_fast(marks_all[h].y);
                 x.x *= inv, x.y *= inv;
                 if (p.gate) x.x *= sigmoid_fast(__uint_as_float(gates[i] << 16)), x.y *= sigmoid_fast(__uint_as_float(gates[i] & 0xffff0000u));
                 *reinterpret_cast<uint32_t*>(p.out + now.b * p.ldo + (h0 + h) * D + d) = pack2(x.x, x.y);
@@ -493,8 +500,10 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
         }
         if (!whole) {
             if (tid < nh) p.marks[piece * kHeads + tid] = marks_all[tid];
-            // a span that begins here and is cut at the end of this CTA's range: the CTA that has its last unit
-            if (now.u0 == 0) record = make_int4(now.b, now.kvh * p.blocks_per_group + now.hb, static_cast<int>(((stop - now.n + now.units) * workers - 1) / total), 0);
+            if (now.u0 == 0) {  // a span that begins here and is cut at the end of this CTA's range: the CTA that has its last unit
+                const int end = stop - now.n + now.units - 1, border = longer * (share + 1);
+                record = make_int4(now.b, now.kvh * p.blocks_per_group + now.hb, end < border ? end / (share + 1) : longer + (end - border) / share, 0);
+            }
         }
         hand_q(next_q);
         __syncthreads();  // the stage is a ring again
@@ -555,7 +564,7 @@ __global__ void __launch_bounds__(kJoinThreads) s1_attention_paged_join_kernel(c
         float y = 0.f, total = 0.f;
 #pragma unroll
         for (int w = 0; w < kJoinWarps; ++w) y += sums[w][tid], total += totals[w];
-        y = total == 0.f ? 0.f : y / total;
+        y = total == 0.f ? 0.f : y * rcp_fast(total);
         if (p.gate) y *= sigmoid_fast(gate);
         p.out[rec.x * p.ldo + head * D + tid] = __float2bfloat16_rn(y);
     }
@@ -627,13 +636,16 @@ extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, lon
     S1DeviceGuard guard(ctx->device);
     if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
     const int group = heads / kv_heads, blocks = (group + kHeads - 1) / kHeads;
-    float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas);
+    if (static_cast<long long>(num_seqs) * kv_heads * blocks > (1ll << 31) / ((static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit + 4) - 1)
+        return s1_fail(ctx, S1_EINVAL, "%s: rows x KV heads x (tokens of a block table) / 128 must be below 2^31", who);    float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas);
     PagedParams p{static_cast<const __nv_bfloat16*>(q), ldq, q_head_stride, static_cast<const __nv_bfloat16*>(k_cache),
                   static_cast<const __nv_bfloat16*>(v_cache), page_stride, token_stride, head_stride, num_pages, __builtin_ctz(page_size), tables, ldt,
                   table_width, lengths, num_seqs, heads, kv_heads, group, kv_heads * blocks, blocks, scale * 1.4426950408889634f,
                   static_cast<const __nv_bfloat16*>(gate), ldg, gate_head_stride, static_cast<__nv_bfloat16*>(out), ldo,
                   reinterpret_cast<float*>(marks + 2 * kMaxCtas * kHeads), marks, static_cast<int4*>(workspace), ctx->status_dev};
-    const int ctas = std::min(ctx->sm_count, kMaxCtas);
+    // one CTA per SM, and no more than the block tables could make units of
+    const long long most = static_cast<long long>(num_seqs) * kv_heads * blocks * ((static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit + 4);
+    const int ctas = static_cast<int>(std::min<long long>(std::min(ctx->sm_count, kMaxCtas), most));
     if (head_dim == 64) return launch<64>(ctx, p, ctas);
     if (head_dim == 128) return launch<128>(ctx, p, ctas);
     return launch<256>(ctx, p, ctas);
