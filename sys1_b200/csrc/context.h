@@ -151,8 +151,8 @@ inline void s1_keep_projection_split(Kernel kernel) {
 int s1_exchange_launch(s1_ctx* ctx, void* buf, size_t count, cudaStream_t stream);
 
 // Leaves the last rows before the conv of every sequence in the rings that s1_gated_delta_rule_step reads (delta_step.cu).
-int s1_conv_state_launch(s1_ctx* ctx, const void* mixed, long long ldm, const int32_t* cu_seqlens, int num_seqs, const int32_t* index, int num_states,
-                         int channels, void* conv_state);
+int s1_conv_state_launch(s1_ctx* ctx, const void* mixed, long long ldm, const int32_t* cu_seqlens, int num_seqs, int total_tokens, const int32_t* index,
+                         int num_states, int channels, void* conv_state);
 
 int s1_get_tmap(s1_ctx* ctx, const void* ptr, long long rows, long long cols, long long ld, int box_rows,
                 int box_cols, int elem_bytes, int swizzle_bytes, CUtensorMap* out);

@@ -1113,7 +1113,7 @@ static int gated_delta_rule(s1_ctx* ctx, const char* who, const void* mixed, lon
                          static_cast<uint8_t*>(workspace) + obytes, workspace_bytes - obytes, kept);
     if (rc) return rc;
     if (kept.state) {
-        rc = s1_conv_state_launch(ctx, mixed, ldm, kept.cu_seqlens, num_seqs, kept.index, kept.num_states, static_cast<int>(width), kept.conv_state);
+        rc = s1_conv_state_launch(ctx, mixed, ldm, kept.cu_seqlens, num_seqs, total_tokens, kept.index, kept.num_states, static_cast<int>(width), kept.conv_state);
         if (rc) return rc;
     }
     return s1_delta_finish(ctx, o, z, ldz, norm_weight, eps, total_tokens, value_heads, y, ldy);
@@ -1151,7 +1151,7 @@ extern "C" int s1_gated_delta_rule_prefill(s1_ctx* ctx, const void* mixed_before
     const char* who = "s1_gated_delta_rule_prefill";
     if (!ctx) return S1_EINVAL;
     if (!conv_weight || !positions || !cu_seqlens || !state_index || !conv_state || !state) return s1_fail(ctx, S1_EINVAL, "%s: null pointer", who);
-    if (num_states < 1 || num_seqs > 65535) return s1_fail(ctx, S1_EINVAL, "%s: %d sequences, %d states", who, num_seqs, num_states);
+    if (num_states < 1) return s1_fail(ctx, S1_EINVAL, "%s: %d states", who, num_states);
     if ((reinterpret_cast<uintptr_t>(conv_state) | reinterpret_cast<uintptr_t>(state)) & 15u)
         return s1_fail(ctx, S1_EINVAL, "%s: the states must be 16-byte aligned", who);
     KeptState kept;

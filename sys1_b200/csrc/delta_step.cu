@@ -253,9 +253,9 @@ __global__ void __launch_bounds__(kThreads, 2) s1_delta_step_kernel(const StepPa
 
 // The last rows before the conv of every sequence of a prompt batch into the ring that the step kernel reads.
 __global__ void __launch_bounds__(256) s1_conv_state_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const int32_t* __restrict__ cu,
-                                                            const int32_t* __restrict__ index, int num_states, int C, __nv_bfloat16* __restrict__ ring) {
+                                                            const int32_t* __restrict__ index, int num_states, int total_tokens, int C, __nv_bfloat16* __restrict__ ring) {
     const int s = blockIdx.x, back = blockIdx.y;  // the token `back` before the sequence's last
-    const int slot = index[s], a = cu[s], len = cu[s + 1] - a;
+    const int slot = index[s], a = cu[s], end = cu[s + 1], len = a >= 0 && end <= total_tokens ? end - a : 0;
     // a slot that does not exist, or that a sequence before this one has, is left alone, like the state (delta_chunked.cu reports it)
     bool bad = slot >= num_states;
     for (int j = threadIdx.x; slot >= 0 && j < s; j += 256) bad = bad || (index[j] == slot && cu[j + 1] > cu[j]);
@@ -271,10 +271,10 @@ inline bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintpt
 
 }  // namespace
 
-int s1_conv_state_launch(s1_ctx* ctx, const void* mixed, long long ldm, const int32_t* cu_seqlens, int num_seqs, const int32_t* index, int num_states,
-                         int channels, void* conv_state) {
+int s1_conv_state_launch(s1_ctx* ctx, const void* mixed, long long ldm, const int32_t* cu_seqlens, int num_seqs, int total_tokens, const int32_t* index,
+                         int num_states, int channels, void* conv_state) {
     s1_conv_state_kernel<<<dim3(num_seqs, kTaps), 256, 0, ctx->stream>>>(static_cast<const __nv_bfloat16*>(mixed), ldm, cu_seqlens, index, num_states,
-                                                                         channels, static_cast<__nv_bfloat16*>(conv_state));
+                                                                         total_tokens, channels, static_cast<__nv_bfloat16*>(conv_state));
     S1_CUDA_OK(ctx, cudaGetLastError());
     ctx->launches += 1;
     return S1_OK;

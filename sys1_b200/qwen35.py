@@ -519,20 +519,24 @@ class Decoder:
         for n in lengths:
             bounds.append(bounds[-1] + n)
         plan = cache.enter(rows, lengths)
-        cu, index = torch.tensor([bounds, rows + [0]], dtype=torch.int32).to(ids.device)
-        x = _norm.embedding(self.w["embed_tokens"], ids.to(torch.int32).contiguous())
         previous = getattr(ctx, "_plan", None)
-        ctx.use_plan(batch_plan_cached(self, ctx, bounds))
         try:
+            cu, index = torch.tensor([bounds, rows + [0]], dtype=torch.int32).to(ids.device)
+            x = _norm.embedding(self.w["embed_tokens"], ids.to(torch.int32).contiguous())
+            ctx.use_plan(batch_plan_cached(self, ctx, bounds))
             for layer, part in zip(self.layers, cache.layers):
                 x = layer.forward(x, bounds, plan.positions, inplace=True, kept=Kept(part, plan.positions, plan.slots, index, cu_seqlens=cu))
+            x = self.norm(x)
+        except BaseException:
+            cache.release(rows)   # half a prompt is of no use to a step
+            raise
         finally:
             ctx.use_plan(previous)
-        return self.norm(x), rows
+        return x, rows
 
     def step(self, ids: torch.Tensor, cache: "paged.PagedCache") -> torch.Tensor:
-        """One new token of every active row of the cache: `ids [cache.rows]` (CUDA; those of idle rows are not looked at further than
-        the embedding). Returns the hidden states `[cache.rows, hidden]` after the final norm; the rows of idle requests mean nothing.
+        """One new token of every active row of the cache: `ids [cache.rows]` (CUDA; idle rows need an id of the vocabulary too,
+        which is of no account). Returns the hidden states `[cache.rows, hidden]` after the final norm; the rows of idle requests mean nothing.
         Can be captured into a CUDA graph and replayed (`cache.advanced` tells the host's mirror)."""
         if ids.dim() != 1 or not ids.is_cuda or ids.shape[0] != cache.rows:
             raise ValueError(f"ids must be a CUDA tensor [{cache.rows}], a token for every row of the cache (no CPU fallback)")

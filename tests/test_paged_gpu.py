@@ -345,6 +345,48 @@ def test_paged_attention_refusals(ctx):
     assert paged.attention_paged(q[:0], kc, vc, tables[:0], lengths[:0]).shape == (0, 256)
 
 
+def test_paged_attention_captured_follows_its_lengths(ctx):
+    """A captured call works from the lengths and tables that are there when it is replayed."""
+    lens = [700, 30, 0, 129]
+    q, kc, vc, tables, lengths, gate = _attention_case([900] * 4, 8, 2, 128, 16, 21, poison=False)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        other = device.load(0)
+        paged.attention_paged(q, kc, vc, tables, lengths, gate=gate)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate)
+        for n in (lens, [1] * 4, [900] * 4, [0] * 4, [5, 800, 16, 17]):
+            lengths.copy_(ints(n))
+            graph.replay()
+            got = out.clone()
+            assert torch.equal(got, paged.attention_paged(q, kc, vc, tables, ints(n), gate=gate))
+            _check_attention(got, q, kc, vc, tables, n, gate)
+        other.sync()
+
+
+def test_two_streams_at_once(ctx):
+    """Calls that run at the same time on two streams (each with its own context and workspace) give what they give alone."""
+    cases = [_attention_case([3000, 1, 900], 8, 2, 128, 16, 31), _attention_case([10, 2500, 70], 8, 2, 128, 16, 32)]
+    steps = [_step_case(9, 2, 4, 33), _step_case(9, 2, 4, 34)]
+    alone = [paged.attention_paged(*c[:5], gate=c[5]) for c in cases]
+    after = [dict(c, state=c["state"].clone(), conv_state=c["conv_state"].clone()) for c in steps]
+    for _ in range(5):
+        [qwen35.gated_delta_rule_step(**c) for c in after]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = paged.attention_paged(*cases[i][:5], gate=cases[i][5])
+                qwen35.gated_delta_rule_step(**steps[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i], alone[i]) and torch.equal(steps[i]["state"], after[i]["state"])
+
+
 # ------------------------------------------------------------------------------------------------ delta rule
 def _step_case(rows, keys, values, seed, states=None, fresh=(), idle=()):
     g, h = gen(seed), np.random.RandomState(seed)
@@ -411,6 +453,20 @@ def test_delta_step_reports_bad_states(ctx, what):
     want = qwen35.gated_delta_rule_step(**good)
     ctx.sync()
     assert torch.equal(y, want) and torch.equal(c["state"], good["state"]) and torch.equal(c["conv_state"], good["conv_state"])
+
+
+def test_delta_step_of_many_rows(ctx):
+    """More rows than a block has threads (a state given twice is found there too), more pairs of rows and heads than blocks."""
+    c = _step_case(700, 1, 1, 12, fresh=range(0, 700, 9), idle=range(3, 700, 11))
+    y64, yb, S64, Sb, ring = _step_reference(c)
+    y = qwen35.gated_delta_rule_step(**c)
+    ctx.sync()
+    assert torch.equal(c["conv_state"], ring) and bool(((y.double() - y64).abs() <= yb).all()) and bool(((c["state"].double() - S64).abs() <= Sb).all())
+    c["state_index"][699] = c["state_index"][601] if int(c["state_index"][601]) >= 0 else c["state_index"][602]
+    before = c["state"].clone()
+    qwen35.gated_delta_rule_step(**c)
+    _refused(ctx, "row 699 has state")
+    assert not torch.equal(c["state"], before) and bool(torch.isfinite(c["state"]).all())
 
 
 def test_delta_step_refusals(ctx):
@@ -578,6 +634,20 @@ def test_a_captured_step_is_the_step(ctx):
             assert torch.equal(x.state[:2], y.state[:2]) and torch.equal(x.conv[:2], y.conv[:2])
     with pytest.raises(ValueError, match="do not fit"):
         b.advanced(100)
+
+
+def test_a_prefill_that_fails_leaves_the_cache_as_it_was(ctx, monkeypatch):
+    cfg, w, dec = _decoder(layers=2)
+    cache = paged.PagedCache(cfg, rows=3, num_pages=8, page_size=16, max_length=64, dev=DEV)
+    ids = torch.zeros(40, dtype=torch.int64, device=DEV)
+    dec.prefill(ids[:20], [20], cache)
+    with monkeypatch.context() as m:
+        m.setattr(dec.layers[1].mlp, "forward", lambda *a, **k: (_ for _ in ()).throw(RuntimeError("no")))
+        with pytest.raises(RuntimeError, match="no"):
+            dec.prefill(ids, [40], cache)
+    ctx.sync()
+    assert cache.held.tolist() == [20, -1, -1] and cache.lengths.tolist() == [20, -1, -1] and cache.free_count.tolist() == [6] == [cache.pages_left]
+    assert cache.state_index.tolist() == [0, -1, -1]
 
 
 def test_the_cache_refuses_what_does_not_fit(ctx):
