@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x, ctas = gridDim.x;
 
+    griddep_wait();
     griddep_launch_dependents();  // the join's blocks may take the SMs that run out of work first (they wait for the whole grid)
 
     // ---- rows without a key: zeros
@@ -524,6 +525,7 @@ __global__ void __launch_bounds__(kJoinThreads) s1_attention_paged_join_kernel(c
     __shared__ float weights[kJoinThreads];
     __shared__ float tops[kJoinWarps], totals[kJoinWarps];
     griddep_wait();
+    griddep_launch_dependents();
     const int4 rec = p.records[blockIdx.x];
     if (rec.z < 0) return;
     const int h = blockIdx.y, kvh = rec.y / p.blocks_per_group, hb = rec.y % p.blocks_per_group;
@@ -585,15 +587,9 @@ int launch(s1_ctx* ctx, const PagedParams& p, int ctas) {
         S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         told.fetch_or(1ull << (ctx->device & 63), std::memory_order_relaxed);
     }
-    s1_attention_paged_kernel<D><<<ctas, kThreads, smem, ctx->stream>>>(p);
-    S1_CUDA_OK(ctx, cudaGetLastError());
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(ctas, std::min(kHeads, p.group)), cfg.blockDim = dim3(kJoinThreads), cfg.stream = ctx->stream;
-    cfg.attrs = attr, cfg.numAttrs = 1;
-    S1_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, s1_attention_paged_join_kernel<D>, p));
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D>, static_cast<unsigned>(ctas), 1u, kThreads, smem, p));
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_join_kernel<D>, static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(kHeads, p.group)),
+                                      kJoinThreads, 0, p));
     ctx->launches += 2;
     return S1_OK;
 }

@@ -17,6 +17,7 @@
 #include "context.h"
 #include "device_guard.h"
 #include "head_norm_rope.cuh"
+#include "ptx.cuh"
 
 using namespace s1;
 namespace cg = cooperative_groups;
@@ -92,6 +93,8 @@ __global__ void __launch_bounds__(kTableThreads) s1_block_tables_kernel(const Ta
     int32_t* old = off + p.num_seqs;              // [num_seqs] tokens before this call, negative: idle
     __shared__ unsigned warp_sums[33];
     __shared__ unsigned taken_sh;
+    griddep_wait();
+    griddep_launch_dependents();
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank()), blocks = static_cast<int>(cluster.num_blocks());
     const int tid = threadIdx.x;
@@ -195,6 +198,8 @@ __global__ void __launch_bounds__(kTableThreads) s1_release_blocks_kernel(const 
     __shared__ unsigned warp_sums[33];
     __shared__ unsigned put_sh;
     const int tid = threadIdx.x;
+    griddep_wait();
+    griddep_launch_dependents();
     const unsigned held = static_cast<unsigned>(min(max(*p.free_count, 0), p.free_capacity));
     if (tid == 0) put_sh = 0u;
     unsigned pages = 0;
@@ -259,6 +264,8 @@ template <int LPR, bool NORM, int U>
 __global__ void __launch_bounds__(256) s1_cache_write_kernel(const WriteParams p) {
     constexpr int RPW = 32 / LPR;
     const int lane = threadIdx.x & 31, sub = lane % LPR;
+    griddep_wait();
+    griddep_launch_dependents();
     const unsigned rows = static_cast<unsigned>(p.T) * static_cast<unsigned>(p.kv_heads);  // of keys; as many of values behind them
     const unsigned first = ((blockIdx.x * 256u + threadIdx.x) >> 5) * (RPW * U) + lane / LPR;
     uint4 raw[U];
@@ -336,15 +343,9 @@ extern "C" int s1_block_tables(s1_ctx* ctx, const int32_t* cached, const int32_t
         S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (3 * kMaxTableRows + 1)));
         told.fetch_or(1ull << (ctx->device & 63), std::memory_order_relaxed);
     }
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
     // one block up to four tokens a thread, then more blocks, up to the eight of a portable cluster
     const unsigned blocks = max_tokens <= 4 * kTableThreads ? 1u : max_tokens <= 8 * kTableThreads ? 2u : max_tokens <= 16 * kTableThreads ? 4u : 8u;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = blocks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(blocks), cfg.blockDim = dim3(kTableThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
-    cfg.attrs = attr, cfg.numAttrs = 1;
-    S1_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, s1_block_tables_kernel, p));
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_block_tables_kernel, blocks, 1u, kTableThreads, smem, p, blocks));
     ctx->launches += 1;
     return S1_OK;
 }
@@ -364,8 +365,7 @@ extern "C" int s1_release_blocks(s1_ctx* ctx, const int32_t* ended, int num_seqs
     ReleaseParams p{ended, num_seqs, __builtin_ctz(page_size), lengths, tables, ldt, table_width, free_pages, free_capacity, free_count, ctx->status_dev};
     const int smem = static_cast<int>(sizeof(int32_t)) * 2 * num_seqs;
     S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_release_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * 2 * kMaxTableRows));
-    s1_release_blocks_kernel<<<1, kTableThreads, smem, ctx->stream>>>(p);
-    S1_CUDA_OK(ctx, cudaGetLastError());
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_release_blocks_kernel, 1u, 1u, kTableThreads, smem, p));
     ctx->launches += 1;
     return S1_OK;
 }
@@ -409,18 +409,12 @@ extern "C" int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long lo
                   kv_heads, static_cast<const __nv_bfloat16*>(norm_weight), eps, cos_table, sin_table, positions, max_positions, rotary_dim, bf16_ops,
                   static_cast<__nv_bfloat16*>(k_cache), static_cast<__nv_bfloat16*>(v_cache), static_cast<long long>(num_pages) * page_size,
                   __builtin_ctz(page_size), page_stride, token_stride, head_stride, ctx->status_dev};
-    const unsigned grid = static_cast<unsigned>(blocks);
-#define S1_WRITE(LPR_)                                                                                              \
-    do {                                                                                                            \
-        if (norm_weight) s1_cache_write_kernel<LPR_, true, 1><<<grid, 256, 0, ctx->stream>>>(p);                     \
-        else if (unroll == 2) s1_cache_write_kernel<LPR_, false, 2><<<grid, 256, 0, ctx->stream>>>(p);              \
-        else s1_cache_write_kernel<LPR_, false, 1><<<grid, 256, 0, ctx->stream>>>(p);                               \
-    } while (0)
-    if (lpr == 8) S1_WRITE(8);
-    else if (lpr == 16) S1_WRITE(16);
-    else S1_WRITE(32);
+    auto launch = [&](void (*kernel)(WriteParams)) { return s1_launch_waiting(ctx, kernel, static_cast<unsigned>(blocks), 1u, 256u, 0, p); };
+#define S1_WRITE(LPR_)                                                                                          \
+    launch(norm_weight ? s1_cache_write_kernel<LPR_, true, 1> : unroll == 2 ? s1_cache_write_kernel<LPR_, false, 2> \
+                                                                            : s1_cache_write_kernel<LPR_, false, 1>)
+    S1_CUDA_OK(ctx, lpr == 8 ? S1_WRITE(8) : lpr == 16 ? S1_WRITE(16) : S1_WRITE(32));
 #undef S1_WRITE
-    S1_CUDA_OK(ctx, cudaGetLastError());
     ctx->launches += 1;
     return S1_OK;
 }
