@@ -1,4 +1,5 @@
 """Shared fixtures. GPU tests are marked `gpu`; everything else runs on a CPU-only box."""
+import gc
 import os
 import subprocess
 import sys
@@ -28,6 +29,14 @@ def _built_artifacts():
     if not so.exists():
         subprocess.run(["make", "-C", str(ROOT / "oracle" / "c")], check=False, capture_output=True)
     yield
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _nothing_left_behind():
+    """What a module's tests leave in reference cycles (the frames of caught errors hold their tensors) goes when the module is done,
+    and not while a later test counts the allocator's bytes."""
+    yield
+    gc.collect()
 
 
 @pytest.fixture(scope="session")
