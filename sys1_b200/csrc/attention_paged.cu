@@ -5,7 +5,7 @@
 //
 // What bounds it: every key and value is read once for the query heads that share it, 4 * group flops per 4 bytes - HBM, whatever
 // the group size. So the kernel is built around the loads:
-//  * work is cut into units of kUnit keys of one (row, KV head, up to 8 query heads) - a "span" is all units of one such triple -
+//  * work is cut into units of kUnit keys of one (row, KV head, 8 or 16 of its query heads) - a "span" is all units of one such triple -
 //    and the units of the whole batch, in order, are dealt out in contiguous ranges of equal cost, one to each CTA of the grid; a
 //    span's beginning is counted too, as so many units (kStart; without it 32 short contexts beside 30 of 8192 tokens took 340 us,
 //    with it 209). The CTAs find their ranges from the lengths in device memory, so that nothing of a step depends on the host and
@@ -40,7 +40,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;               // keys of one warp step
 constexpr int kUnit = kWarps * kTile;   // keys of one unit of work
-constexpr int kHeads = 8;               // query heads of one span (columns of the MMAs)
+constexpr int kCols = 8;                // query heads of one MMA (its columns); a span has NT times as many
 constexpr int kRingBytes = 24 * 1024;   // per warp
 
 // What a span costs beyond its units (its queries, the first keys' way, the warps' results put together), in units of its head dim.
@@ -58,14 +58,14 @@ struct PagedParams {
     long long ldt;
     int table_width;
     const int32_t* lengths;
-    int num_seqs, heads, kv_heads, group, spans_per_row, blocks_per_group;
+    int num_seqs, heads, kv_heads, group, spans_per_row, blocks_per_group;  // blocks: of 8 NT heads
     float scale_log2;
     const __nv_bfloat16* gate;
     long long ldg, gate_head_stride;
     __nv_bfloat16* out;
     long long ldo;
-    float* parts;   // [2 * grid][kHeads][D]: unnormalised outputs of the cut spans' pieces
-    float2* marks;  // [2 * grid][kHeads]: maximum (in units of log2) and sum of the same pieces
+    float* parts;   // [2 * grid][heads of a span][D]: unnormalised outputs of the cut spans' pieces
+    float2* marks;  // [2 * grid][heads of a span]: maximum (in units of log2) and sum of the same pieces
     int4* records;  // [grid]: row, span of the row, last CTA of the span that begins in this CTA and is cut (or -1)
     int* status;
 };
@@ -124,22 +124,25 @@ __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
-// One warp's pass over its tiles of a span: keys first + 16 (warp + 8 i), below `end`.
-template <int D>
+// One warp's pass over its tiles of a span: keys first + 16 (warp + 8 i), below `end`. NT = 1: up to 8 query heads, held in registers;
+// NT = 2: up to 16, read from shared memory step by step, so that a group of more than 8 does not read its keys twice (32 x 8192
+// tokens, 16 heads to a KV head of 256: 166 us as two spans of 8, 98 as one of 16).
+template <int D, int NT>
 struct WarpPass {
     static constexpr int kSlotBytes = kTile * D * 2;
     static constexpr int kSlots = kRingBytes / kSlotBytes;  // 3, 6 or 12
     static constexpr int kChunks = D / 8;                   // 16-byte pieces of a key
     static constexpr int kRowsPerCopy = 32 / kChunks;
     static constexpr int kSteps = D / 16;
-    static constexpr int kChains = D == 256 ? 4 : 2;        // independent accumulators of S^T
+    static constexpr int kChains = D == 256 && NT == 1 ? 4 : 2;  // independent accumulators of S^T
+    static constexpr int kQueryRow = D + 8;                 // values of a row of queries in shared memory: no bank conflicts by columns
 
     const PagedParams& p;
     const int lane;
     const uint32_t ring;            // shared address of this warp's ring
     volatile uint32_t* masks;       // [kSlots] which of the 16 keys a slot holds
-    float O[kSteps][4];             // O^T: dims 16 s + lane/4 (+ 8), heads 2 (lane % 4) (+ 1)
-    float m[2], l[2];
+    float O[NT][kSteps][4];         // O^T: dims 16 s + lane/4 (+ 8), heads 8 t + 2 (lane % 4) (+ 1)
+    float m[NT][2], l[NT][2];
     const bool one_page;            // pages of 16 tokens and more: a tile never leaves its page
     long long off;                  // where the tile whose keys were requested last begins (one_page), or lane j's key of it
     uint32_t mask;                  // which of its keys there are
@@ -203,11 +206,27 @@ struct WarpPass {
     }
     __device__ __forceinline__ void load(int n) { request(n & 1, wslot, b, kvh, first + (n >> 1) * kUnit, end); }  // request number n
 
-    __device__ __forceinline__ void run(const uint32_t (&qf)[kSteps][2]) {
+    // `queries`: 8 NT rows of kQueryRow values in shared memory
+    __device__ __forceinline__ void run(const __nv_bfloat16* queries) {
+        uint32_t qf[NT == 1 ? kSteps : 1][2];
+        uint32_t qat = 0;
+        if constexpr (NT == 1) {
+            const __nv_bfloat16* q = queries + (lane >> 2) * kQueryRow + 2 * (lane & 3);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) O[s][0] = O[s][1] = O[s][2] = O[s][3] = 0.f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
+            for (int s = 0; s < kSteps; ++s) {
+                qf[s][0] = *reinterpret_cast<const uint32_t*>(q + 16 * s);
+                qf[s][1] = *reinterpret_cast<const uint32_t*>(q + 16 * s + 8);
+            }
+        } else {  // an ldmatrix for each step: heads 0 .. 7 of its two halves, then heads 8 .. 15
+            qat = smem_u32(queries + ((lane >> 4) * kCols + (lane & 7)) * kQueryRow + (lane >> 3 & 1) * 8);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) O[t][s][0] = O[t][s][1] = O[t][s][2] = O[t][s][3] = 0.f;
+            m[t][0] = m[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.f;
+        }
         int rslot = 0;
         // this lane's rows of the ldmatrix tiles: the 16-byte pieces 2 s + h of row r lie at r * 2 D + ((2 s + h) ^ (r & 7)) * 16, which is
         // one of four places and a multiple of 128 bytes
@@ -219,7 +238,7 @@ struct WarpPass {
         }
 #pragma unroll 1
         for (int n = 0; n < requests; n += 2) {
-            uint32_t pb0, pb1;
+            uint32_t pb[NT][2];
             // ---- keys: S^T = K Q^T
             asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
             __syncwarp();  // the slot has landed for every lane, and every lane is done with the one refilled next
@@ -228,51 +247,74 @@ struct WarpPass {
             wslot = wslot + 1 == kSlots ? 0 : wslot + 1;
             {
                 const uint32_t live = masks[rslot], slot = ring + rslot * kSlotBytes;
-                float c[kChains][4];
+                float c[NT][kChains][4];
 #pragma unroll
-                for (int i = 0; i < kChains; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < kChains; ++i) c[t][i][0] = c[t][i][1] = c[t][i][2] = c[t][i][3] = 0.f;
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
                     uint32_t a[4];
                     ldsm4(a, slot + kat[s & 3] + (s >> 2) * 128);
-                    mma16816(c[s % kChains], a, qf[s][0], qf[s][1]);
+                    if constexpr (NT == 1) {
+                        mma16816(c[0][s % kChains], a, qf[s][0], qf[s][1]);
+                    } else {
+                        uint32_t q[4];
+                        ldsm4(q, qat + 32 * s);
+                        mma16816(c[0][s % kChains], a, q[0], q[1]);
+                        mma16816(c[1][s % kChains], a, q[2], q[3]);
+                    }
                 }
-#pragma unroll
-                for (int i = 1; i < kChains; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) c[0][e] += c[i][e];
                 const bool in0 = live >> (lane >> 2) & 1u, in1 = live >> ((lane >> 2) + 8) & 1u;
-                float s[4];
-                s[0] = in0 ? c[0][0] * p.scale_log2 : -INFINITY;
-                s[1] = in0 ? c[0][1] * p.scale_log2 : -INFINITY;
-                s[2] = in1 ? c[0][2] * p.scale_log2 : -INFINITY;
-                s[3] = in1 ? c[0][3] * p.scale_log2 : -INFINITY;
-                float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+                float s[NT][4], top[NT][2];
+                bool grows = false;
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
-                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (int i = 1; i < kChains; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[t][0][e] += c[t][i][e];
+                    s[t][0] = in0 ? c[t][0][0] * p.scale_log2 : -INFINITY;
+                    s[t][1] = in0 ? c[t][0][1] * p.scale_log2 : -INFINITY;
+                    s[t][2] = in1 ? c[t][0][2] * p.scale_log2 : -INFINITY;
+                    s[t][3] = in1 ? c[t][0][3] * p.scale_log2 : -INFINITY;
+                    top[t][0] = fmaxf(s[t][0], s[t][2]), top[t][1] = fmaxf(s[t][1], s[t][3]);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        top[t][0] = fmaxf(top[t][0], __shfl_xor_sync(0xffffffffu, top[t][0], o));
+                        top[t][1] = fmaxf(top[t][1], __shfl_xor_sync(0xffffffffu, top[t][1], o));
+                    }
+                    grows = grows || top[t][0] > m[t][0] || top[t][1] > m[t][1];
                 }
                 if (n == 0) {
-                    m[0] = top[0], m[1] = top[1];
-                } else if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-                    float scale[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float now = fmaxf(m[e], top[e]);
-                        scale[e] = now == -INFINITY ? 1.f : exp2_fast(m[e] - now);
-                        m[e] = now;
-                        l[e] *= scale[e];
+                    for (int t = 0; t < NT; ++t) m[t][0] = top[t][0], m[t][1] = top[t][1];
+                } else if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        float scale[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float now = fmaxf(m[t][e], top[t][e]);
+                            scale[e] = now == -INFINITY ? 1.f : exp2_fast(m[t][e] - now);
+                            m[t][e] = now;
+                            l[t][e] *= scale[e];
+                        }
+#pragma unroll
+                        for (int i = 0; i < kSteps; ++i)
+                            O[t][i][0] *= scale[0], O[t][i][1] *= scale[1], O[t][i][2] *= scale[0], O[t][i][3] *= scale[1];
                     }
-#pragma unroll
-                    for (int t = 0; t < kSteps; ++t) O[t][0] *= scale[0], O[t][1] *= scale[1], O[t][2] *= scale[0], O[t][3] *= scale[1];
                 }
-                const float ref0 = m[0] == -INFINITY ? 0.f : m[0], ref1 = m[1] == -INFINITY ? 0.f : m[1];  // no key seen yet: all weights are 0
-                s[0] = exp2_fast(s[0] - ref0), s[1] = exp2_fast(s[1] - ref1), s[2] = exp2_fast(s[2] - ref0), s[3] = exp2_fast(s[3] - ref1);
-                l[0] += s[0] + s[2];
-                l[1] += s[1] + s[3];
-                pb0 = transpose8(pack2(s[0], s[1]));
-                pb1 = transpose8(pack2(s[2], s[3]));
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const float ref0 = m[t][0] == -INFINITY ? 0.f : m[t][0], ref1 = m[t][1] == -INFINITY ? 0.f : m[t][1];  // no key seen yet: all weights are 0
+                    s[t][0] = exp2_fast(s[t][0] - ref0), s[t][1] = exp2_fast(s[t][1] - ref1);
+                    s[t][2] = exp2_fast(s[t][2] - ref0), s[t][3] = exp2_fast(s[t][3] - ref1);
+                    l[t][0] += s[t][0] + s[t][2];
+                    l[t][1] += s[t][1] + s[t][3];
+                    pb[t][0] = transpose8(pack2(s[t][0], s[t][1]));
+                    pb[t][1] = transpose8(pack2(s[t][2], s[t][3]));
+                }
             }
             rslot = rslot + 1 == kSlots ? 0 : rslot + 1;
             // ---- values: O^T += V^T P^T
@@ -284,20 +326,23 @@ struct WarpPass {
             {
                 const uint32_t slot = ring + rslot * kSlotBytes;
 #pragma unroll
-                for (int t = 0; t < kSteps; ++t) {
+                for (int i = 0; i < kSteps; ++i) {
                     uint32_t a[4];
-                    ldsm4_t(a, slot + vat[t & 3] + (t >> 2) * 128);
-                    mma16816(O[t], a, pb0, pb1);
+                    ldsm4_t(a, slot + vat[i & 3] + (i >> 2) * 128);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) mma16816(O[t][i], a, pb[t][0], pb[t][1]);
                 }
             }
             rslot = rslot + 1 == kSlots ? 0 : rslot + 1;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
-            l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
-        }
+        for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                l[t][0] += __shfl_xor_sync(0xffffffffu, l[t][0], o);
+                l[t][1] += __shfl_xor_sync(0xffffffffu, l[t][1], o);
+            }
     }
 };
 
@@ -312,17 +357,17 @@ struct Segment {     // the part of one span that lies in the range
     int end;             // keys u0 * kUnit .. end - 1
 };
 
-template <int D>
+template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const PagedParams p) {
-    using Pass = WarpPass<D>;
+    using Pass = WarpPass<D, NT>;
+    constexpr int kHeads = NT * kCols;
     extern __shared__ __align__(128) uint8_t ring_smem[];
     float* stage = reinterpret_cast<float*>(ring_smem);  // [warp][head][D + 4], after the rings have been read
     constexpr int kStage = D + 4;                        // keeps the four head columns of a store on different banks
     __shared__ uint32_t masks[kWarps][Pass::kSlots];
     __shared__ float2 marks[kWarps][kHeads];             // maximum and sum of every warp
     __shared__ float2 marks_all[kHeads];
-    constexpr int kQueryRow = D + 8;                     // eight rows that a warp reads by columns without bank conflicts
-    __shared__ __align__(16) __nv_bfloat16 queries[kHeads][kQueryRow];
+    __shared__ __align__(16) __nv_bfloat16 queries[kHeads][Pass::kQueryRow];
     __shared__ int warp_costs[kWarps];
     __shared__ Walk begin_sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -401,21 +446,33 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
     int4 record = make_int4(0, 0, -1, 0);
     Pass pass(p, lane, smem_u32(ring_smem) + warp * kRingBytes, masks[warp]);
 
-    // the queries of a span: 16 bytes a thread, fetched a span ahead (rows past the group's last head repeat it and are not written out)
-    constexpr int kQueryThreads = kHeads * D / 8;
-    const int qrow = tid / (D / 8), qcol = tid % (D / 8) * 8;
-    auto fetch_q = [&](const Segment& s) {
-        const int h = s.kvh * p.group + min(s.hb * kHeads + qrow, p.group - 1);
-        return tid < kQueryThreads ? __ldg(reinterpret_cast<const uint4*>(p.q + s.b * p.ldq + h * p.q_head_stride + qcol)) : make_uint4(0, 0, 0, 0);
+    // the queries of a span: 16 bytes a thread and turn, fetched a span ahead (rows past the group's last head repeat it and are not
+    // written out)
+    constexpr int kQueryThreads = kHeads * D / 8, kTurns = (kQueryThreads + kThreads - 1) / kThreads;
+    struct Queries {
+        uint4 q[kTurns];
     };
-    auto hand_q = [&](const uint4& q) {
-        if (tid < kQueryThreads) *reinterpret_cast<uint4*>(&queries[qrow][qcol]) = q;
+    auto fetch_q = [&](const Segment& s) {
+        Queries r;
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+            const int at = tid + i * kThreads, h = s.kvh * p.group + min(s.hb * kHeads + at / (D / 8), p.group - 1);
+            r.q[i] = at < kQueryThreads ? __ldg(reinterpret_cast<const uint4*>(p.q + s.b * p.ldq + h * p.q_head_stride + at % (D / 8) * 8)) : make_uint4(0, 0, 0, 0);
+        }
+        return r;
+    };
+    auto hand_q = [&](const Queries& r) {
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+            const int at = tid + i * kThreads;
+            if (at < kQueryThreads) *reinterpret_cast<uint4*>(&queries[at / (D / 8)][at % (D / 8) * 8]) = r.q[i];
+        }
     };
 
     Segment now = {}, next = {};
     bool more = advance(now);
     if (more) {
-        const uint4 q = fetch_q(now);
+        const Queries q = fetch_q(now);
         pass.start(now.b, now.kvh, now.u0 * kUnit + warp * kTile, now.end);
         hand_q(q);
     }
@@ -429,15 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
         int next_j = next.u0 * kUnit + warp * kTile + lane;
         const bool fetch = more && lane < kTile && next_j < next.end;
         const int next_page = fetch ? __ldg(p.tables + next.b * p.ldt + (next_j >> p.shift)) : -1;
-        {
-            uint32_t qf[Pass::kSteps][2];
-#pragma unroll
-            for (int s = 0; s < Pass::kSteps; ++s) {
-                qf[s][0] = *reinterpret_cast<const uint32_t*>(&queries[lane >> 2][16 * s + 2 * (lane & 3)]);
-                qf[s][1] = *reinterpret_cast<const uint32_t*>(&queries[lane >> 2][16 * s + 8 + 2 * (lane & 3)]);
-            }
-            pass.run(qf);
-        }
+        pass.run(&queries[0][0]);
         // ---- the next span's first tile is fetched into L2, its queries and this one's gates into registers, while the warps' results
         //      are put together
         if (next_page >= 0 && next_page < p.num_pages) {
@@ -445,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
             prefetch_l2(p.k + o, D * 2);
             prefetch_l2(p.v + o, D * 2);
         }
-        const uint4 next_q = more ? fetch_q(next) : make_uint4(0, 0, 0, 0);
+        const Queries next_q = fetch_q(more ? next : now);
         constexpr int kPairs = kHeads * D / 2 / kThreads;  // pairs of outputs of a thread
         uint32_t gates[kPairs];
 #pragma unroll
@@ -453,21 +502,29 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
             const int h = (tid + i * kThreads) / (D / 2), d = 2 * ((tid + i * kThreads) % (D / 2));
             gates[i] = whole && p.gate && h < nh ? __ldg(reinterpret_cast<const uint32_t*>(p.gate + now.b * p.ldg + (h0 + h) * p.gate_head_stride + d)) : 0u;
         }
-        if (lane < 4) marks[warp][2 * lane] = make_float2(pass.m[0], pass.l[0]), marks[warp][2 * lane + 1] = make_float2(pass.m[1], pass.l[1]);
+        if (lane < 4)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                marks[warp][kCols * t + 2 * lane] = make_float2(pass.m[t][0], pass.l[t][0]), marks[warp][kCols * t + 2 * lane + 1] = make_float2(pass.m[t][1], pass.l[t][1]);
         __syncthreads();  // every ring has been read
         const int parts = min(kWarps, (now.end - now.u0 * kUnit + kTile - 1) / kTile);  // warps that had a tile
         if (warp < parts) {
-            float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top[0] = fmaxf(top[0], marks[w][2 * (lane & 3)].x), top[1] = fmaxf(top[1], marks[w][2 * (lane & 3) + 1].x);
-            const float f0 = pass.m[0] == -INFINITY ? 0.f : exp2_fast(pass.m[0] - top[0]), f1 = pass.m[1] == -INFINITY ? 0.f : exp2_fast(pass.m[1] - top[1]);
-            float* st = stage + warp * kHeads * kStage + 2 * (lane & 3) * kStage + (lane >> 2);
+            for (int t = 0; t < NT; ++t) {
+                const int col = kCols * t + 2 * (lane & 3);
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int s = 0; s < Pass::kSteps; ++s) {
-                st[16 * s] = pass.O[s][0] * f0;
-                st[kStage + 16 * s] = pass.O[s][1] * f1;
-                st[16 * s + 8] = pass.O[s][2] * f0;
-                st[kStage + 16 * s + 8] = pass.O[s][3] * f1;
+                for (int w = 0; w < kWarps; ++w) top[0] = fmaxf(top[0], marks[w][col].x), top[1] = fmaxf(top[1], marks[w][col + 1].x);
+                const float f0 = pass.m[t][0] == -INFINITY ? 0.f : exp2_fast(pass.m[t][0] - top[0]);
+                const float f1 = pass.m[t][1] == -INFINITY ? 0.f : exp2_fast(pass.m[t][1] - top[1]);
+                float* st = stage + (warp * kHeads + col) * kStage + (lane >> 2);
+#pragma unroll
+                for (int s = 0; s < Pass::kSteps; ++s) {
+                    st[16 * s] = pass.O[t][s][0] * f0;
+                    st[kStage + 16 * s] = pass.O[t][s][1] * f1;
+                    st[16 * s + 8] = pass.O[t][s][2] * f0;
+                    st[kStage + 16 * s + 8] = pass.O[t][s][3] * f1;
+                }
             }
             if (tid < kHeads) {
                 float high = -INFINITY, sum = 0.f;
@@ -518,9 +575,9 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
 // heads (blockIdx.y). There may be over a hundred pieces when one context is alone: a thread looks at one mark each, and the warps
 // share the pieces, so that the block waits for the record, the marks and the pieces once each.
 constexpr int kJoinThreads = 512;
-template <int D>
+template <int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) s1_attention_paged_join_kernel(const PagedParams p) {
-    constexpr int kVec = D / 32, kJoinWarps = kJoinThreads / 32;
+    constexpr int kHeads = NT * kCols, kVec = D / 32, kJoinWarps = kJoinThreads / 32;
     __shared__ float sums[kJoinWarps][D];
     __shared__ float weights[kJoinThreads];
     __shared__ float tops[kJoinWarps], totals[kJoinWarps];
@@ -576,19 +633,19 @@ constexpr int kMaxCtas = 256;  // the workspace's share: more than one CTA per S
 static_assert(kMaxCtas <= kJoinThreads, "the join looks at one piece a thread");
 
 size_t workspace_bytes_of(int head_dim) {
-    return sizeof(int4) * kMaxCtas + 2 * kMaxCtas * kHeads * (sizeof(float2) + sizeof(float) * static_cast<size_t>(head_dim));
+    return sizeof(int4) * kMaxCtas + 2 * kMaxCtas * 2 * kCols * (sizeof(float2) + sizeof(float) * static_cast<size_t>(head_dim));
 }
 
-template <int D>
+template <int D, int NT>
 int launch(s1_ctx* ctx, const PagedParams& p, int ctas) {
     constexpr int smem = kWarps * kRingBytes;
     static std::atomic<unsigned long long> told{0};  // one bit per device
     if (!(told.load(std::memory_order_relaxed) >> (ctx->device & 63) & 1)) {
-        S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         told.fetch_or(1ull << (ctx->device & 63), std::memory_order_relaxed);
     }
-    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D>, static_cast<unsigned>(ctas), 1u, kThreads, smem, p));
-    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_join_kernel<D>, static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(kHeads, p.group)),
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D, NT>, static_cast<unsigned>(ctas), 1u, kThreads, smem, p));
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_join_kernel<D, NT>, static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(NT * kCols, p.group)),
                                       kJoinThreads, 0, p));
     ctx->launches += 2;
     return S1_OK;
@@ -631,18 +688,17 @@ extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, lon
     if (num_seqs == 0) return S1_OK;
     S1DeviceGuard guard(ctx->device);
     if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
-    const int group = heads / kv_heads, blocks = (group + kHeads - 1) / kHeads;
+    const int group = heads / kv_heads, columns = group > kCols ? 2 * kCols : kCols, blocks = (group + columns - 1) / columns;
     if (static_cast<long long>(num_seqs) * kv_heads * blocks > (1ll << 31) / ((static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit + 4) - 1)
         return s1_fail(ctx, S1_EINVAL, "%s: rows x KV heads x (tokens of a block table) / 128 must be below 2^31", who);    float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas);
     PagedParams p{static_cast<const __nv_bfloat16*>(q), ldq, q_head_stride, static_cast<const __nv_bfloat16*>(k_cache),
                   static_cast<const __nv_bfloat16*>(v_cache), page_stride, token_stride, head_stride, num_pages, __builtin_ctz(page_size), tables, ldt,
                   table_width, lengths, num_seqs, heads, kv_heads, group, kv_heads * blocks, blocks, scale * 1.4426950408889634f,
                   static_cast<const __nv_bfloat16*>(gate), ldg, gate_head_stride, static_cast<__nv_bfloat16*>(out), ldo,
-                  reinterpret_cast<float*>(marks + 2 * kMaxCtas * kHeads), marks, static_cast<int4*>(workspace), ctx->status_dev};
+                  reinterpret_cast<float*>(marks + 2 * kMaxCtas * 2 * kCols), marks, static_cast<int4*>(workspace), ctx->status_dev};
     // one CTA per SM, and no more than the block tables could make units of
     const long long most = static_cast<long long>(num_seqs) * kv_heads * blocks * ((static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit + 4);
     const int ctas = static_cast<int>(std::min<long long>(std::min(ctx->sm_count, kMaxCtas), most));
-    if (head_dim == 64) return launch<64>(ctx, p, ctas);
-    if (head_dim == 128) return launch<128>(ctx, p, ctas);
-    return launch<256>(ctx, p, ctas);
+    if (columns == kCols) return head_dim == 64 ? launch<64, 1>(ctx, p, ctas) : head_dim == 128 ? launch<128, 1>(ctx, p, ctas) : launch<256, 1>(ctx, p, ctas);
+    return head_dim == 64 ? launch<64, 2>(ctx, p, ctas) : head_dim == 128 ? launch<128, 2>(ctx, p, ctas) : launch<256, 2>(ctx, p, ctas);
 }

@@ -243,7 +243,7 @@ def _check_attention(got, q, kc, vc, tables, lens, gate, scale=None):
     ([1], 1, 1, 64, 16, "token"), ([17], 8, 2, 256, 16, "token"), ([0, -1, 5, 16, 15], 4, 4, 128, 16, "head"),
     ([128, 129, 127, 1, 300], 6, 2, 256, 64, "token"), ([1000, 3, 0, 64, 65, 2049], 24, 4, 256, 16, "head"),
     ([255, 256, 257], 16, 1, 64, 1, "token"), ([77, 200], 9, 1, 256, 2, "token"), ([513, 40], 16, 2, 128, 8, "head"), ([3000], 34, 2, 64, 128, "token"),
-    ([20000, 5], 3, 1, 256, 65536, "token"), ([30000], 8, 2, 256, 64, "head")])
+    ([3000, 200], 32, 2, 256, 16, "token"), ([5000, 0, 130], 12, 1, 128, 64, "head"), ([20000, 5], 3, 1, 256, 65536, "token"), ([30000], 8, 2, 256, 64, "head")])
 @pytest.mark.parametrize("gated", [False, True])
 def test_paged_attention(ctx, lens, H, kv, dim, page, layout, gated):
     q, kc, vc, tables, lengths, gate = _attention_case(lens, H, kv, dim, page, sum(map(abs, lens)) + H, layout, gated)
