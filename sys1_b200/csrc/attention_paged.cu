@@ -573,13 +573,14 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
 
 // Joins the pieces of the span that began in CTA blockIdx.x of the first kernel and went on in the CTAs after it, for one of its
 // heads (blockIdx.y). There may be over a hundred pieces when one context is alone: a thread looks at one mark each, and the warps
-// share the pieces, so that the block waits for the record, the marks and the pieces once each.
-constexpr int kJoinThreads = 512;
-template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) s1_attention_paged_join_kernel(const PagedParams p) {
-    constexpr int kHeads = NT * kCols, kVec = D / 32, kJoinWarps = kJoinThreads / 32;
+// share the pieces, so that the block waits for the record, the marks and the pieces once each. THREADS: 512 where there are fewer spans
+// than CTAs and so many pieces to a span (one context of 131071 tokens 49 us, with 256 threads 53), else 256 (64 contexts up to 8192
+// tokens 168 us, with 512 threads 170).
+template <int D, int NT, int THREADS>
+__global__ void __launch_bounds__(THREADS) s1_attention_paged_join_kernel(const PagedParams p) {
+    constexpr int kHeads = NT * kCols, kVec = D / 32, kJoinWarps = THREADS / 32;
     __shared__ float sums[kJoinWarps][D];
-    __shared__ float weights[kJoinThreads];
+    __shared__ float weights[THREADS];
     __shared__ float tops[kJoinWarps], totals[kJoinWarps];
     griddep_wait();
     griddep_launch_dependents();
@@ -630,7 +631,7 @@ __global__ void __launch_bounds__(kJoinThreads) s1_attention_paged_join_kernel(c
 }
 
 constexpr int kMaxCtas = 256;  // the workspace's share: more than one CTA per SM of any sm_100 part
-static_assert(kMaxCtas <= kJoinThreads, "the join looks at one piece a thread");
+static_assert(kMaxCtas <= 256, "the join looks at one piece a thread");
 
 size_t workspace_bytes_of(int head_dim) {
     return sizeof(int4) * kMaxCtas + 2 * kMaxCtas * 2 * kCols * (sizeof(float2) + sizeof(float) * static_cast<size_t>(head_dim));
@@ -645,8 +646,9 @@ int launch(s1_ctx* ctx, const PagedParams& p, int ctas) {
         told.fetch_or(1ull << (ctx->device & 63), std::memory_order_relaxed);
     }
     S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D, NT>, static_cast<unsigned>(ctas), 1u, kThreads, smem, p));
-    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_join_kernel<D, NT>, static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(NT * kCols, p.group)),
-                                      kJoinThreads, 0, p));
+    const bool many = static_cast<long long>(p.num_seqs) * p.spans_per_row >= ctas;
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, many ? s1_attention_paged_join_kernel<D, NT, 256> : s1_attention_paged_join_kernel<D, NT, 512>,
+                                      static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(NT * kCols, p.group)), many ? 256u : 512u, 0, p));
     ctx->launches += 2;
     return S1_OK;
 }
