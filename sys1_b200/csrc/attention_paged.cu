@@ -19,6 +19,8 @@
 //  * the products run on mma.sync m16n8k16 with the operands turned round - S^T = K Q^T, O^T = V^T P^T - so that the 16 rows are
 //    keys and head dimensions, which there are enough of, and the 8 columns the query heads of the group. tcgen05 would want 64 or
 //    128 rows of queries where there are 1 to 16; at the rate that HBM delivers keys, mma.sync is a fifth busy.
+// Measured: 62 contexts of 100 .. 8192 tokens, 24 query and 4 KV heads of 256: 168 us = 6.3 TB/s; one of 131071 tokens, 8 and 2 heads:
+// 49 us = 5.4 TB/s; 31 of 1 .. 2048 tokens: 20 us; one of 17: 7 us.
 // Scores, maxima, sums and outputs are f32; the probabilities are rounded to bf16 for the second product, as in s1_attention
 // (an error of 2^-9 of each weight, averaged over the keys), while their sum is that of the unrounded ones.
 #include <cuda_bf16.h>
@@ -105,9 +107,11 @@ __device__ __forceinline__ void report(int* status, int code, int where, int val
         status[3] = value;
     }
 }
+// (Everything a call is given is read with plain loads: the kernel may be resident while the one before still writes it, which the
+// read-only path does not allow for.)
 // Keys that a row attends to; a length beyond its block table is reported and the row treated as empty.
 __device__ __forceinline__ int row_length(const PagedParams& p, int b, bool tell) {
-    const int len = max(__ldg(p.lengths + b), 0);
+    const int len = max(p.lengths[b], 0);
     if (len > (static_cast<long long>(p.table_width) << p.shift)) {
         if (tell) report(p.status, 117, b, len);
         return 0;
@@ -154,7 +158,7 @@ struct WarpPass {
     __device__ __forceinline__ void request(bool values, int slot, int b, int kvh, int j0, int end) {
         if (!values) {
             if (one_page) {
-                const int page = __ldg(p.tables + b * p.ldt + (j0 >> p.shift));
+                const int page = p.tables[b * p.ldt + (j0 >> p.shift)];
                 const bool ok = page >= 0 && page < p.num_pages;
                 if (!ok && lane == 0) report(p.status, 118, b, page);
                 off = page * p.page_stride + (j0 & ((1 << p.shift) - 1)) * p.token_stride + kvh * p.head_stride;
@@ -162,7 +166,7 @@ struct WarpPass {
             } else {
                 const int j = j0 + lane;
                 const bool want = lane < kTile && j < end;
-                const int page = want ? __ldg(p.tables + b * p.ldt + (j >> p.shift)) : 0;
+                const int page = want ? p.tables[b * p.ldt + (j >> p.shift)] : 0;
                 const bool ok = want && page >= 0 && page < p.num_pages;
                 if (want && !ok) report(p.status, 118, b, page);
                 off = ok ? page * p.page_stride + (j & ((1 << p.shift) - 1)) * p.token_stride + kvh * p.head_stride : 0;
@@ -457,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
 #pragma unroll
         for (int i = 0; i < kTurns; ++i) {
             const int at = tid + i * kThreads, h = s.kvh * p.group + min(s.hb * kHeads + at / (D / 8), p.group - 1);
-            r.q[i] = at < kQueryThreads ? __ldg(reinterpret_cast<const uint4*>(p.q + s.b * p.ldq + h * p.q_head_stride + at % (D / 8) * 8)) : make_uint4(0, 0, 0, 0);
+            r.q[i] = at < kQueryThreads ? *reinterpret_cast<const uint4*>(p.q + s.b * p.ldq + h * p.q_head_stride + at % (D / 8) * 8) : make_uint4(0, 0, 0, 0);
         }
         return r;
     };
@@ -485,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
         // where the next span's keys begin for this warp: looked up now, wanted when this span is done
         int next_j = next.u0 * kUnit + warp * kTile + lane;
         const bool fetch = more && lane < kTile && next_j < next.end;
-        const int next_page = fetch ? __ldg(p.tables + next.b * p.ldt + (next_j >> p.shift)) : -1;
+        const int next_page = fetch ? p.tables[next.b * p.ldt + (next_j >> p.shift)] : -1;
         pass.run(&queries[0][0]);
         // ---- the next span's first tile is fetched into L2, its queries and this one's gates into registers, while the warps' results
         //      are put together
@@ -500,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
             const int h = (tid + i * kThreads) / (D / 2), d = 2 * ((tid + i * kThreads) % (D / 2));
-            gates[i] = whole && p.gate && h < nh ? __ldg(reinterpret_cast<const uint32_t*>(p.gate + now.b * p.ldg + (h0 + h) * p.gate_head_stride + d)) : 0u;
+            gates[i] = whole && p.gate && h < nh ? *reinterpret_cast<const uint32_t*>(p.gate + now.b * p.ldg + (h0 + h) * p.gate_head_stride + d) : 0u;
         }
         if (lane < 4)
 #pragma unroll

@@ -24,7 +24,8 @@ struct S1DeviceGuard {
 
 // Launches a kernel that waits (griddepcontrol.wait) before it touches memory, with programmatic stream serialization unless the
 // context's "pdl" option is off: a step of a decoder is a chain of kernels of a few microseconds, and their set-up then lies under
-// the kernel before.
+// the kernel before. Such a kernel reads what others may have written with plain loads: its blocks can be there while the kernel
+// before still reads and writes on the same SM, and the read-only path promises nothing about data that changes in a kernel's life.
 template <typename Params>
 inline cudaError_t s1_launch_waiting(s1_ctx* ctx, void (*kernel)(Params), unsigned grid_x, unsigned grid_y, unsigned threads, size_t smem,
                                      const Params& params, unsigned cluster = 1) {

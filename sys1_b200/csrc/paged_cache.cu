@@ -85,7 +85,8 @@ struct TableParams {
 // Latency is all there is here: a few kilobytes in and out, and the prefix sums over the rows in between. Every block of the
 // (one) cluster forms the sums for itself, which costs less than handing them round, and then takes its share of the tokens.
 // The cluster's barrier between the last read of an input and the first write lets `lengths` be `cached` and
-// `free_count_out` be `free_count`: a step captured into a graph then advances the same buffers at every replay.
+// `free_count_out` be `free_count`: a step captured into a graph then advances the same buffers at every replay. Measured: 8 rows of one token 2.9 us, 1024 rows 3.6, 31
+// prompts of 16399 tokens 6.2.
 __global__ void __launch_bounds__(kTableThreads) s1_block_tables_kernel(const TableParams p) {
     extern __shared__ int32_t rows_smem[];
     int32_t* cu = rows_smem;                      // [num_seqs + 1] first token of every row
@@ -279,10 +280,10 @@ __global__ void __launch_bounds__(256) s1_cache_write_kernel(const WriteParams p
         if (value[u]) row -= rows;
         live[u] = row < rows;
         t[u] = live[u] ? static_cast<int>(row / static_cast<unsigned>(p.kv_heads)) : 0, h[u] = live[u] ? static_cast<int>(row) - t[u] * p.kv_heads : 0;
-        slot[u] = live[u] ? __ldg(p.slots + t[u]) : -1;
-        pos[u] = NORM && live[u] && !value[u] ? __ldg(p.positions + t[u]) : 0;
+        slot[u] = live[u] ? p.slots[t[u]] : -1;
+        pos[u] = NORM && live[u] && !value[u] ? p.positions[t[u]] : 0;
         const __nv_bfloat16* src = value[u] ? p.v + t[u] * p.ldv + h[u] * p.v_head_stride : p.k + t[u] * p.ldk + h[u] * p.k_head_stride;
-        raw[u] = live[u] ? __ldg(reinterpret_cast<const uint4*>(src + sub * 8)) : make_uint4(0, 0, 0, 0);
+        raw[u] = live[u] ? *reinterpret_cast<const uint4*>(src + sub * 8) : make_uint4(0, 0, 0, 0);  // (plain: see s1_launch_waiting)
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {

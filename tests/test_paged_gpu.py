@@ -367,6 +367,21 @@ def test_paged_attention_captured_follows_its_lengths(ctx):
         other.sync()
 
 
+def test_without_programmatic_serialization(ctx):
+    """The context's "pdl" option off: plain launches, the same results."""
+    q, kc, vc, tables, lengths, gate = _attention_case([700, 30, 0, 2000], 8, 2, 256, 16, 41)
+    c = _step_case(5, 2, 4, 42)
+    d = dict(c, state=c["state"].clone(), conv_state=c["conv_state"].clone())
+    want = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate), qwen35.gated_delta_rule_step(**c)
+    ctx.set_option("pdl", 0)
+    try:
+        got = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate), qwen35.gated_delta_rule_step(**d)
+    finally:
+        ctx.set_option("pdl", 1)
+    ctx.sync()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(c["state"], d["state"])
+
+
 def test_two_streams_at_once(ctx):
     """Calls that run at the same time on two streams (each with its own context and workspace) give what they give alone."""
     cases = [_attention_case([3000, 1, 900], 8, 2, 128, 16, 31), _attention_case([10, 2500, 70], 8, 2, 128, 16, 32)]
