@@ -696,7 +696,8 @@ extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, lon
     if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
     const int group = heads / kv_heads, columns = group > kCols ? 2 * kCols : kCols, blocks = (group + columns - 1) / columns;
     if (static_cast<long long>(num_seqs) * kv_heads * blocks > (1ll << 31) / ((static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit + 4) - 1)
-        return s1_fail(ctx, S1_EINVAL, "%s: rows x KV heads x (tokens of a block table) / 128 must be below 2^31", who);    float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas);
+        return s1_fail(ctx, S1_EINVAL, "%s: rows x KV heads x (tokens of a block table) / 128 must be below 2^31", who);
+    float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas);
     PagedParams p{static_cast<const __nv_bfloat16*>(q), ldq, q_head_stride, static_cast<const __nv_bfloat16*>(k_cache),
                   static_cast<const __nv_bfloat16*>(v_cache), page_stride, token_stride, head_stride, num_pages, __builtin_ctz(page_size), tables, ldt,
                   table_width, lengths, num_seqs, heads, kv_heads, group, kv_heads * blocks, blocks, scale * 1.4426950408889634f,
