@@ -124,9 +124,7 @@ __device__ __forceinline__ float rcp_fast(float x) {  // relative error 2^-23, b
     return r;
 }
 __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.f + exp2_fast(-1.4426950408889634f * x)); }
-__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory"); }
 
 // One warp's pass over its tiles of a span: keys first + 16 (warp + 8 i), below `end`. NT = 1: up to 8 query heads, held in registers;
 // NT = 2: up to 16, read from shared memory step by step, so that a group of more than 8 does not read its keys twice (32 x 8192
@@ -487,16 +485,25 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
         const int stop = walk.at;  // where this segment ends
         more = advance(next);
         // where the next span's keys begin for this warp: looked up now, wanted when this span is done
-        int next_j = next.u0 * kUnit + warp * kTile + lane;
-        const bool fetch = more && lane < kTile && next_j < next.end;
-        const int next_page = fetch ? p.tables[next.b * p.ldt + (next_j >> p.shift)] : -1;
+        const int next_j = next.u0 * kUnit + warp * kTile + lane;
+        const int next_page = more && lane < kTile && next_j < next.end ? p.tables[next.b * p.ldt + (next_j >> p.shift)] : -1;
         pass.run(&queries[0][0]);
         // ---- the next span's first tile is fetched into L2, its queries and this one's gates into registers, while the warps' results
         //      are put together
-        if (next_page >= 0 && next_page < p.num_pages) {
-            const long long o = next_page * p.page_stride + (next_j & ((1 << p.shift) - 1)) * p.token_stride + next.kvh * p.head_stride;
-            prefetch_l2(p.k + o, D * 2);
-            prefetch_l2(p.v + o, D * 2);
+        {
+            const bool there = next_page >= 0 && next_page < p.num_pages;
+            const long long o = there ? next_page * p.page_stride + (next_j & ((1 << p.shift) - 1)) * p.token_stride + next.kvh * p.head_stride : -1;
+            constexpr int kLines = D / 64;  // 128-byte lines of a key (one prefetch a lane: the bulk form is issued lane by lane, 2000 cycles here)
+#pragma unroll
+            for (int i = 0; i < kTile * kLines / 32; ++i) {
+                const int at = lane + 32 * i;
+                const long long row = __shfl_sync(0xffffffffu, o, at / kLines);
+                if (row >= 0) prefetch_l2(p.k + row + at % kLines * 64), prefetch_l2(p.v + row + at % kLines * 64);
+            }
+            if (kTile * kLines < 32) {  // head dim 64: one line a key
+                const long long row = __shfl_sync(0xffffffffu, o, lane % kTile);
+                if (row >= 0) prefetch_l2((lane < kTile ? p.k : p.v) + row);
+            }
         }
         const Queries next_q = fetch_q(more ? next : now);
         constexpr int kPairs = kHeads * D / 2 / kThreads;  // pairs of outputs of a thread
