@@ -38,10 +38,7 @@ using namespace s1;
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;               // keys of one warp step
-constexpr int kUnit = kWarps * kTile;   // keys of one unit of work
 constexpr int kCols = 8;                // query heads of one MMA (its columns); a span has NT times as many
 constexpr int kRingBytes = 24 * 1024;   // per warp
 
@@ -126,11 +123,12 @@ __device__ __forceinline__ float rcp_fast(float x) {  // relative error 2^-23, b
 __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.f + exp2_fast(-1.4426950408889634f * x)); }
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory"); }
 
-// One warp's pass over its tiles of a span: keys first + 16 (warp + 8 i), below `end`. NT = 1: up to 8 query heads, held in registers;
+// One warp's pass over its tiles of a span: keys first, first + 16 W, ..., 16 to a tile, below `end`. NT = 1: up to 8 query heads, held in registers;
 // NT = 2: up to 16, read from shared memory step by step, so that a group of more than 8 does not read its keys twice (32 x 8192
 // tokens, 16 heads to a KV head of 256: 166 us as two spans of 8, 98 as one of 16).
-template <int D, int NT>
+template <int D, int NT, int W>
 struct WarpPass {
+    static constexpr int kUnit = W * kTile;                 // keys of one unit: a tile for each of the CTA's W warps
     static constexpr int kSlotBytes = kTile * D * 2;
     static constexpr int kSlots = kRingBytes / kSlotBytes;  // 3, 6 or 12
     static constexpr int kChunks = D / 8;                   // 16-byte pieces of a key
@@ -359,10 +357,13 @@ struct Segment {     // the part of one span that lies in the range
     int end;             // keys u0 * kUnit .. end - 1
 };
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const PagedParams p) {
-    using Pass = WarpPass<D, NT>;
-    constexpr int kHeads = NT * kCols;
+// W = 8: one CTA per SM. W = 4: two, with half the warps and rings each - where there are many spans, one's keys come while the
+// other puts its results together (512 contexts of 100 tokens 40 us with W = 8, 35 with 4; of 17 tokens 35 and 24); with few and
+// long ones the larger units stream a little faster (64 contexts up to 8192 tokens 168 and 172 us).
+template <int D, int NT, int W>
+__global__ void __launch_bounds__(W * 32, 8 / W) s1_attention_paged_kernel(const PagedParams p) {
+    using Pass = WarpPass<D, NT, W>;
+    constexpr int kHeads = NT * kCols, kWarps = W, kThreads = W * 32, kUnit = Pass::kUnit;
     extern __shared__ __align__(128) uint8_t ring_smem[];
     float* stage = reinterpret_cast<float*>(ring_smem);  // [warp][head][D + 4], after the rings have been read
     constexpr int kStage = D + 4;                        // keeps the four head columns of a store on different banks
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) s1_attention_paged_kernel(const P
 // Joins the pieces of the span that began in CTA blockIdx.x of the first kernel and went on in the CTAs after it, for one of its
 // heads (blockIdx.y). There may be over a hundred pieces when one context is alone: a thread looks at one mark each, and the warps
 // share the pieces, so that the block waits for the record, the marks and the pieces once each. THREADS: 512 where there are fewer spans
-// than CTAs and so many pieces to a span (one context of 131071 tokens 49 us, with 256 threads 53), else 256 (64 contexts up to 8192
+// than CTAs and so many pieces to a span (one context of 131071 tokens 49 us, with 256 threads 53), else 320 (64 contexts up to 8192
 // tokens 168 us, with 512 threads 170).
 template <int D, int NT, int THREADS>
 __global__ void __launch_bounds__(THREADS) s1_attention_paged_join_kernel(const PagedParams p) {
@@ -641,27 +642,35 @@ __global__ void __launch_bounds__(THREADS) s1_attention_paged_join_kernel(const 
     }
 }
 
-constexpr int kMaxCtas = 256;  // the workspace's share: more than one CTA per SM of any sm_100 part
-static_assert(kMaxCtas <= 256, "the join looks at one piece a thread");
+constexpr int kMaxCtas = 320;  // the workspace's share: two CTAs per SM of any sm_100 part
+static_assert(kMaxCtas <= 320, "the join looks at one piece a thread");
 
 size_t workspace_bytes_of(int head_dim) {
     return sizeof(int4) * kMaxCtas + 2 * kMaxCtas * 2 * kCols * (sizeof(float2) + sizeof(float) * static_cast<size_t>(head_dim));
 }
 
-template <int D, int NT>
-int launch(s1_ctx* ctx, const PagedParams& p, int ctas) {
-    constexpr int smem = kWarps * kRingBytes;
+template <int D, int NT, int W>
+int launch(s1_ctx* ctx, PagedParams p, int units) {
+    constexpr int smem = W * kRingBytes;
     static std::atomic<unsigned long long> told{0};  // one bit per device
     if (!(told.load(std::memory_order_relaxed) >> (ctx->device & 63) & 1)) {
-        S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         told.fetch_or(1ull << (ctx->device & 63), std::memory_order_relaxed);
     }
-    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D, NT>, static_cast<unsigned>(ctas), 1u, kThreads, smem, p));
+    const int ctas = std::min({8 / W * ctx->sm_count, kMaxCtas, units});  // no more than the block tables could make units of
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D, NT, W>, static_cast<unsigned>(ctas), 1u, W * 32u, smem, p));
     const bool many = static_cast<long long>(p.num_seqs) * p.spans_per_row >= ctas;
-    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, many ? s1_attention_paged_join_kernel<D, NT, 256> : s1_attention_paged_join_kernel<D, NT, 512>,
-                                      static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(NT * kCols, p.group)), many ? 256u : 512u, 0, p));
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, many ? s1_attention_paged_join_kernel<D, NT, 320> : s1_attention_paged_join_kernel<D, NT, 512>,
+                                      static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(NT * kCols, p.group)), many ? 320u : 512u, 0, p));
     ctx->launches += 2;
     return S1_OK;
+}
+
+template <int D>
+int launch(s1_ctx* ctx, const PagedParams& p, int units) {
+    const bool wide = p.group > kCols, many = static_cast<long long>(p.num_seqs) * p.spans_per_row >= 3ll * ctx->sm_count;
+    if (wide) return many ? launch<D, 2, 4>(ctx, p, units) : launch<D, 2, 8>(ctx, p, units);
+    return many ? launch<D, 1, 4>(ctx, p, units) : launch<D, 1, 8>(ctx, p, units);
 }
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -702,17 +711,15 @@ extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, lon
     S1DeviceGuard guard(ctx->device);
     if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
     const int group = heads / kv_heads, columns = group > kCols ? 2 * kCols : kCols, blocks = (group + columns - 1) / columns;
-    if (static_cast<long long>(num_seqs) * kv_heads * blocks > (1ll << 31) / ((static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit + 4) - 1)
-        return s1_fail(ctx, S1_EINVAL, "%s: rows x KV heads x (tokens of a block table) / 128 must be below 2^31", who);
+    // the costs of all spans, with the smaller units, have to fit 31 bits
+    const long long spans = static_cast<long long>(num_seqs) * kv_heads * blocks, cost = static_cast<long long>(table_width) * page_size / (4 * kTile) + 5;
+    if (spans > (1ll << 31) / cost - 1) return s1_fail(ctx, S1_EINVAL, "%s: rows x KV heads x (tokens of a block table) / 64 must be below 2^31", who);
     float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas);
     PagedParams p{static_cast<const __nv_bfloat16*>(q), ldq, q_head_stride, static_cast<const __nv_bfloat16*>(k_cache),
                   static_cast<const __nv_bfloat16*>(v_cache), page_stride, token_stride, head_stride, num_pages, __builtin_ctz(page_size), tables, ldt,
                   table_width, lengths, num_seqs, heads, kv_heads, group, kv_heads * blocks, blocks, scale * 1.4426950408889634f,
                   static_cast<const __nv_bfloat16*>(gate), ldg, gate_head_stride, static_cast<__nv_bfloat16*>(out), ldo,
                   reinterpret_cast<float*>(marks + 2 * kMaxCtas * 2 * kCols), marks, static_cast<int4*>(workspace), ctx->status_dev};
-    // one CTA per SM, and no more than the block tables could make units of
-    const long long most = static_cast<long long>(num_seqs) * kv_heads * blocks * ((static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit + 4);
-    const int ctas = static_cast<int>(std::min<long long>(std::min(ctx->sm_count, kMaxCtas), most));
-    if (columns == kCols) return head_dim == 64 ? launch<64, 1>(ctx, p, ctas) : head_dim == 128 ? launch<128, 1>(ctx, p, ctas) : launch<256, 1>(ctx, p, ctas);
-    return head_dim == 64 ? launch<64, 2>(ctx, p, ctas) : head_dim == 128 ? launch<128, 2>(ctx, p, ctas) : launch<256, 2>(ctx, p, ctas);
+    const int units = static_cast<int>(std::min(spans * cost, 1ll << 30));
+    return head_dim == 64 ? launch<64>(ctx, p, units) : head_dim == 128 ? launch<128>(ctx, p, units) : launch<256>(ctx, p, units);
 }

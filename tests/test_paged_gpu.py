@@ -259,11 +259,13 @@ def test_paged_attention(ctx, lens, H, kv, dim, page, layout, gated):
     assert bool((out[:, H * dim:] == 7).all())
 
 
-def test_paged_attention_many_ragged_rows(ctx):
+@pytest.mark.parametrize("rows,H,kv,dim,longest", [(700, 4, 2, 64, 900), (250, 8, 2, 256, 900), (300, 24, 2, 128, 500), (230, 32, 2, 256, 300),
+                                                   (90, 12, 6, 128, 5000), (120, 6, 1, 256, 3000)])
+def test_paged_attention_many_ragged_rows(ctx, rows, H, kv, dim, longest):
     """More rows than threads in a block, and more units than CTAs: ranges that begin and end anywhere."""
     h = np.random.RandomState(5)
-    lens = [int(n) for n in np.where(h.rand(700) < 0.1, 0, np.exp(h.uniform(0, np.log(900), 700)))]
-    q, kc, vc, tables, lengths, gate = _attention_case(lens, 4, 2, 64, 16, 5)
+    lens = [int(n) for n in np.where(h.rand(rows) < 0.1, 0, np.exp(h.uniform(0, np.log(longest), rows)))]
+    q, kc, vc, tables, lengths, gate = _attention_case(lens, H, kv, dim, 16, 5)
     got = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate)
     ctx.sync()
     _check_attention(got, q, kc, vc, tables, lens, gate)
