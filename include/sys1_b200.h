@@ -364,7 +364,7 @@ int s1_head_norm_rope(s1_ctx* ctx, void* x, long long ldx, long long head_stride
  *   cu_seqlens [num_seqs + 1] first token of every row in the packed batch (may be NULL)
  *   positions, slots [max_tokens]  of every token of the packed batch, row after row. `added` NULL: token b belongs to row b and
  *                             max_tokens = num_seqs. Tokens of idle rows and those behind the last get position 0 and slot -1.
- * A row whose tokens do not fit (its block table's width, the free pages, max_tokens) is reported and gets nothing: no page, its
+ * A row whose tokens do not fit (its block table's width, 2^31 - 1 tokens, the free pages, max_tokens) is reported and gets nothing: no page, its
  * length unchanged, position 0 and slot -1 for its tokens (with too few pages that holds for every later row that needs one too).
  * num_seqs <= 8192, max_tokens and free_capacity (entries of free_pages) < 2^30. The outputs must not overlap other arguments
  * except as said.

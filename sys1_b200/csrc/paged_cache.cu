@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(kTableThreads) s1_block_tables_kernel(const Ta
         const long long now = static_cast<long long>(max(was, 0)) + add;
         const long long mask = (1ll << p.shift) - 1;
         const long long had = (max(was, 0) + mask) >> p.shift, want = (now + mask) >> p.shift;
-        const bool fits = want <= p.table_width && end <= static_cast<unsigned>(p.max_tokens);
+        const bool holds = want <= p.table_width && now <= 2147483647ll;  // lengths and positions are 32 bits, whatever the table could hold
+        const bool fits = holds && end <= static_cast<unsigned>(p.max_tokens);
         const unsigned need = (row && fits) ? static_cast<unsigned>(want - had) : 0u;
         const unsigned upto = add_sat(pages, block_scan(need, warp_sums));
         pages = add_sat(pages, warp_sums[32]);
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kTableThreads) s1_block_tables_kernel(const Ta
             off[b] = served ? static_cast<int>(upto - need) : -1;
             old[b] = was;
             if (served && need) atomicMax(&taken_sh, upto);
-            if (!served && rank == 0) report(p.status, !fits ? (want > p.table_width ? 110 : 112) : 111, b, static_cast<int>(min(now, 2147483647ll)));
+            if (!served && rank == 0) report(p.status, !holds ? 110 : !fits ? 112 : 111, b, static_cast<int>(min(now, 2147483647ll)));
         }
     }
     __syncthreads();

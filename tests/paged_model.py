@@ -19,7 +19,7 @@ def block_tables_model(cached, added, page, free, count, tables, max_tokens):
         cu.append(cu[-1] + (1 if added is None else add))
         old = max(int(cached[b]), 0)
         need = pages(old + add, page) - pages(old, page)
-        if pages(old + add, page) > width or cu[-1] > max_tokens:
+        if pages(old + add, page) > width or old + add >= 2 ** 31 or cu[-1] > max_tokens:
             refused.append(b)
             lengths.append(int(cached[b]))
             continue

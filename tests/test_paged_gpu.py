@@ -111,6 +111,19 @@ def test_block_tables_that_do_not_fit(ctx, what):
         _check_tables(r, dt, want)
 
 
+def test_block_tables_up_to_the_last_length(ctx):
+    """Lengths end at 2^31 - 1, also where a row's block table could hold more."""
+    page, width = 65536, 32770
+    tables = np.tile(np.arange(width, dtype=np.int32) % 32768, (3, 1))
+    cached, add, free = [2 ** 31 - 1, 2 ** 31 - 3, 5], [3, 2, 1], [4, 9]
+    want = block_tables_model(cached, add, page, free, 2, tables, 6)
+    assert want["refused"] == [0] and want["lengths"][:2] == [2 ** 31 - 1] * 2
+    dt = ints(tables)
+    r = paged.block_tables(ints(cached), dt, ints(free), ints([2]), page, added=ints(add), max_tokens=6)
+    _refused(ctx, "more pages than")
+    _check_tables(r, dt, want)
+
+
 @pytest.mark.parametrize("rows,page,width", [(1, 1, 3), (9, 16, 5), (1500, 16, 4), (8192, 64, 2)])
 def test_release(ctx, rows, page, width):
     h = np.random.RandomState(rows)
