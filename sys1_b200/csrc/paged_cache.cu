@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(256) s1_cache_write_kernel(const WriteParams p
     griddep_wait();
     griddep_launch_dependents();
     const unsigned rows = static_cast<unsigned>(p.T) * static_cast<unsigned>(p.kv_heads);  // of keys; as many of values behind them
-    const unsigned first = ((blockIdx.x * 256u + threadIdx.x) >> 5) * (RPW * U) + lane / LPR;
+    const unsigned first = (blockIdx.x * 8u + (threadIdx.x >> 5)) * (RPW * U) + lane / LPR;  // (warps are counted: threads may pass 32 bits)
     uint4 raw[U];
     long long slot[U];
     int t[U], h[U], pos[U];

@@ -196,6 +196,22 @@ def test_cache_write(ctx, T, kv, dim, rot, page, layout, normed):
             assert bool((err <= (2.0 ** -8 + 2.0 ** -14) * (size + ref.abs())).all())
 
 
+def test_cache_write_of_more_threads_than_32_bits(ctx):
+    """2^27 + 16 head rows of 32 lanes each: the last tokens' values are written by the last blocks."""
+    T, dim, g = 2 ** 26 + 8, 256, gen(19)
+    x = torch.empty(T, 1, dim, dtype=torch.bfloat16, device=DEV)  # 34 GB, keys and values in one; only the last rows are copied
+    x[-3:] = bf(g, 3, 1, dim)
+    slots, positions = torch.full((T,), -1, dtype=torch.int32, device=DEV), torch.zeros(T, dtype=torch.int32, device=DEV)
+    slots[-3:] = ints([2, 0, 1])
+    kc, vc = torch.zeros(2, 1, 4, 1, dim, dtype=torch.bfloat16, device=DEV)
+    cos, sin = torch.ones(1, 8, device=DEV), torch.zeros(1, 8, device=DEV)
+    paged.cache_write(x, x, kc, vc, slots, norm_weight=bf(g, dim), cos=cos, sin=sin, positions=positions, rotary_dim=16)
+    ctx.sync()
+    assert torch.equal(vc[0, [2, 0, 1]], x[-3:]) and int((kc[0, :3] != 0).any(-1).sum()) == 3 and not kc[0, 3].any() and not vc[0, 3].any()
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_cache_write_reports_slots_and_positions_outside(ctx):
     g = gen(1)
     k, v, kc = bf(g, 3, 1, 64), bf(g, 3, 1, 64), bf(g, 2, 16, 1, 64)
