@@ -216,6 +216,10 @@ class PagedCache:
     def __init__(self, cfg, rows: int, num_pages: int, page_size: int = 64, max_length: int = 8192, dev="cuda"):
         if rows < 1 or num_pages < 1 or max_length < 1 or page_size < 1 or page_size & (page_size - 1):
             raise ValueError("rows, num_pages and max_length must be positive, page_size a power of two")
+        if rows > 8192 or page_size > 65536 or num_pages >= 1 << 30 or num_pages * page_size > 1 << 31 or max_length > 1 << 30:
+            raise ValueError("at most 8192 rows, pages of 65536 tokens, 2^31 tokens in all pages and 2^30 in a row")
+        if cfg.head_dim not in (64, 128, 256):
+            raise ValueError(f"the paged attention has head dim 64, 128 or 256, not {cfg.head_dim}")
         self.rows, self.num_pages, self.page_size, self.max_length = int(rows), int(num_pages), int(page_size), int(max_length)
         dev = torch.device(dev)
         if dev.type != "cuda":
@@ -225,6 +229,9 @@ class PagedCache:
         self.device = dev
         i32 = dict(dtype=torch.int32, device=dev)
         width = -(-max_length // page_size)
+        spans = rows * cfg.num_key_value_heads * -(-cfg.num_attention_heads // (8 * cfg.num_key_value_heads))  # s1_attention_paged's limit
+        if (spans + 1) * (width * page_size // 64 + 5) > 1 << 31:
+            raise ValueError("rows x KV heads x max_length / 64 must be below 2^31")
         self.tables = torch.zeros((rows, width), **i32)
         self.lengths = torch.full((rows,), -1, **i32)
         self.free_pages = torch.arange(num_pages - 1, -1, -1, **i32)

@@ -35,6 +35,15 @@ def test_python_calls_refuse_cpu_tensors():
         paged.PagedCache(cfg, rows=1, num_pages=1, page_size=24)
 
 
+@pytest.mark.parametrize("bad,match", [(dict(rows=8193), "8192"), (dict(page_size=1 << 17), "65536"), (dict(num_pages=1 << 26), "2.31"),
+                                       (dict(max_length=(1 << 30) + 1), "2.30"), (dict(head_dim=96), "96")])
+def test_the_cache_refuses_what_its_kernels_do(bad, match):
+    """Before anything is allocated: a step that the kernels refuse would leave the rows' lengths a token ahead of their keys."""
+    cfg = type("Cfg", (), dict(linear_num_key_heads=1, linear_num_value_heads=1, num_hidden_layers=0, head_dim=bad.pop("head_dim", 64)))()
+    with pytest.raises(ValueError, match=match):
+        paged.PagedCache(cfg, **{**dict(rows=1, num_pages=1), **bad}, dev="cpu")
+
+
 def test_c_calls_refuse_a_null_context():
     lib = _lib.load_library()
     n = None
