@@ -204,6 +204,12 @@ class DeltaState(NamedTuple):
     state: torch.Tensor
 
 
+def layout(cfg) -> tuple:
+    """What a decoder of configuration `cfg` keeps of a request in each layer: KV heads and head dim, or key and value heads."""
+    return tuple(("pages", cfg.num_key_value_heads, cfg.head_dim) if cfg.layer_type(i) == "full_attention" else
+                 ("state", cfg.linear_num_key_heads, cfg.linear_num_value_heads) for i in range(cfg.num_hidden_layers))
+
+
 class PagedCache:
     """The memory of up to `rows` requests in flight for a decoder of configuration `cfg` (see `qwen35.Decoder`): `num_pages` pages of
     `page_size` tokens that the rows share, at most `max_length` tokens a row, and one recurrent state a row and layer.
@@ -241,6 +247,7 @@ class PagedCache:
         self.pages_left = int(num_pages)
         channels = (2 * cfg.linear_num_key_heads + cfg.linear_num_value_heads) * 128
         self.layers: List = []
+        self.layout = layout(cfg)
         for i in range(cfg.num_hidden_layers):
             if cfg.layer_type(i) == "full_attention":
                 shape = (num_pages, page_size, cfg.num_key_value_heads, cfg.head_dim)

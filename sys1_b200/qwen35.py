@@ -218,8 +218,10 @@ class LinearAttention:
         tail = (P(bb), P(aa), bb.stride(0), P(self.dt_bias), P(self.decay), P(zz), zz.stride(0), P(self.norm), C.c_float(self.eps), offsets,
                 len(cu) - 1, T, self.key_heads, self.value_heads, P(y), y.stride(0), C.c_void_p(ptr), need)
         if kept is not None:
-            conv, state = kept.layer
-            rc = ctx._lib.s1_gated_delta_rule_prefill(ctx.handle, P(pre), pre.stride(0), P(self.conv_taps), P(positions), *tail, P(kept.cu_seqlens),
+            conv, state, pos = *kept.layer, kept.positions
+            if state.shape[1:] != (self.value_heads, 128, 128) or conv.shape[1:] != (4, pre.shape[1]) or conv.shape[0] != state.shape[0]:
+                raise ValueError(f"the states are those of other heads: {list(conv.shape)} and {list(state.shape)}")
+            rc = ctx._lib.s1_gated_delta_rule_prefill(ctx.handle, P(pre), pre.stride(0), P(self.conv_taps), P(pos), *tail, P(kept.cu_seqlens),
                                                       P(kept.state_index), state.shape[0], P(conv), P(state))
         elif self.fuse_conv:
             pos = positions if positions.dtype == torch.int32 and positions.is_contiguous() else positions.to(torch.int32).contiguous()
@@ -458,7 +460,7 @@ class Decoder:
     linear-attention layers, see `LinearAttention`."""
 
     def __init__(self, weights, cfg, max_positions: int = 8192, recurrence: str = "chunked"):
-        self.cfg, self.w, self.max_positions = cfg, weights, int(max_positions)
+        self.cfg, self.w, self.max_positions, self.layout = cfg, weights, int(max_positions), paged.layout(cfg)
         dev = weights["embed_tokens"].device
         lin = lambda name: Linear(weights[name])
         rope = RopeParams(cfg.rope_theta, cfg.rotary_dim, max_positions, dev)
@@ -553,8 +555,8 @@ class Decoder:
     def _check(self, cache, ids) -> None:
         if cache.device != ids.device or cache.device != self.w["embed_tokens"].device:
             raise ValueError("the cache, the ids and the weights must be on one GPU")
-        if len(cache.layers) != len(self.layers):
-            raise ValueError(f"the cache was made for {len(cache.layers)} layers, the decoder has {len(self.layers)}")
+        if cache.layout != self.layout:
+            raise ValueError("the cache was made for a decoder of other layers or heads")
 
 
 def batch_plan_cached(owner, ctx, bounds):

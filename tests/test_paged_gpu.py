@@ -4,6 +4,8 @@ prompt leaves, each against 64-bit arithmetic or an integer model, then the deco
 Tolerances count roundings. A value rounded to bf16 is off by at most 2^-8 of itself. Paged attention rounds every softmax weight
 to bf16 once (2^-8 of the weight, so 2^-8 of the output's sum taken with |v|) and its output once; its f32 sums and exponentials
 stay below 2^-15 of the same sums. The step kernel is f32 throughout (`paged_model.delta_step_64` carries the bound)."""
+import dataclasses
+
 import numpy as np
 import pytest
 import torch
@@ -723,3 +725,17 @@ def test_the_cache_refuses_what_does_not_fit(ctx):
     with pytest.raises(ValueError, match="33 positions"):
         short.step(ids[:2], cache)
     ctx.sync()
+
+
+@pytest.mark.parametrize("other", [dict(linear_num_value_heads=4), dict(linear_num_key_heads=2), dict(num_key_value_heads=1), dict(head_dim=128),
+                                   dict(num_hidden_layers=8), dict(full_attention_interval=2)])
+def test_the_decoder_refuses_the_cache_of_another(ctx, other):
+    cfg, w, dec = _decoder()
+    cache = paged.PagedCache(dataclasses.replace(cfg, **other), rows=2, num_pages=4, page_size=16, max_length=32, dev=DEV)
+    ids = torch.zeros(5, dtype=torch.int64, device=DEV)
+    with pytest.raises(ValueError, match="other layers or heads"):
+        dec.prefill(ids, [5], cache)
+    with pytest.raises(ValueError, match="other layers or heads"):
+        dec.step(ids[:2], cache)
+    ctx.sync()
+    assert cache.held.tolist() == [-1, -1] and cache.lengths.tolist() == [-1, -1]
