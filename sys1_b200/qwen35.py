@@ -547,8 +547,10 @@ class Decoder:
             raise ValueError(f"a row has reached the decoder's {self.max_positions} positions")
         plan = cache.extend()
         x = _norm.embedding(self.w["embed_tokens"], ids.to(torch.int32).contiguous())
+        # a row that got no page (a replayed step that the host did not look after) has no slot, and keeps its states as they are
+        index = torch.where(plan.slots < 0, plan.slots, cache.state_index)
         for layer, part in zip(self.layers, cache.layers):
-            x = layer.step(x, Kept(part, plan.positions, plan.slots, cache.state_index, tables=cache.tables, lengths=cache.lengths,
+            x = layer.step(x, Kept(part, plan.positions, plan.slots, index, tables=cache.tables, lengths=cache.lengths,
                                    workspace=cache.workspace), inplace=True)
         return self.norm(x)
 

@@ -684,6 +684,31 @@ def test_a_captured_step_is_the_step(ctx):
         b.advanced(100)
 
 
+def test_a_row_that_gets_no_page_keeps_its_states(ctx, monkeypatch):
+    """A step that the host's mirror did not look after (a replay without `advanced`): the row without a page is reported and stays
+    where it was, the others go on; once pages are free again, it goes on too."""
+    cfg, w, dec = _decoder()
+    cache, free = (paged.PagedCache(cfg, rows=3, num_pages=n, page_size=16, max_length=64, dev=DEV) for n in (4, 12))
+    ids = torch.randint(0, 500, (47,), generator=torch.Generator().manual_seed(6)).to(DEV)
+    for c in (cache, free):
+        dec.prefill(ids, [10, 32, 5], c)
+    tokens = torch.randint(0, 500, (2, 3), generator=torch.Generator().manual_seed(7)).to(DEV)
+    before = [(t.state[1].clone(), t.conv[1].clone()) for t in cache.layers if isinstance(t, paged.DeltaState)]
+    monkeypatch.setattr(cache, "fits", lambda steps=1: True)
+    y = dec.step(tokens[0], cache)
+    _refused(ctx, "no free pages")
+    want = dec.step(tokens[0], free)
+    assert torch.equal(y[[0, 2]], want[[0, 2]]) and cache.lengths.tolist() == [11, 32, 6] and cache.free_count.tolist() == [0]
+    for t, (state, conv) in zip((t for t in cache.layers if isinstance(t, paged.DeltaState)), before):
+        assert torch.equal(t.state[1], state) and torch.equal(t.conv[1], conv)
+    monkeypatch.undo()
+    cache.held[:], cache.pages_left = [11, 32, 6], 0
+    cache.release([0])
+    assert max_rel(dec.step(tokens[0], cache)[1], want[1]) <= 2e-2
+    ctx.sync()
+    assert cache.lengths.tolist() == [-1, 33, 7] == cache.held.tolist()
+
+
 def test_a_prefill_that_fails_leaves_the_cache_as_it_was(ctx, monkeypatch):
     cfg, w, dec = _decoder(layers=2)
     cache = paged.PagedCache(cfg, rows=3, num_pages=8, page_size=16, max_length=64, dev=DEV)
