@@ -199,6 +199,8 @@ def load(ordinal: Optional[int] = None) -> Context:
     """Context for GPU `ordinal` (default: PyTorch's current device) on PyTorch's current stream."""
     if ordinal is None:
         ordinal = torch.cuda.current_device()
+    if not _contexts:
+        torch.cuda.init()  # (the bare handle does not start CUDA, nor say why it cannot)
     key = (ordinal, _current_stream(ordinal))
     ctx = _contexts.get(key)
     if ctx is None:

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from paged_model import block_tables_model, release_model
-from sys1_b200 import _lib, paged, qwen35
+from sys1_b200 import _lib, device, paged, qwen35
 
 
 def _i(*shape):
@@ -53,6 +53,16 @@ def test_c_calls_refuse_a_null_context():
     assert lib.s1_attention_paged(n, n, 0, 0, n, n, 1, 16, 0, 0, 0, n, 0, 0, n, 1, 1, 1, 64, 1.0, n, 0, 0, n, 0, n, 0) == _lib.S1_EINVAL
     assert lib.s1_gated_delta_rule_step(n, n, 0, n, n, n, n, 0, n, n, n, 0, n, 0.0, n, 1, n, n, 1, 1, 1, n, 0) == _lib.S1_EINVAL
     assert lib.s1_gated_delta_rule_prefill(n, n, 0, n, n, n, n, 0, n, n, n, 0, n, 0.0, n, 1, 1, 1, 1, n, 0, n, 0, n, n, 1, n, n) == _lib.S1_EINVAL
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="says what happens without a GPU")
+@pytest.mark.parametrize("ordinal", [None, 0])
+def test_a_context_without_a_gpu_says_so(ordinal):
+    with pytest.raises(Exception) as plain:
+        torch.cuda.init()
+    with pytest.raises(type(plain.value)) as e:
+        device.load(ordinal)
+    assert str(e.value) == str(plain.value)
 
 
 def test_workspace_sizes():
