@@ -97,6 +97,8 @@ def block_tables(cached: torch.Tensor, tables: torch.Tensor, free_pages: torch.T
         op, count = _ints(free_count_out, dev, 1, "free_count_out"), free_count_out
     if ctx is None:
         ctx = device.load(dev)
+    elif ctx.ordinal != dev:
+        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
     rc = ctx._lib.s1_block_tables(ctx._h, cp, ap, rows, page_size, fp, pool, np_, op, tp, ldt, width, lp, up, pp, sp, max_tokens)
     if rc:
         ctx.check(rc)
@@ -112,6 +114,8 @@ def release_blocks(ended: torch.Tensor, lengths: torch.Tensor, tables: torch.Ten
     tp, ldt, width = _table(tables, dev, rows)
     if ctx is None:
         ctx = device.load(dev)
+    elif ctx.ordinal != dev:
+        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
     ctx.check(ctx._lib.s1_release_blocks(ctx._h, ep, rows, page_size, lp, tp, ldt, width, fp, pool, np_))
 
 
@@ -142,6 +146,8 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
         return
     if ctx is None:
         ctx = device.load(dev)
+    elif ctx.ordinal != dev:
+        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
     rc = ctx._lib.s1_cache_write(ctx._h, kp, ldk, khs, vp, ldv, vhs, sp, T, kv, dim, wp, eps, cp, np_, pp, rows, rotary_dim, 1 if bf16_ops else 0,
                                  k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs)
     if rc:
@@ -173,6 +179,8 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         return out
     if ctx is None:
         ctx = device.load(dev)
+    elif ctx.ordinal != dev:
+        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
     if workspace is None:
         workspace = ctx.attention_workspace()
     elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():

@@ -287,6 +287,8 @@ def gated_delta_rule_step(mixed: torch.Tensor, conv_weight: torch.Tensor, positi
         return out
     if ctx is None:
         ctx = device.load(dev)
+    elif ctx.ordinal != dev:
+        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
     rc = ctx._lib.s1_gated_delta_rule_step(
         ctx._h, mixed.data_ptr(), mixed.stride(0), conv_weight.data_ptr(), positions.data_ptr(), b.data_ptr(), a.data_ptr(), ldba, dt_bias.data_ptr(),
         neg_exp_a.data_ptr(), z.data_ptr(), z.stride(0), norm_weight.data_ptr(), eps, 0 if state_index is None else state_index.data_ptr(), states,

@@ -764,3 +764,18 @@ def test_the_decoder_refuses_the_cache_of_another(ctx, other):
         dec.step(ids[:2], cache)
     ctx.sync()
     assert cache.held.tolist() == [-1, -1] and cache.lengths.tolist() == [-1, -1]
+
+
+def test_a_context_of_another_gpu_is_refused(ctx):
+    other = type("Other", (), dict(ordinal=1))()
+    g, i32 = gen(1), ints([0])
+    kc = bf(g, 2, 16, 1, 64)
+    x = bf(g, 1, 384)
+    for call in (lambda: paged.block_tables(i32, ints([[0]]), ints([0]), i32, 16, ctx=other),
+                 lambda: paged.release_blocks(i32, i32, ints([[0]]), ints([0]), i32, 16, ctx=other),
+                 lambda: paged.cache_write(kc[:1, 0], kc[:1, 0], kc, kc, i32, ctx=other),
+                 lambda: paged.attention_paged(kc[:1, 0], kc, kc, ints([[0]]), i32, ctx=other),
+                 lambda: qwen35.gated_delta_rule_step(x, bf(g, 384, 4), i32, x[:, :1], x[:, :1], torch.zeros(1, device=DEV), torch.zeros(1, device=DEV),
+                                                      x[:, :128], x[0, :128], 1e-6, bf(g, 1, 4, 384), torch.zeros(1, 1, 128, 128, device=DEV), 1, ctx=other)):
+        with pytest.raises(ValueError, match="GPU 0, the context on GPU 1"):
+            call()
