@@ -14,6 +14,7 @@ import numpy as np
 import torch
 
 from . import device
+from ._lib import packed
 
 
 class BlockTables(NamedTuple):
@@ -27,6 +28,7 @@ class BlockTables(NamedTuple):
 
 
 _I32, _BF16 = torch.int32, torch.bfloat16
+_block_tables, _cache_write, _attention_paged = packed("s1_block_tables"), packed("s1_cache_write"), packed("s1_attention_paged")
 
 
 def _ints(t: torch.Tensor, dev: int, n: int, name: str) -> int:
@@ -90,7 +92,7 @@ def block_tables(cached: torch.Tensor, tables: torch.Tensor, free_pages: torch.T
     out = cached.new_empty(2 * rows + 2 + 2 * max_tokens)
     at = out.data_ptr()
     lp, up, pp, sp, op = at, at + 4 * rows, at + 4 * (2 * rows + 1), at + 4 * (2 * rows + 1 + max_tokens), at + 4 * (2 * rows + 1 + 2 * max_tokens)
-    new_lengths, cu, positions, slots, count = out.split_with_sizes((rows, rows + 1, max_tokens, max_tokens, 1))
+    new_lengths, cu, positions, slots, count = torch.unsafe_split_with_sizes(out, (rows, rows + 1, max_tokens, max_tokens, 1))
     if lengths is not None:
         lp, new_lengths = _ints(lengths, dev, rows, "lengths"), lengths
     if free_count_out is not None:
@@ -99,7 +101,7 @@ def block_tables(cached: torch.Tensor, tables: torch.Tensor, free_pages: torch.T
         ctx = device.load(dev)
     elif ctx.ordinal != dev:
         raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
-    rc = ctx._lib.s1_block_tables(ctx._h, cp, ap, rows, page_size, fp, pool, np_, op, tp, ldt, width, lp, up, pp, sp, max_tokens)
+    rc = _block_tables(ctx._h, cp, ap, rows, page_size, fp, pool, np_, op, tp, ldt, width, lp, up, pp, sp, max_tokens)
     if rc:
         ctx.check(rc)
     return BlockTables(new_lengths, cu, positions, slots, count)
@@ -148,7 +150,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
         ctx = device.load(dev)
     elif ctx.ordinal != dev:
         raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
-    rc = ctx._lib.s1_cache_write(ctx._h, kp, ldk, khs, vp, ldv, vhs, sp, T, kv, dim, wp, eps, cp, np_, pp, rows, rotary_dim, 1 if bf16_ops else 0,
+    rc = _cache_write(ctx._h, kp, ldk, khs, vp, ldv, vhs, sp, T, kv, dim, wp, eps, cp, np_, pp, rows, rotary_dim, 1 if bf16_ops else 0,
                                  k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs)
     if rc:
         ctx.check(rc)
@@ -185,7 +187,7 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         workspace = ctx.attention_workspace()
     elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
         raise ValueError("the workspace must be a contiguous uint8 CUDA tensor")
-    rc = ctx._lib.s1_attention_paged(ctx._h, qp, ldq, qhs, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs, tp, ldt, width, lp, B, H, kv, dim,
+    rc = _attention_paged(ctx._h, qp, ldq, qhs, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs, tp, ldt, width, lp, B, H, kv, dim,
                                      dim ** -0.5 if scale is None else scale, gp, ldg, ghs, out.data_ptr(), out.stride(0), workspace.data_ptr(),
                                      workspace.numel())
     if rc:

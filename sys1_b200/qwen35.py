@@ -15,7 +15,7 @@ import torch
 from . import device
 from . import norm as _norm
 from . import paged
-from ._lib import EPI_SWIGLU
+from ._lib import EPI_SWIGLU, packed
 from .linear import Linear, fused_linear
 
 
@@ -248,6 +248,9 @@ class LinearAttention:
                                            P(y), y.stride(0)))
 
 
+_delta_step = packed("s1_gated_delta_rule_step")
+
+
 def gated_delta_rule_step(mixed: torch.Tensor, conv_weight: torch.Tensor, positions: torch.Tensor, b: torch.Tensor, a: torch.Tensor,
                           dt_bias: torch.Tensor, neg_exp_a: torch.Tensor, z: torch.Tensor, norm_weight: torch.Tensor, eps: float,
                           conv_state: torch.Tensor, state: torch.Tensor, key_heads: int, state_index: Optional[torch.Tensor] = None,
@@ -289,7 +292,7 @@ def gated_delta_rule_step(mixed: torch.Tensor, conv_weight: torch.Tensor, positi
         ctx = device.load(dev)
     elif ctx.ordinal != dev:
         raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
-    rc = ctx._lib.s1_gated_delta_rule_step(
+    rc = _delta_step(
         ctx._h, mixed.data_ptr(), mixed.stride(0), conv_weight.data_ptr(), positions.data_ptr(), b.data_ptr(), a.data_ptr(), ldba, dt_bias.data_ptr(),
         neg_exp_a.data_ptr(), z.data_ptr(), z.stride(0), norm_weight.data_ptr(), eps, 0 if state_index is None else state_index.data_ptr(), states,
         conv_state.data_ptr(), state.data_ptr(), rows, key_heads, Hv, out.data_ptr(), out.stride(0))

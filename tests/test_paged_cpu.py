@@ -65,6 +65,26 @@ def test_a_context_without_a_gpu_says_so(ordinal):
     assert str(e.value) == str(plain.value)
 
 
+def test_packed_calls():
+    """`s1_call` needs a context; the words of a call are its arguments, and the types agree with the header's order of calls."""
+    import re
+    from test_abi import HEADER
+    lib, text = _lib.load_library(), HEADER.read_text()
+    assert lib.s1_call(None, 0, b"", 0) == _lib.S1_EINVAL
+    numbers = {n.lower(): int(i) for n, i in re.findall(r"S1_CALL_([A-Z_]+) = (\d+)", text)}
+    assert numbers == {n[3:]: i for i, n in enumerate(_lib.PACKED)}
+    for name in _lib.PACKED:
+        declared = re.search(rf"int {name}\(([^)]*)\)", text).group(1).split(",")[1:]
+        kinds = ["d" if re.match(r"\s*float \w", d) else "q" for d in declared]
+        assert kinds == ["d" if t.__name__ == "c_float" else "q" for t in _lib.SIGNATURES[name][1][1:]], name
+        call = _lib.packed(name)
+        assert call(None, *([0] * len(declared))) == _lib.S1_EINVAL
+        with pytest.raises(Exception):
+            call(None, *([0] * (len(declared) - 1)))
+        with pytest.raises(Exception):
+            call(None, *(["0"] * len(declared)))
+
+
 def test_workspace_sizes():
     assert paged.attention_paged_workspace(96) == 0
     assert 0 < paged.attention_paged_workspace(64) < paged.attention_paged_workspace(128) < paged.attention_paged_workspace(256)

@@ -779,3 +779,17 @@ def test_a_context_of_another_gpu_is_refused(ctx):
                                                       x[:, :128], x[0, :128], 1e-6, bf(g, 1, 4, 384), torch.zeros(1, 1, 128, 128, device=DEV), 1, ctx=other)):
         with pytest.raises(ValueError, match="GPU 0, the context on GPU 1"):
             call()
+
+
+def test_packed_calls_refuse_what_is_not_their_arguments(ctx):
+    call = ctx._lib.s1_call
+    for which, words, match in ((9, 3, "no call 9"), (0, 3, "16 argument words, not 3"), (2, 25, "26 argument words, not 25")):
+        with pytest.raises(_lib.S1Error, match=match):
+            ctx.check(call(ctx.handle, which, bytes(8 * words), words))
+    with pytest.raises(_lib.S1Error, match="null pointer"):
+        ctx.check(call(ctx.handle, 0, None, 16))
+    with pytest.raises(_lib.S1Error, match="beyond 32 bits"):
+        paged.block_tables(ints([3]), ints([[0]]), ints([0]), ints([1]), 2 ** 32 + 16)
+    with pytest.raises(_lib.S1Error, match="power of two"):
+        paged.block_tables(ints([3]), ints([[0]]), ints([0]), ints([1]), 24)
+    ctx.sync()
