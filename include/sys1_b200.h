@@ -435,19 +435,6 @@ int s1_gated_delta_rule_step(s1_ctx* ctx, const void* mixed, long long ldm, cons
                              void* conv_state, float* state, int num_seqs, int key_heads, int value_heads, void* y, long long ldy);
 
 /*
- * The calls of a decoding step for bindings whose foreign calls cost by the argument: args points to `words` 8-byte words, the
- * arguments of call `which` after ctx in their order - pointers and integers as int64, floats as double. Same checks, same results;
- * an int argument beyond 32 bits, or another number of words than the call has arguments, is refused.
- */
-enum {
-    S1_CALL_BLOCK_TABLES = 0,
-    S1_CALL_CACHE_WRITE = 1,
-    S1_CALL_ATTENTION_PAGED = 2,
-    S1_CALL_GATED_DELTA_RULE_STEP = 3
-};
-int s1_call(s1_ctx* ctx, int which, const void* args, int words);
-
-/*
  * Tensor parallelism: the sum over ranks that follows a row-parallel projection (each rank holds a K range of the
  * weight and produces a partial [T, N]). The reference has no multi-GPU path (`device::load` opens GPU 0 only,
  * src/device.rs:43-56); these entry points exist for the sharded projections of the large hybrid model.

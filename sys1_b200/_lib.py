@@ -7,7 +7,6 @@ to the library are plain addresses.
 from __future__ import annotations
 
 import ctypes as C
-import struct
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -120,32 +119,11 @@ SIGNATURES = {
     "s1_gated_delta_rule_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                            C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_float,
                                            C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_longlong]),
-    "s1_call": (C.c_int, [C.c_void_p, C.c_int, C.c_char_p, C.c_int]),
     "s1_linear_rope": (C.c_int, [C.c_void_p, C.POINTER(LinearDesc), C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int,
                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
     "s1_linear": (C.c_int, [C.c_void_p, C.POINTER(LinearDesc), C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong,
                             C.c_void_p, C.c_longlong, C.c_int]),
 }
-
-# The calls that `s1_call` takes with their arguments packed into one array of 8-byte words, in its numbering.
-PACKED = ("s1_block_tables", "s1_cache_write", "s1_attention_paged", "s1_gated_delta_rule_step")
-
-
-def packed(name: str):
-    """`name` of the C ABI as `f(ctx_handle, *arguments)`, through `s1_call`: ctypes converts four arguments instead of up to 27 (0.2 us
-    each, more than the rest of a small call). Numbers and addresses only."""
-    which, types = PACKED.index(name), SIGNATURES[name][1][1:]
-    words, pack = len(types), struct.Struct("=" + "".join("d" if t is C.c_float else "q" for t in types)).pack
-    call = None
-
-    def packed_call(handle, *args):
-        nonlocal call
-        if call is None:
-            call = load_library().s1_call
-        return call(handle, which, pack(*args), words)
-
-    return packed_call
-
 
 _lib = None
 
@@ -166,3 +144,20 @@ def load_library() -> C.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+binding = None  # the module of `load_binding`, once loaded
+
+
+def load_binding():
+    """The compiled Python side of the decode-step calls (`csrc/binding.cpp`), which calls the same library. Raises if it has not been built."""
+    global binding
+    if binding is None:
+        load_library()
+        try:
+            from . import _binding
+        except ImportError as exc:
+            raise RuntimeError(f"{PKG / '_binding.so'} cannot be loaded ({exc}): build it with `python -m sys1_b200.build`. "
+                               "There is no fallback for this path.") from exc
+        binding = _binding
+    return binding

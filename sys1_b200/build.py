@@ -2,17 +2,21 @@
 
 Takes the place of the reference's `build.rs:51-83` (which concatenates `src/kernels/*.cu` and emits generic
 PTX for whatever compute capability it finds): here there is exactly one target, `sm_100a`, and the output is
-a shared library exporting the C ABI declared in `include/sys1_b200.h`.
+a shared library exporting the C ABI declared in `include/sys1_b200.h`. Beside it goes `_binding.so`, the Python side of the
+decode-step calls (`csrc/binding.cpp`, g++), built against this interpreter and its PyTorch.
 
 Run as `python -m sys1_b200.build` (add `-v` for the ptxas resource report).
 """
 from __future__ import annotations
 
 import hashlib
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,7 +26,7 @@ LIB = PKG / "libsys1_b200.so"
 STAMP = PKG / "csrc" / ".build_stamp"
 OBJ = PKG / "csrc" / ".obj"
 
-SOURCES = ["api.cu", "linear_static.cu", "batching.cu", "plan.cu", "delta_rule.cu", "delta_chunked.cu", "delta_io.cu", "attention.cu", "attention_gqa.cu", "norm_rope.cu", "paged_cache.cu", "attention_paged.cu", "delta_step.cu", "call.cu", "comm.cu", "exchange.cu"]
+SOURCES = ["api.cu", "linear_static.cu", "batching.cu", "plan.cu", "delta_rule.cu", "delta_chunked.cu", "delta_io.cu", "attention.cu", "attention_gqa.cu", "norm_rope.cu", "paged_cache.cu", "attention_paged.cu", "delta_step.cu", "comm.cu", "exchange.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
@@ -30,6 +34,18 @@ NVCC_FLAGS = [
     "--expt-relaxed-constexpr",
     "-Xcudafe", "--diag_suppress=177",
 ]
+
+
+BINDING = PKG / "_binding.so"
+
+
+def _binding_command() -> list:
+    """g++ on the Python side of the decode-step calls, against this interpreter's and its PyTorch's headers and the library beside it."""
+    torch_dir = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    inc = [sysconfig.get_paths()["include"], torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include"]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", *(f"-I{p}" for p in inc),
+            str(CSRC / "binding.cpp"), "-o", str(BINDING), "-L", str(PKG), "-l:libsys1_b200.so", "-L", str(torch_dir / "lib"),
+            "-ltorch_python", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN"]
 
 
 def _nvcc() -> str:
@@ -50,9 +66,10 @@ def _deps_digest() -> str:
 
 def _fingerprint() -> str:
     h = hashlib.sha256(_deps_digest().encode())
-    for f in sorted(CSRC.glob("*.cu")):
+    for f in sorted([*CSRC.glob("*.cu"), *CSRC.glob("*.cpp")]):
         h.update(f.name.encode())
         h.update(f.read_bytes())
+    h.update((importlib.metadata.version("torch") + sys.version).encode())  # the binding is built against these
     return h.hexdigest()
 
 
@@ -61,7 +78,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     compiled to an object of its own (in parallel, and only if it or a header changed), then the objects are linked."""
     from concurrent.futures import ThreadPoolExecutor
     fp = _fingerprint()
-    if not force and LIB.exists() and STAMP.exists() and STAMP.read_text().strip() == fp:
+    if not force and LIB.exists() and BINDING.exists() and STAMP.exists() and STAMP.read_text().strip() == fp:
         return LIB
     nvcc = _nvcc()
     OBJ.mkdir(exist_ok=True)
@@ -94,6 +111,10 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("linking libsys1_b200.so failed")
+    res = subprocess.run(_binding_command(), capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("building _binding.so failed")
     STAMP.write_text(fp)
     return LIB
 

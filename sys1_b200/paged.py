@@ -13,8 +13,7 @@ from typing import List, NamedTuple, Optional, Sequence
 import numpy as np
 import torch
 
-from . import device
-from ._lib import packed
+from . import _lib, device
 
 
 class BlockTables(NamedTuple):
@@ -28,7 +27,6 @@ class BlockTables(NamedTuple):
 
 
 _I32, _BF16 = torch.int32, torch.bfloat16
-_block_tables, _cache_write, _attention_paged = packed("s1_block_tables"), packed("s1_cache_write"), packed("s1_attention_paged")
 
 
 def _ints(t: torch.Tensor, dev: int, n: int, name: str) -> int:
@@ -46,28 +44,15 @@ def _table(t: torch.Tensor, dev: int, rows: int):
     return t.data_ptr(), t.stride(0), t.shape[1]
 
 
-def _heads(t: torch.Tensor, dev: int, shape, name: str):
-    """Address, token stride and head stride of a tensor of head rows."""
-    if t.dtype is not _BF16 or t.get_device() != dev or dev < 0 or t.dim() != 3:
-        raise ValueError(f"{name} must be a bf16 CUDA tensor [tokens, heads, head_dim] with contiguous head rows (no CPU fallback)")
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
-    token, head, one = t.stride()
-    if one != 1:
-        raise ValueError(f"{name} must have contiguous head rows")
-    return t.data_ptr(), token, head
-
-
-def _caches(k: torch.Tensor, v: torch.Tensor, dev: int):
-    """The caches' shape and strides."""
-    for t in (k, v):
-        if t.dtype is not _BF16 or t.get_device() != dev or dev < 0 or t.dim() != 4:
-            raise ValueError("k_cache and v_cache must be bf16 CUDA tensors [pages, page_size, kv_heads, head_dim] with contiguous head rows "
-                             "(no CPU fallback)")
-    shape, strides = k.shape, k.stride()
-    if v.shape != shape or v.stride() != strides or strides[3] != 1:
-        raise ValueError("k_cache and v_cache must have the same shape and strides, and contiguous head rows")
-    return shape, strides
+def _context(dev: int, ctx: Optional[device.Context]):
+    """The context of a call on tensors of GPU `dev` (-1: none - the call will refuse them) and its address."""
+    if ctx is None:
+        if dev < 0:
+            return None, None
+        ctx = device.load(dev)
+    elif ctx.ordinal != dev:
+        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
+    return ctx, ctx.handle.value
 
 
 def block_tables(cached: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
@@ -78,33 +63,11 @@ def block_tables(cached: torch.Tensor, tables: torch.Tensor, free_pages: torch.T
     pages are taken from, `tables` int32 `[rows, width]` updated in place. `max_tokens`: tokens of the packed batch, with those
     behind the last row (needed with `added`). `lengths` may be `cached` and `free_count_out` may be `free_count`: both are then
     advanced in place."""
-    dev, rows, pool = cached.get_device(), cached.numel(), free_pages.numel()
-    if max_tokens is None:
-        if added is not None:
-            raise ValueError("max_tokens is needed with `added`: the host knows how many tokens the batch has")
-        max_tokens = rows
-    if max_tokens < 0:
-        raise ValueError("max_tokens must not be negative")
-    cp, fp, np_ = _ints(cached, dev, rows, "cached"), _ints(free_pages, dev, pool, "free_pages"), _ints(free_count, dev, 1, "free_count")
-    ap = 0 if added is None else _ints(added, dev, rows, "added")
-    tp, ldt, width = _table(tables, dev, rows)
-    # one buffer for what is new: lengths, first tokens, positions, slots, pages left
-    out = cached.new_empty(2 * rows + 2 + 2 * max_tokens)
-    at = out.data_ptr()
-    lp, up, pp, sp, op = at, at + 4 * rows, at + 4 * (2 * rows + 1), at + 4 * (2 * rows + 1 + max_tokens), at + 4 * (2 * rows + 1 + 2 * max_tokens)
-    new_lengths, cu, positions, slots, count = torch.unsafe_split_with_sizes(out, (rows, rows + 1, max_tokens, max_tokens, 1))
-    if lengths is not None:
-        lp, new_lengths = _ints(lengths, dev, rows, "lengths"), lengths
-    if free_count_out is not None:
-        op, count = _ints(free_count_out, dev, 1, "free_count_out"), free_count_out
-    if ctx is None:
-        ctx = device.load(dev)
-    elif ctx.ordinal != dev:
-        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
-    rc = _block_tables(ctx._h, cp, ap, rows, page_size, fp, pool, np_, op, tp, ldt, width, lp, up, pp, sp, max_tokens)
-    if rc:
-        ctx.check(rc)
-    return BlockTables(new_lengths, cu, positions, slots, count)
+    ctx, handle = _context(cached.get_device(), ctx)
+    r = (_lib.binding or _lib.load_binding()).block_tables(handle, cached, tables, free_pages, free_count, page_size, added, max_tokens, lengths, free_count_out)
+    if r.__class__ is int:
+        ctx.check(r)
+    return BlockTables._make(r)
 
 
 def release_blocks(ended: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
@@ -127,31 +90,8 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     """Keys and values `[T, kv_heads, head_dim]` (rows may be strided) into the slots of `k_cache`, `v_cache` `[pages, page_size,
     kv_heads, head_dim]` (`s1_cache_write`); a token with slot -1 is left out. With `norm_weight` `[head_dim]` the keys are normed and
     rotated on the way, as `norm.head_norm_rope_` would do in place (`cos`, `sin` f32 `[positions, rotary_dim / 2]`)."""
-    dev = k.get_device()
-    (pages, page, kv, dim), (ps, ts, hs, _) = _caches(k_cache, v_cache, dev)
-    T = k.shape[0]
-    kp, ldk, khs = _heads(k, dev, (T, kv, dim), "k")
-    vp, ldv, vhs = _heads(v, dev, (T, kv, dim), "v")
-    sp = _ints(slots, dev, T, "slots")
-    wp = cp = np_ = pp = rows = 0
-    if norm_weight is not None:
-        if cos is None or sin is None or positions is None:
-            raise ValueError("keys that are normed are rotated too: cos, sin and positions are needed")
-        if norm_weight.get_device() != dev or norm_weight.dtype is not _BF16 or norm_weight.shape != (dim,) or not norm_weight.is_contiguous():
-            raise ValueError(f"norm_weight must be a contiguous bf16 CUDA tensor [{dim}]")
-        rows = cos.shape[0]
-        for t in (cos, sin):
-            if t.get_device() != dev or t.dtype is not torch.float32 or t.shape != (rows, rotary_dim // 2) or not t.is_contiguous():
-                raise ValueError("cos and sin must be contiguous f32 CUDA tensors [positions, rotary_dim / 2]")
-        wp, cp, np_, pp = norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ints(positions, dev, T, "positions")
-    if T == 0:
-        return
-    if ctx is None:
-        ctx = device.load(dev)
-    elif ctx.ordinal != dev:
-        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
-    rc = _cache_write(ctx._h, kp, ldk, khs, vp, ldv, vhs, sp, T, kv, dim, wp, eps, cp, np_, pp, rows, rotary_dim, 1 if bf16_ops else 0,
-                                 k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs)
+    ctx, handle = _context(k.get_device(), ctx)
+    rc = (_lib.binding or _lib.load_binding()).cache_write(handle, k, v, k_cache, v_cache, slots, norm_weight, eps, cos, sin, positions, rotary_dim, bf16_ops)
     if rc:
         ctx.check(rc)
 
@@ -163,42 +103,18 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     heads, head_dim]` (rows may be strided), optional gate of the same shape (pre-sigmoid). Rows of length <= 0 get zeros. Returns
     `[rows, heads * head_dim]`. `workspace`: uint8 CUDA tensor of `attention_paged_workspace(head_dim)` bytes; by default
     the context's own, which the calls of one stream share. Graphs that may run at the same time need one each."""
-    dev = q.get_device()
-    (pages, page, kv, dim), (ps, ts, hs, _) = _caches(k_cache, v_cache, dev)
-    shape = q.shape
-    B, H = shape[0], shape[1]
-    qp, ldq, qhs = _heads(q, dev, (B, H, dim), "q")
-    tp, ldt, width = _table(tables, dev, B)
-    lp = _ints(lengths, dev, B, "lengths")
-    gp = ldg = ghs = 0
-    if gate is not None:
-        gp, ldg, ghs = _heads(gate, dev, (B, H, dim), "gate")
-    if out is None:
-        out = q.new_empty((B, H * dim))
-    elif out.get_device() != dev or out.dtype is not _BF16 or out.shape != (B, H * dim) or out.stride(1) != 1:
-        raise ValueError(f"out must be a bf16 CUDA tensor [{B}, {H * dim}] with contiguous rows")
-    if B == 0:
-        return out
-    if ctx is None:
-        ctx = device.load(dev)
-    elif ctx.ordinal != dev:
-        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
-    if workspace is None:
+    ctx, handle = _context(q.get_device(), ctx)
+    if workspace is None and ctx is not None:
         workspace = ctx.attention_workspace()
-    elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
-        raise ValueError("the workspace must be a contiguous uint8 CUDA tensor")
-    rc = _attention_paged(ctx._h, qp, ldq, qhs, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, ps, ts, hs, tp, ldt, width, lp, B, H, kv, dim,
-                                     dim ** -0.5 if scale is None else scale, gp, ldg, ghs, out.data_ptr(), out.stride(0), workspace.data_ptr(),
-                                     workspace.numel())
-    if rc:
-        ctx.check(rc)
-    return out
+    r = (_lib.binding or _lib.load_binding()).attention_paged(handle, q, k_cache, v_cache, tables, lengths, gate, scale, out, workspace)
+    if r.__class__ is int:
+        ctx.check(r)
+    return r
 
 
 def attention_paged_workspace(head_dim: int) -> int:
     """Bytes of workspace that `attention_paged` needs, whatever the batch."""
-    from ._lib import load_library
-    return int(load_library().s1_attention_paged_workspace(int(head_dim)))
+    return int(_lib.load_library().s1_attention_paged_workspace(int(head_dim)))
 
 
 # ------------------------------------------------------------------------------------------------ the decoder's cache

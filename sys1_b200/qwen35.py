@@ -12,10 +12,10 @@ from typing import Optional
 
 import torch
 
-from . import device
+from . import _lib, device
 from . import norm as _norm
 from . import paged
-from ._lib import EPI_SWIGLU, packed
+from ._lib import EPI_SWIGLU
 from .linear import Linear, fused_linear
 
 
@@ -248,9 +248,6 @@ class LinearAttention:
                                            P(y), y.stride(0)))
 
 
-_delta_step = packed("s1_gated_delta_rule_step")
-
-
 def gated_delta_rule_step(mixed: torch.Tensor, conv_weight: torch.Tensor, positions: torch.Tensor, b: torch.Tensor, a: torch.Tensor,
                           dt_bias: torch.Tensor, neg_exp_a: torch.Tensor, z: torch.Tensor, norm_weight: torch.Tensor, eps: float,
                           conv_state: torch.Tensor, state: torch.Tensor, key_heads: int, state_index: Optional[torch.Tensor] = None,
@@ -260,62 +257,12 @@ def gated_delta_rule_step(mixed: torch.Tensor, conv_weight: torch.Tensor, positi
     positions int32 `[rows]`, dt_bias, neg_exp_a f32 `[value_heads]`. `conv_state` bf16 `[states, 4, C]` and `state` f32 `[states,
     value_heads, 128, 128]` are updated in place; row r has state `state_index[r]` (int32, -1: none, its output is zero; None: r).
     Returns `[rows, value_heads * 128]`."""
-    dev, shape, held, bf16, f32 = mixed.get_device(), mixed.shape, state.shape, torch.bfloat16, torch.float32
-    if len(shape) != 2 or len(held) != 4:
-        raise ValueError("mixed must be [rows, channels] and state [states, value_heads, 128, 128]")
-    rows, C_, states, Hv = shape[0], shape[-1], held[0], held[1]
-    inner, ldba = Hv * 128, b.stride(0)
-    if not (dev >= 0 and mixed.dtype is bf16 and shape == (rows, C_) and mixed.stride(1) == 1 and C_ == 2 * key_heads * 128 + inner
-            and b.dtype is bf16 and b.get_device() == dev and b.shape == (rows, Hv) and b.stride(1) == 1
-            and a.dtype is bf16 and a.get_device() == dev and a.shape == (rows, Hv) and a.stride(1) == 1 and (a.stride(0) == ldba or rows < 2)
-            and z.dtype is bf16 and z.get_device() == dev and z.shape == (rows, inner) and z.stride(1) == 1
-            and positions.dtype is torch.int32 and positions.get_device() == dev and positions.shape == (rows,) and positions.is_contiguous()
-            and (state_index is None or state_index.dtype is torch.int32 and state_index.get_device() == dev and state_index.shape == (rows,)
-                 and state_index.is_contiguous())
-            and conv_weight.dtype is bf16 and conv_weight.get_device() == dev and conv_weight.numel() == 4 * C_ and conv_weight.shape[0] == C_ and conv_weight.shape[-1] == 4
-            and conv_weight.is_contiguous()
-            and dt_bias.dtype is f32 and dt_bias.get_device() == dev and dt_bias.shape == (Hv,) and dt_bias.is_contiguous()
-            and neg_exp_a.dtype is f32 and neg_exp_a.get_device() == dev and neg_exp_a.shape == (Hv,) and neg_exp_a.is_contiguous()
-            and norm_weight.dtype is bf16 and norm_weight.get_device() == dev and norm_weight.shape == (128,) and norm_weight.is_contiguous()
-            and state.dtype is f32 and state.get_device() == dev and held == (states, Hv, 128, 128) and state.is_contiguous()
-            and conv_state.dtype is bf16 and conv_state.get_device() == dev and conv_state.shape == (states, 4, C_) and conv_state.is_contiguous()):
-        _refuse_step(dev, rows, C_, states, Hv, key_heads, dict(mixed=mixed, b=b, a=a, z=z, positions=positions, state_index=state_index,
-                                                                conv_weight=conv_weight, dt_bias=dt_bias, neg_exp_a=neg_exp_a,
-                                                                norm_weight=norm_weight, state=state, conv_state=conv_state))
-    if out is None:
-        out = mixed.new_empty((rows, inner))
-    elif out.dtype is not bf16 or out.get_device() != dev or out.shape != (rows, inner) or out.stride(1) != 1:
-        raise ValueError(f"out must be a bf16 CUDA tensor [{rows}, {inner}] with contiguous rows")
-    if rows == 0:
-        return out
-    if ctx is None:
-        ctx = device.load(dev)
-    elif ctx.ordinal != dev:
-        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
-    rc = _delta_step(
-        ctx._h, mixed.data_ptr(), mixed.stride(0), conv_weight.data_ptr(), positions.data_ptr(), b.data_ptr(), a.data_ptr(), ldba, dt_bias.data_ptr(),
-        neg_exp_a.data_ptr(), z.data_ptr(), z.stride(0), norm_weight.data_ptr(), eps, 0 if state_index is None else state_index.data_ptr(), states,
-        conv_state.data_ptr(), state.data_ptr(), rows, key_heads, Hv, out.data_ptr(), out.stride(0))
-    if rc:
-        ctx.check(rc)
-    return out
-
-
-def _refuse_step(dev, rows, C_, states, Hv, key_heads, given) -> None:
-    """Says which argument of `gated_delta_rule_step` is not what it has to be."""
-    if C_ != (2 * key_heads + Hv) * 128:
-        raise ValueError(f"mixed must have {(2 * key_heads + Hv) * 128} columns for {key_heads} key and {Hv} value heads, not {C_}")
-    wanted = dict(mixed=(rows, C_), b=(rows, Hv), a=(rows, Hv), z=(rows, Hv * 128), positions=(rows,), state_index=(rows,), conv_weight=(C_, 4),
-                  dt_bias=(Hv,), neg_exp_a=(Hv,), norm_weight=(128,), state=(states, Hv, 128, 128), conv_state=(states, 4, C_))
-    types = dict(positions=torch.int32, state_index=torch.int32, dt_bias=torch.float32, neg_exp_a=torch.float32, state=torch.float32)
-    for name, t in given.items():
-        rowwise = name in ("mixed", "b", "a", "z")
-        dtype = types.get(name, torch.bfloat16)
-        if t is not None and (dev < 0 or t.get_device() != dev or t.dtype != dtype or (tuple(t.shape) != wanted[name] and not (name == "conv_weight" and tuple(t.shape) == (C_, 1, 4)))
-                              or (t.stride(-1) != 1 if rowwise else not t.is_contiguous())):
-            raise ValueError(f"{name} must be a {'' if rowwise else 'contiguous '}{str(dtype)[6:]} CUDA tensor {list(wanted[name])}"
-                             f"{' with contiguous rows' if rowwise else ''} on the call's GPU (no CPU fallback)")
-    raise ValueError("b and a must have the same row stride (column ranges of one projection, or contiguous)")
+    ctx, handle = paged._context(mixed.get_device(), ctx)
+    r = (_lib.binding or _lib.load_binding()).gated_delta_rule_step(handle, mixed, conv_weight, positions, b, a, dt_bias, neg_exp_a, z, norm_weight, eps,
+                                                                    conv_state, state, key_heads, state_index, out)
+    if r.__class__ is int:
+        ctx.check(r)
+    return r
 
 
 class RopeParams:

@@ -65,24 +65,24 @@ def test_a_context_without_a_gpu_says_so(ordinal):
     assert str(e.value) == str(plain.value)
 
 
-def test_packed_calls():
-    """`s1_call` needs a context; the words of a call are its arguments, and the types agree with the header's order of calls."""
-    import re
-    from test_abi import HEADER
-    lib, text = _lib.load_library(), HEADER.read_text()
-    assert lib.s1_call(None, 0, b"", 0) == _lib.S1_EINVAL
-    numbers = {n.lower(): int(i) for n, i in re.findall(r"S1_CALL_([A-Z_]+) = (\d+)", text)}
-    assert numbers == {n[3:]: i for i, n in enumerate(_lib.PACKED)}
-    for name in _lib.PACKED:
-        declared = re.search(rf"int {name}\(([^)]*)\)", text).group(1).split(",")[1:]
-        kinds = ["d" if re.match(r"\s*float \w", d) else "q" for d in declared]
-        assert kinds == ["d" if t.__name__ == "c_float" else "q" for t in _lib.SIGNATURES[name][1][1:]], name
-        call = _lib.packed(name)
-        assert call(None, *([0] * len(declared))) == _lib.S1_EINVAL
-        with pytest.raises(Exception):
-            call(None, *([0] * (len(declared) - 1)))
-        with pytest.raises(Exception):
-            call(None, *(["0"] * len(declared)))
+def test_the_binding_refuses_what_is_no_argument():
+    """Before any of it is read: another number of arguments, things that are no tensors, no numbers, or integers that the C ABI would cut off."""
+    b = _lib.load_binding()
+    for call, n in ((b.block_tables, 10), (b.cache_write, 13), (b.attention_paged, 10), (b.gated_delta_rule_step, 16)):
+        for m in (0, n - 1, n + 1):
+            with pytest.raises(TypeError, match=f"{n} arguments"):
+                call(*[None] * m)
+        with pytest.raises(ValueError, match="must be a tensor"):
+            call(*[None] * n)
+    for page, error in ((1 << 32, ValueError), (1 << 70, OverflowError), (1.5, TypeError), (None, TypeError)):
+        with pytest.raises(error):
+            paged.block_tables(_i(2), _i(2, 4), _i(8), _i(1), page)
+    with pytest.raises(ValueError, match="max_tokens is needed"):
+        paged.block_tables(_i(2), _i(2, 4), _i(8), _i(1), 16, added=_i(2))
+    with pytest.raises(ValueError, match="must not be negative"):
+        paged.block_tables(_i(2), _i(2, 4), _i(8), _i(1), 16, max_tokens=-1)
+    with pytest.raises(ValueError, match="v must be a tensor"):
+        paged.cache_write(_b(3, 2, 64), [1], _b(4, 16, 2, 64), _b(4, 16, 2, 64), _i(3))
 
 
 def test_workspace_sizes():

@@ -781,15 +781,33 @@ def test_a_context_of_another_gpu_is_refused(ctx):
             call()
 
 
-def test_packed_calls_refuse_what_is_not_their_arguments(ctx):
-    call = ctx._lib.s1_call
-    for which, words, match in ((9, 3, "no call 9"), (0, 3, "16 argument words, not 3"), (2, 25, "26 argument words, not 25")):
-        with pytest.raises(_lib.S1Error, match=match):
-            ctx.check(call(ctx.handle, which, bytes(8 * words), words))
-    with pytest.raises(_lib.S1Error, match="null pointer"):
-        ctx.check(call(ctx.handle, 0, None, 16))
-    with pytest.raises(_lib.S1Error, match="beyond 32 bits"):
-        paged.block_tables(ints([3]), ints([[0]]), ints([0]), ints([1]), 2 ** 32 + 16)
-    with pytest.raises(_lib.S1Error, match="power of two"):
-        paged.block_tables(ints([3]), ints([[0]]), ints([0]), ints([1]), 24)
+def test_outputs_given_come_back(ctx):
+    """The tensors of the call themselves, on every path (no rows included); whole numbers of other types are numbers too."""
+    cached, left = ints([3, 15]), ints([4])
+    r = paged.block_tables(cached, ints([[0, 1], [2, 3]]), ints([4, 5, 6, 7]), left, np.int64(16), lengths=cached, free_count_out=left)
+    assert r.lengths is cached and r.free_count is left and cached.tolist() == [4, 16] and r.slots.tolist() == [3, 47]
+    assert r.cu_seqlens.tolist() == [0, 1, 2] and r.positions.tolist() == [3, 15]
+    q, kc, vc, tables, lengths, gate = _attention_case([20, 30], 4, 2, 64, 16, 1)
+    wide = torch.zeros(2, 304, dtype=torch.bfloat16, device=DEV)
+    for out in (wide[:, 8:264], wide[:0, 8:264]):
+        n = out.shape[0]
+        assert paged.attention_paged(q[:n], kc, vc, tables[:n], lengths[:n], out=out) is out
+    assert torch.equal(wide[:, 8:264], paged.attention_paged(q, kc, vc, tables, lengths)) and not wide[:, :8].any() and not wide[:, 264:].any()
+    c = _step_case(3, 2, 4, 8)
+    y = qwen35.gated_delta_rule_step(**dict(c, state=c["state"].clone(), conv_state=c["conv_state"].clone()))
+    out = torch.empty_like(y)
+    assert qwen35.gated_delta_rule_step(**c, out=out) is out and torch.equal(out, y)
+    with pytest.raises(ValueError, match="out must be"):
+        qwen35.gated_delta_rule_step(**c, out=out[:, :-8])
+    ctx.sync()
+
+
+@pytest.mark.parametrize("name,change", [("mixed", lambda t: t.float()), ("conv_weight", lambda t: t[:, :3]), ("positions", lambda t: t.long()), ("b", lambda t: t[:, :-1]),
+                                         ("a", lambda t: t.cpu()), ("dt_bias", lambda t: t.to(torch.bfloat16)), ("neg_exp_a", lambda t: t[:-1]),
+                                         ("z", lambda t: t[:, ::2]), ("norm_weight", lambda t: t[:64]), ("state", lambda t: t.to(torch.bfloat16)),
+                                         ("conv_state", lambda t: t[:, :3]), ("state_index", lambda t: t.repeat(2))])
+def test_delta_step_names_the_argument_it_refuses(ctx, name, change):
+    c = _step_case(3, 2, 4, 8)
+    with pytest.raises(ValueError, match="mixed must|columns" if name == "mixed" else f"{name} must be"):
+        qwen35.gated_delta_rule_step(**dict(c, **{name: change(c[name])}))
     ctx.sync()
