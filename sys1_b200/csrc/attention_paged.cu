@@ -20,7 +20,7 @@
 //    keys and head dimensions, which there are enough of, and the 8 columns the query heads of the group. tcgen05 would want 64 or
 //    128 rows of queries where there are 1 to 16; at the rate that HBM delivers keys, mma.sync is a fifth busy.
 // Measured: 62 contexts of 100 .. 8192 tokens, 24 query and 4 KV heads of 256: 168 us = 6.3 TB/s; one of 131071 tokens, 8 and 2 heads:
-// 49 us = 5.4 TB/s; 31 of 1 .. 2048 tokens: 20 us; one of 17: 7 us.
+// 49 us = 5.4 TB/s; 31 of 1 .. 2048 tokens: 20 us; one of 17: 6 us.
 // Scores, maxima, sums and outputs are f32; the probabilities are rounded to bf16 for the second product, as in s1_attention
 // (an error of 2^-9 of each weight, averaged over the keys), while their sum is that of the unrounded ones.
 #include <cuda_bf16.h>
@@ -659,10 +659,14 @@ int launch(s1_ctx* ctx, PagedParams p, int units) {
     }
     const int ctas = std::min({8 / W * ctx->sm_count, kMaxCtas, units});  // no more than the block tables could make units of
     S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D, NT, W>, static_cast<unsigned>(ctas), 1u, W * 32u, smem, p));
+    ctx->launches += 1;
+    // a span of one unit is never cut: block tables that hold no more than a unit leave nothing to join (one context of 17 tokens in a
+    // table of 32: 7.3 us with the second kernel, 6.3 without)
+    if (static_cast<long long>(p.table_width) << p.shift <= WarpPass<D, NT, W>::kUnit) return S1_OK;
     const bool many = static_cast<long long>(p.num_seqs) * p.spans_per_row >= ctas;
     S1_CUDA_OK(ctx, s1_launch_waiting(ctx, many ? s1_attention_paged_join_kernel<D, NT, 320> : s1_attention_paged_join_kernel<D, NT, 512>,
                                       static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(NT * kCols, p.group)), many ? 320u : 512u, 0, p));
-    ctx->launches += 2;
+    ctx->launches += 1;
     return S1_OK;
 }
 

@@ -302,6 +302,19 @@ def test_paged_attention_many_ragged_rows(ctx, rows, H, kv, dim, longest):
     _check_attention(got, q, kc, vc, tables, lens, gate)
 
 
+@pytest.mark.parametrize("rows,kv,page,longest", [(3, 2, 16, 112), (3, 2, 16, 128), (70, 3, 16, 112), (1, 1, 64, 64), (250, 2, 16, 48), (250, 2, 16, 64), (600, 1, 2, 62)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_paged_attention_of_tables_about_a_unit_wide(ctx, rows, kv, page, longest, dim):
+    """Block tables of just a unit (128 keys, 64 with many rows), whose spans are never cut, and of a page more."""
+    lens = [int(n) for n in np.random.RandomState(rows).randint(0, longest + 1, rows)]
+    lens[0] = longest
+    q, kc, vc, tables, lengths, gate = _attention_case(lens, 4 * kv, kv, dim, page, rows)
+    got = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate)
+    ctx.sync()
+    _check_attention(got, q, kc, vc, tables, lens, gate)
+    assert torch.equal(got, paged.attention_paged(q, kc, vc, torch.nn.functional.pad(tables, (0, 100)), lengths, gate=gate))
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_paged_attention_of_sharp_and_flat_scores(ctx, dim):
     lens = [700, 33]
