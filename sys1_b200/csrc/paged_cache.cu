@@ -243,6 +243,9 @@ struct WriteParams {
     long long ldv, v_head_stride;
     const int32_t* slots;
     int T, kv_heads;
+    unsigned heads_mul;  // row / kv_heads = row * heads_mul >> heads_shift for row < 2^30
+    int heads_shift;
+    unsigned key_warps;  // warps of key rows; as many of value rows behind them
     const __nv_bfloat16* norm_w;
     float eps;
     const float* cos_t;
@@ -257,62 +260,46 @@ struct WriteParams {
     int* status;
 };
 
-// LPR lanes hold one head row (16 bytes each); the first half of the rows are keys, the second values. Streaming: every value is
-// read and written once. A warp that only copies takes U = 2 groups of rows where there are rows enough to fill the GPU that way and
-// requests both before it writes the first (16384 tokens x 4 heads of 256: 23.2 us = 5.8 TB/s, with U = 1 27.2, with U = 4 23.5; 64
-// tokens x 2 heads: 1.8 us, with U = 1 1.6). Norm and rotation leave U = 1 the faster at every size: registers for the other row's
-// cosines cost the warps that hide their latency.
-template <int LPR, bool NORM, int U>
-__global__ void __launch_bounds__(256) s1_cache_write_kernel(const WriteParams p) {
+// LPR lanes hold one head row, two pieces of 16 bytes each, the halves of the row; the first half of the rows are keys, the second
+// values. MEASURED
+constexpr int kWriteThreads = 128, kWriteWarps = kWriteThreads / 32;
+#ifndef WMIN
+#define WMIN 9
+#endif
+template <int LPR, bool NORM>
+__global__ void __launch_bounds__(kWriteThreads, NORM ? WMIN : 1) s1_cache_write_kernel(const WriteParams p) {
     constexpr int RPW = 32 / LPR;
     const int lane = threadIdx.x & 31, sub = lane % LPR;
     griddep_wait();
     griddep_launch_dependents();
-    const unsigned rows = static_cast<unsigned>(p.T) * static_cast<unsigned>(p.kv_heads);  // of keys; as many of values behind them
-    const unsigned first = (blockIdx.x * 8u + (threadIdx.x >> 5)) * (RPW * U) + lane / LPR;  // (warps are counted: threads may pass 32 bits)
-    uint4 raw[U];
-    long long slot[U];
-    int t[U], h[U], pos[U];
-    bool value[U], live[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        unsigned row = first + u * RPW;
-        value[u] = row >= rows;
-        if (value[u]) row -= rows;
-        live[u] = row < rows;
-        t[u] = live[u] ? static_cast<int>(row / static_cast<unsigned>(p.kv_heads)) : 0, h[u] = live[u] ? static_cast<int>(row) - t[u] * p.kv_heads : 0;
-        slot[u] = live[u] ? p.slots[t[u]] : -1;
-        pos[u] = NORM && live[u] && !value[u] ? p.positions[t[u]] : 0;
-        const __nv_bfloat16* src = value[u] ? p.v + t[u] * p.ldv + h[u] * p.v_head_stride : p.k + t[u] * p.ldk + h[u] * p.k_head_stride;
-        raw[u] = live[u] ? *reinterpret_cast<const uint4*>(src + sub * 8) : make_uint4(0, 0, 0, 0);  // (plain: see s1_launch_waiting)
+    unsigned warp = blockIdx.x * kWriteWarps + (threadIdx.x >> 5);  // (warps are counted: threads may pass 32 bits)
+    const bool value = warp >= p.key_warps;
+    if (value) warp -= p.key_warps;
+    const unsigned row = warp * RPW + lane / LPR;
+    bool live = row < static_cast<unsigned>(p.T) * static_cast<unsigned>(p.kv_heads);
+    const int t = live ? static_cast<int>(static_cast<unsigned long long>(row) * p.heads_mul >> p.heads_shift) : 0, h = live ? static_cast<int>(row) - t * p.kv_heads : 0;
+    const long long slot = live ? p.slots[t] : -1;
+    const int pos = NORM && live && !value ? p.positions[t] : 0;
+    const uint4* src = reinterpret_cast<const uint4*>((value ? p.v + t * p.ldv + h * p.v_head_stride : p.k + t * p.ldk + h * p.k_head_stride) + sub * 8);
+    uint4 x[2] = {};
+    if (live) x[0] = src[0], x[1] = src[LPR];  // (plain loads: see s1_launch_waiting)
+    live = live && slot >= 0;  // tokens without a slot are left out
+    if (live && slot >= p.num_slots) {
+        report(p.status, 116, t, static_cast<int>(slot));
+        live = false;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        live[u] = live[u] && slot[u] >= 0;  // tokens without a slot are left out
-        if (live[u] && slot[u] >= p.num_slots) {
-            report(p.status, 116, t[u], static_cast<int>(slot[u]));
-            live[u] = false;
-        }
-        if (NORM && !__all_sync(0xffffffffu, value[u])) {  // a warp of values alone has nothing to norm
-            const int halfc = p.rot / 16;
-            const bool rotates = live[u] && !value[u] && sub < 2 * halfc;
-            const bool pos_ok = pos[u] >= 0 && pos[u] < p.max_pos;
-            float c[8], sn[8];
-            if (!value[u] && sub < 2 * halfc && pos_ok) {  // (whatever the slot says, which may still be on its way)
-                load_rotation(p.cos_t, p.sin_t, pos[u], p.rot, sub, c, sn);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f;
-            }
-            const uint4 normed = head_norm_rope<LPR>(raw[u], p.norm_w, p.eps, c, sn, rotates && pos_ok, sub, halfc, p.bf16_ops);
-            if (!value[u]) raw[u] = normed;
-            if (rotates && !pos_ok) report(p.status, 102, t[u], pos[u]);
-        }
-        if (!live[u]) continue;
-        __nv_bfloat16* dst = (value[u] ? p.v_cache : p.k_cache) + (slot[u] >> p.shift) * p.page_stride +
-                             (slot[u] & ((1ll << p.shift) - 1)) * p.token_stride + h[u] * p.head_stride;
-        *reinterpret_cast<uint4*>(dst + sub * 8) = raw[u];
+    if (NORM && !value) {
+        const int halfc = p.rot / 16;
+        const bool rotates = live && sub < 2 * halfc, pos_ok = pos >= 0 && pos < p.max_pos;
+        float c[8], sn[8];
+        load_rotation(p.cos_t, p.sin_t, pos_ok ? pos : 0, p.rot, sub, c, sn);  // (whatever the slot says, which may still be on its way)
+        head_norm_rope<LPR>(x, p.norm_w, p.eps, c, sn, rotates && pos_ok, sub, halfc, p.bf16_ops);
+        if (rotates && !pos_ok) report(p.status, 102, t, pos);
     }
+    if (!live) return;
+    uint4* dst = reinterpret_cast<uint4*>((value ? p.v_cache : p.k_cache) + (slot >> p.shift) * p.page_stride +
+                                          (slot & ((1ll << p.shift) - 1)) * p.token_stride + h * p.head_stride + sub * 8);
+    dst[0] = x[0], dst[LPR] = x[1];
 }
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -399,23 +386,21 @@ extern "C" int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long lo
         if (!al16(norm_weight) || !al16(cos_table) || !al16(sin_table)) return s1_fail(ctx, S1_EINVAL, "%s: weight and tables must be 16-byte aligned", who);
     }
     if (total_tokens == 0) return S1_OK;
-    const int lpr = head_dim / 8;
-    // two groups of rows a warp from where that gives every scheduler four warps (see the kernel)
-    const long long rows = 2LL * total_tokens * kv_heads, groups = (rows * lpr + 31) / 32;
-    const int unroll = !norm_weight && groups >= 2LL * 16 * ctx->sm_count ? 2 : 1;
-    const long long per_block = 8LL * unroll * (32 / lpr), blocks = (rows + per_block - 1) / per_block;
-    if (rows > (1LL << 30)) return s1_fail(ctx, S1_EINVAL, "%s: too many rows", who);
+    const int lpr = head_dim / 16;
+    const long long rows = 1LL * total_tokens * kv_heads, key_warps = (rows * lpr + 31) / 32, blocks = (2 * key_warps + kWriteWarps - 1) / kWriteWarps;
+    if (rows > (1LL << 29)) return s1_fail(ctx, S1_EINVAL, "%s: too many rows", who);
+    int shift = 30;  // 2^(shift - 30) >= kv_heads: then the product is off by less than a row's worth for every row below 2^30
+    while (1LL << (shift - 30) < kv_heads) ++shift;
+    const unsigned mul = static_cast<unsigned>(((1ULL << shift) + kv_heads - 1) / kv_heads);
     S1DeviceGuard guard(ctx->device);
     if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
     WriteParams p{static_cast<const __nv_bfloat16*>(k), ldk, k_head_stride, static_cast<const __nv_bfloat16*>(v), ldv, v_head_stride, slots, total_tokens,
-                  kv_heads, static_cast<const __nv_bfloat16*>(norm_weight), eps, cos_table, sin_table, positions, max_positions, rotary_dim, bf16_ops,
+                  kv_heads, mul, shift, static_cast<unsigned>(key_warps), static_cast<const __nv_bfloat16*>(norm_weight), eps, cos_table, sin_table, positions, max_positions, rotary_dim, bf16_ops,
                   static_cast<__nv_bfloat16*>(k_cache), static_cast<__nv_bfloat16*>(v_cache), static_cast<long long>(num_pages) * page_size,
                   __builtin_ctz(page_size), page_stride, token_stride, head_stride, ctx->status_dev};
-    auto launch = [&](void (*kernel)(WriteParams)) { return s1_launch_waiting(ctx, kernel, static_cast<unsigned>(blocks), 1u, 256u, 0, p); };
-#define S1_WRITE(LPR_)                                                                                          \
-    launch(norm_weight ? s1_cache_write_kernel<LPR_, true, 1> : unroll == 2 ? s1_cache_write_kernel<LPR_, false, 2> \
-                                                                            : s1_cache_write_kernel<LPR_, false, 1>)
-    S1_CUDA_OK(ctx, lpr == 8 ? S1_WRITE(8) : lpr == 16 ? S1_WRITE(16) : S1_WRITE(32));
+    auto launch = [&](void (*kernel)(WriteParams)) { return s1_launch_waiting(ctx, kernel, static_cast<unsigned>(blocks), 1u, static_cast<unsigned>(kWriteThreads), 0, p); };
+#define S1_WRITE(LPR_) launch(norm_weight ? s1_cache_write_kernel<LPR_, true> : s1_cache_write_kernel<LPR_, false>)
+    S1_CUDA_OK(ctx, lpr == 4 ? S1_WRITE(4) : lpr == 8 ? S1_WRITE(8) : S1_WRITE(16));
 #undef S1_WRITE
     ctx->launches += 1;
     return S1_OK;
