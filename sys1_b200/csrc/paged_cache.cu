@@ -245,7 +245,6 @@ struct WriteParams {
     int T, kv_heads;
     unsigned heads_mul;  // row / kv_heads = row * heads_mul >> heads_shift for row < 2^30
     int heads_shift;
-    unsigned key_warps;  // warps of key rows; as many of value rows behind them
     const __nv_bfloat16* norm_w;
     float eps;
     const float* cos_t;
@@ -260,46 +259,59 @@ struct WriteParams {
     int* status;
 };
 
-// LPR lanes hold one head row, two pieces of 16 bytes each, the halves of the row; the first half of the rows are keys, the second
-// values. MEASURED
 constexpr int kWriteThreads = 128, kWriteWarps = kWriteThreads / 32;
-#ifndef WMIN
-#define WMIN 9
-#endif
+
+// LPR lanes hold one head row, two pieces of 16 bytes each, the halves of the row. Streaming: every value is read and written once.
+// Where keys are only copied, a warp takes keys or values (every other warp): short, with two loads a lane on the way (16384 tokens x 4
+// heads of 256: 21.4 us = 6.3 TB/s; 1330 tokens x 8 heads 3.3; with keys and values of a row in one lane 21.4 and 4.0, with one piece a
+// lane and 32 lanes a row 27 and 4.0). With the norm, which costs 250 instructions a row and warp, a lane takes a row's key and value:
+// the value's way and the indices come free under the arithmetic (7799 tokens x 4 heads of 256, 32 rotated: 12.0 us = 5.1 TB/s; keys and
+// values in warps of their own 15.4, and 22.6 with 32 lanes a row, whose exchanges and square roots serve half as many columns).
 template <int LPR, bool NORM>
-__global__ void __launch_bounds__(kWriteThreads, NORM ? WMIN : 1) s1_cache_write_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, NORM ? 9 : 1) s1_cache_write_kernel(const WriteParams p) {
     constexpr int RPW = 32 / LPR;
     const int lane = threadIdx.x & 31, sub = lane % LPR;
     griddep_wait();
     griddep_launch_dependents();
     unsigned warp = blockIdx.x * kWriteWarps + (threadIdx.x >> 5);  // (warps are counted: threads may pass 32 bits)
-    const bool value = warp >= p.key_warps;
-    if (value) warp -= p.key_warps;
+    const bool keys = NORM || (warp & 1u) == 0, values = NORM || !keys;
+    if (!NORM) warp >>= 1;
     const unsigned row = warp * RPW + lane / LPR;
     bool live = row < static_cast<unsigned>(p.T) * static_cast<unsigned>(p.kv_heads);
     const int t = live ? static_cast<int>(static_cast<unsigned long long>(row) * p.heads_mul >> p.heads_shift) : 0, h = live ? static_cast<int>(row) - t * p.kv_heads : 0;
     const long long slot = live ? p.slots[t] : -1;
-    const int pos = NORM && live && !value ? p.positions[t] : 0;
-    const uint4* src = reinterpret_cast<const uint4*>((value ? p.v + t * p.ldv + h * p.v_head_stride : p.k + t * p.ldk + h * p.k_head_stride) + sub * 8);
-    uint4 x[2] = {};
-    if (live) x[0] = src[0], x[1] = src[LPR];  // (plain loads: see s1_launch_waiting)
+    const int pos = NORM && live ? p.positions[t] : 0;
+    uint4 k[2] = {}, v[2] = {};
+    if (live && keys) {  // (plain loads: see s1_launch_waiting)
+        const uint4* src = reinterpret_cast<const uint4*>(p.k + t * p.ldk + h * p.k_head_stride + sub * 8);
+        k[0] = src[0], k[1] = src[LPR];
+    }
+    if (live && values) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.v + t * p.ldv + h * p.v_head_stride + sub * 8);
+        v[0] = src[0], v[1] = src[LPR];
+    }
     live = live && slot >= 0;  // tokens without a slot are left out
     if (live && slot >= p.num_slots) {
         report(p.status, 116, t, static_cast<int>(slot));
         live = false;
     }
-    if (NORM && !value) {
+    const long long at = (slot >> p.shift) * p.page_stride + (slot & ((1ll << p.shift) - 1)) * p.token_stride + h * p.head_stride + sub * 8;
+    if (live && values) {
+        uint4* dst = reinterpret_cast<uint4*>(p.v_cache + at);
+        dst[0] = v[0], dst[LPR] = v[1];
+    }
+    if (NORM) {
         const int halfc = p.rot / 16;
         const bool rotates = live && sub < 2 * halfc, pos_ok = pos >= 0 && pos < p.max_pos;
         float c[8], sn[8];
         load_rotation(p.cos_t, p.sin_t, pos_ok ? pos : 0, p.rot, sub, c, sn);  // (whatever the slot says, which may still be on its way)
-        head_norm_rope<LPR>(x, p.norm_w, p.eps, c, sn, rotates && pos_ok, sub, halfc, p.bf16_ops);
+        head_norm_rope<LPR>(k, p.norm_w, p.eps, c, sn, rotates && pos_ok, sub, halfc, p.bf16_ops);
         if (rotates && !pos_ok) report(p.status, 102, t, pos);
     }
-    if (!live) return;
-    uint4* dst = reinterpret_cast<uint4*>((value ? p.v_cache : p.k_cache) + (slot >> p.shift) * p.page_stride +
-                                          (slot & ((1ll << p.shift) - 1)) * p.token_stride + h * p.head_stride + sub * 8);
-    dst[0] = x[0], dst[LPR] = x[1];
+    if (live && keys) {
+        uint4* dst = reinterpret_cast<uint4*>(p.k_cache + at);
+        dst[0] = k[0], dst[LPR] = k[1];
+    }
 }
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -387,7 +399,7 @@ extern "C" int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long lo
     }
     if (total_tokens == 0) return S1_OK;
     const int lpr = head_dim / 16;
-    const long long rows = 1LL * total_tokens * kv_heads, key_warps = (rows * lpr + 31) / 32, blocks = (2 * key_warps + kWriteWarps - 1) / kWriteWarps;
+    const long long rows = 1LL * total_tokens * kv_heads, warps = (rows * lpr + 31) / 32 * (norm_weight ? 1 : 2), blocks = (warps + kWriteWarps - 1) / kWriteWarps;
     if (rows > (1LL << 29)) return s1_fail(ctx, S1_EINVAL, "%s: too many rows", who);
     int shift = 30;  // 2^(shift - 30) >= kv_heads: then the product is off by less than a row's worth for every row below 2^30
     while (1LL << (shift - 30) < kv_heads) ++shift;
@@ -395,7 +407,7 @@ extern "C" int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long lo
     S1DeviceGuard guard(ctx->device);
     if (!guard.ok) return s1_fail(ctx, S1_ECUDA, "%s: cudaSetDevice(%d) failed", who, ctx->device);
     WriteParams p{static_cast<const __nv_bfloat16*>(k), ldk, k_head_stride, static_cast<const __nv_bfloat16*>(v), ldv, v_head_stride, slots, total_tokens,
-                  kv_heads, mul, shift, static_cast<unsigned>(key_warps), static_cast<const __nv_bfloat16*>(norm_weight), eps, cos_table, sin_table, positions, max_positions, rotary_dim, bf16_ops,
+                  kv_heads, mul, shift, static_cast<const __nv_bfloat16*>(norm_weight), eps, cos_table, sin_table, positions, max_positions, rotary_dim, bf16_ops,
                   static_cast<__nv_bfloat16*>(k_cache), static_cast<__nv_bfloat16*>(v_cache), static_cast<long long>(num_pages) * page_size,
                   __builtin_ctz(page_size), page_stride, token_stride, head_stride, ctx->status_dev};
     auto launch = [&](void (*kernel)(WriteParams)) { return s1_launch_waiting(ctx, kernel, static_cast<unsigned>(blocks), 1u, static_cast<unsigned>(kWriteThreads), 0, p); };

@@ -198,8 +198,8 @@ def test_cache_write(ctx, T, kv, dim, rot, page, layout, normed):
             assert bool((err <= (2.0 ** -8 + 2.0 ** -14) * (size + ref.abs())).all())
 
 
-def test_cache_write_of_more_threads_than_32_bits(ctx):
-    """2^27 + 16 head rows of 32 lanes each: the last tokens' values are written by the last blocks."""
+def test_cache_write_of_a_batch_beyond_32_bits(ctx):
+    """2^26 + 8 tokens, whose last rows lie 2^34 elements behind the first."""
     T, dim, g = 2 ** 26 + 8, 256, gen(19)
     x = torch.empty(T, 1, dim, dtype=torch.bfloat16, device=DEV)  # 34 GB, keys and values in one; only the last rows are copied
     x[-3:] = bf(g, 3, 1, dim)
