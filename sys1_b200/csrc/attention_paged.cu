@@ -13,14 +13,14 @@
 //    partial results (maximum, sum, unnormalised output in f32) in the workspace, at most two per CTA; and a second
 //    kernel joins them, in the order of the units: results do not depend on timing. (Joined by the CTA that finds all pieces of a
 //    span there, without the second kernel, the pieces were one CTA's work: 32 contexts up to 2048 took 27 us instead of 21.)
-//  * inside a CTA the warps take tiles of 16 keys in turn, each through a ring of its own in shared memory (cp.async, 24 KB a warp,
-//    192 KB an SM in flight or in use): no warp waits for another until its span is done. The next span's first keys are fetched into
+//  * inside a CTA the warps take tiles of 16 keys in turn, each through a ring of its own in shared memory (cp.async, 192 KB an SM in
+//    flight or in use): no warp waits for another until its span is done. The next span's first keys are fetched into
 //    L2 and its queries into registers while the warps' results are put together.
 //  * the products run on mma.sync m16n8k16 with the operands turned round - S^T = K Q^T, O^T = V^T P^T - so that the 16 rows are
 //    keys and head dimensions, which there are enough of, and the 8 columns the query heads of the group. tcgen05 would want 64 or
 //    128 rows of queries where there are 1 to 16; at the rate that HBM delivers keys, mma.sync is a fifth busy.
 // Measured: 62 contexts of 100 .. 8192 tokens, 24 query and 4 KV heads of 256: 168 us = 6.3 TB/s; one of 131071 tokens, 8 and 2 heads:
-// 49 us = 5.4 TB/s; 31 of 1 .. 2048 tokens: 20 us; one of 17: 6 us.
+// 49 us = 5.4 TB/s; 31 of 1 .. 2048 tokens: 19.6 us; one of 17: 6 us.
 // Scores, maxima, sums and outputs are f32; the probabilities are rounded to bf16 for the second product, as in s1_attention
 // (an error of 2^-9 of each weight, averaged over the keys), while their sum is that of the unrounded ones.
 #include <cuda_bf16.h>
@@ -40,11 +40,14 @@ namespace {
 
 constexpr int kTile = 16;               // keys of one warp step
 constexpr int kCols = 8;                // query heads of one MMA (its columns); a span has NT times as many
-constexpr int kRingBytes = 24 * 1024;   // per warp
+constexpr int kRings = 192 * 1024;      // bytes of an SM's warps' rings
 
 // What a span costs beyond its units (its queries, the first keys' way, the warps' results put together), in units of its head dim.
 template <int D>
 constexpr int kStart = 256 / D;
+
+// CTAs of the first kernel at most: two, three or four per SM of any sm_100 part
+constexpr int max_ctas(int head_dim) { return head_dim == 256 ? 320 : head_dim == 128 ? 480 : 640; }
 
 struct PagedParams {
     const __nv_bfloat16* q;
@@ -65,7 +68,8 @@ struct PagedParams {
     long long ldo;
     float* parts;   // [2 * grid][heads of a span][D]: unnormalised outputs of the cut spans' pieces
     float2* marks;  // [2 * grid][heads of a span]: maximum (in units of log2) and sum of the same pieces
-    int4* records;  // [grid]: row, span of the row, last CTA of the span that begins in this CTA and is cut (or -1)
+    int4* records;  // row, span of the row, last (-1: not cut) and first CTA of a span: by_span one for each span, else one for each CTA, of the
+    bool by_span;   // span that begins in it and is cut
     int* status;
 };
 
@@ -126,11 +130,12 @@ __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefe
 // One warp's pass over its tiles of a span: keys first, first + 16 W, ..., 16 to a tile, below `end`. NT = 1: up to 8 query heads, held in registers;
 // NT = 2: up to 16, read from shared memory step by step, so that a group of more than 8 does not read its keys twice (32 x 8192
 // tokens, 16 heads to a KV head of 256: 166 us as two spans of 8, 98 as one of 16).
-template <int D, int NT, int W>
+template <int D, int NT, int W, int P>
 struct WarpPass {
     static constexpr int kUnit = W * kTile;                 // keys of one unit: a tile for each of the CTA's W warps
     static constexpr int kSlotBytes = kTile * D * 2;
-    static constexpr int kSlots = kRingBytes / kSlotBytes;  // 3, 6 or 12
+    static constexpr int kSlots = kRings / (W * P * kSlotBytes);
+    static constexpr int kRingBytes = kSlots * kSlotBytes;
     static constexpr int kChunks = D / 8;                   // 16-byte pieces of a key
     static constexpr int kRowsPerCopy = 32 / kChunks;
     static constexpr int kSteps = D / 16;
@@ -357,12 +362,15 @@ struct Segment {     // the part of one span that lies in the range
     int end;             // keys u0 * kUnit .. end - 1
 };
 
-// W = 8: one CTA per SM. W = 4: two, with half the warps and rings each - where there are many spans, one's keys come while the
-// other puts its results together (512 contexts of 100 tokens 40 us with W = 8, 35 with 4; of 17 tokens 35 and 24); with few and
-// long ones the larger units stream a little faster (64 contexts up to 8192 tokens 168 and 172 us).
-template <int D, int NT, int W>
-__global__ void __launch_bounds__(W * 32, 8 / W) s1_attention_paged_kernel(const PagedParams p) {
-    using Pass = WarpPass<D, NT, W>;
+// P CTAs of W warps per SM. W = 8 and as many CTAs as the registers allow, one at a head dim of 256 and two below (head dim 128, 28 contexts
+// of up to 61259 tokens, 4 heads on 2: 161 us, with one 163; head dim 64, 4 of 66164, 64 on 4: 37 and 44) but one at head dim 128 with NT
+// = 2, which would spill (94 of 3443, 64 on 4: 92 us, with two 114). Where there are many spans, W = 4: one's keys come while another puts
+// its results together (head dim 256: 512 contexts of 100 tokens 40 us with W = 8, 35 with 4; with few and long ones the larger units
+// stream a little faster, 64 contexts up to 8192 tokens 168 and 172 us), and with NT = 1 three CTAs at head dim 128 (512 of 100 tokens 20 us,
+// with two 23) and four at 64 (700 of up to 900 tokens 37 us, with two 45; long contexts lose, 128 of 2000 tokens 83 us and 75).
+template <int D, int NT, int W, int P>
+__global__ void __launch_bounds__(W * 32, P) s1_attention_paged_kernel(const PagedParams p) {
+    using Pass = WarpPass<D, NT, W, P>;
     constexpr int kHeads = NT * kCols, kWarps = W, kThreads = W * 32, kUnit = Pass::kUnit;
     extern __shared__ __align__(128) uint8_t ring_smem[];
     float* stage = reinterpret_cast<float*>(ring_smem);  // [warp][head][D + 4], after the rings have been read
@@ -381,8 +389,11 @@ __global__ void __launch_bounds__(W * 32, 8 / W) s1_attention_paged_kernel(const
 
     // ---- rows without a key: zeros
     for (int b = cta * kWarps + warp; b < p.num_seqs; b += ctas * kWarps)
-        if (row_length(p, b, lane == 0) == 0)
+        if (row_length(p, b, lane == 0) == 0) {
+            if (p.by_span)
+                for (int i = lane; i < p.spans_per_row; i += 32) p.records[b * p.spans_per_row + i] = make_int4(0, 0, -1, 0);
             for (int i = lane * 8; i < p.heads * D; i += 256) *reinterpret_cast<uint4*>(p.out + b * p.ldo + i) = make_uint4(0, 0, 0, 0);
+        }
 
     // ---- this CTA's range (the host has seen to it that all costs together fit 31 bits)
     auto cost_of = [&](int b) {
@@ -409,7 +420,7 @@ __global__ void __launch_bounds__(W * 32, 8 / W) s1_attention_paged_kernel(const
     }
     const int workers = min(ctas, total);
     if (cta >= workers) {
-        if (tid == 0) p.records[cta] = make_int4(0, 0, -1, 0);
+        if (tid == 0 && !p.by_span) p.records[cta] = make_int4(0, 0, -1, 0);
         return;
     }
     const int share = total / workers, longer = total - share * workers;  // the first `longer` CTAs have one more
@@ -447,7 +458,7 @@ __global__ void __launch_bounds__(W * 32, 8 / W) s1_attention_paged_kernel(const
         return false;
     };
     int4 record = make_int4(0, 0, -1, 0);
-    Pass pass(p, lane, smem_u32(ring_smem) + warp * kRingBytes, masks[warp]);
+    Pass pass(p, lane, smem_u32(ring_smem) + warp * Pass::kRingBytes, masks[warp]);
 
     // the queries of a span: 16 bytes a thread and turn, fetched a span ahead (rows past the group's last head repeat it and are not
     // written out)
@@ -572,30 +583,32 @@ __global__ void __launch_bounds__(W * 32, 8 / W) s1_attention_paged_kernel(const
             if (tid < nh) p.marks[piece * kHeads + tid] = marks_all[tid];
             if (now.u0 == 0) {  // a span that begins here and is cut at the end of this CTA's range: the CTA that has its last unit
                 const int end = stop - now.n + now.units - 1, border = longer * (share + 1);
-                record = make_int4(now.b, now.kvh * p.blocks_per_group + now.hb, end < border ? end / (share + 1) : longer + (end - border) / share, 0);
+                record = make_int4(now.b, now.kvh * p.blocks_per_group + now.hb, end < border ? end / (share + 1) : longer + (end - border) / share, cta);
             }
         }
+        if (p.by_span && now.u0 == 0 && tid == 0) p.records[now.b * p.spans_per_row + now.kvh * p.blocks_per_group + now.hb] = record;
         hand_q(next_q);
         __syncthreads();  // the stage is a ring again
         now = next;
         if (more) pass.start(now.b, now.kvh, now.u0 * kUnit + warp * kTile, now.end);
     }
-    if (tid == 0) p.records[cta] = record;
+    if (tid == 0 && !p.by_span) p.records[cta] = record;
 }
 
-// Joins the pieces of the span that began in CTA blockIdx.x of the first kernel and went on in the CTAs after it, for one of its
-// heads (blockIdx.y). There may be over a hundred pieces when one context is alone: a thread looks at one mark each, and the warps
-// share the pieces, so that the block waits for the record, the marks and the pieces once each. THREADS: 512 where there are fewer spans
-// than CTAs and so many pieces to a span (one context of 131071 tokens 49 us, with 256 threads 53), else 320 (64 contexts up to 8192
-// tokens 168 us, with 512 threads 170).
+// Joins the pieces of a span (that of record blockIdx.x) that began in one CTA of the first kernel and went on in the CTAs after it, for
+// one of its heads (blockIdx.y). There may be over a hundred pieces when one context is alone: a thread looks at a mark, and the warps
+// share the pieces, so that the block waits for the record, the marks and the pieces once each. THREADS: 512 where a span has more than
+// four pieces (one context of 131071 tokens 49 us, with 256 threads 53), else as many as the head has dimensions (128 at least), since the
+// blocks themselves are the cost (300 contexts, 32 heads on 2 of 64: 30 us, with 640 threads 41), and the next kernel's blocks are let in
+// when the pieces have come (128 contexts of 2000 tokens, 32 heads on 8 of 128: 121 us, let in at once 143).
 template <int D, int NT, int THREADS>
 __global__ void __launch_bounds__(THREADS) s1_attention_paged_join_kernel(const PagedParams p) {
     constexpr int kHeads = NT * kCols, kVec = D / 32, kJoinWarps = THREADS / 32;
     __shared__ float sums[kJoinWarps][D];
-    __shared__ float weights[THREADS];
+    __shared__ float weights[max_ctas(D)];
     __shared__ float tops[kJoinWarps], totals[kJoinWarps];
     griddep_wait();
-    griddep_launch_dependents();
+    if (THREADS == 512) griddep_launch_dependents();
     const int4 rec = p.records[blockIdx.x];
     if (rec.z < 0) return;
     const int h = blockIdx.y, kvh = rec.y / p.blocks_per_group, hb = rec.y % p.blocks_per_group;
@@ -604,19 +617,24 @@ __global__ void __launch_bounds__(THREADS) s1_attention_paged_join_kernel(const 
     const int head = kvh * p.group + hb * kHeads + h;
     float gate = 0.f;
     if (p.gate && tid < D) gate = __bfloat162float(p.gate[rec.x * p.ldg + head * p.gate_head_stride + tid]);
-    const int first = blockIdx.x, pieces = rec.z - first + 1;  // piece i: of CTA first + i, its second (i = 0) or its first
+    const int first = rec.w, pieces = rec.z - first + 1;  // piece i: of CTA first + i, its second (i = 0) or its first
     auto place = [&](int i) { return (2 * (first + i) + (i == 0 ? 1 : 0)) * kHeads + h; };
     const float2 mark = tid < pieces ? p.marks[place(tid)] : make_float2(-INFINITY, 0.f);
     float top = mark.x;
+    for (int i = tid + THREADS; i < pieces; i += THREADS) top = fmaxf(top, p.marks[place(i)].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) tops[warp] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
-    const float weight = mark.x == -INFINITY ? 0.f : exp2_fast(mark.x - top);
-    weights[tid] = weight;
-    float sum = mark.y * weight;
+    float sum = 0.f;
+    auto weigh = [&](int i, const float2& m) {
+        weights[i] = m.x == -INFINITY ? 0.f : exp2_fast(m.x - top);
+        sum += m.y * weights[i];
+    };
+    if (tid < pieces) weigh(tid, mark);
+    for (int i = tid + THREADS; i < pieces; i += THREADS) weigh(i, p.marks[place(i)]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) totals[warp] = sum;
@@ -631,6 +649,7 @@ __global__ void __launch_bounds__(THREADS) s1_attention_paged_join_kernel(const 
     }
 #pragma unroll
     for (int e = 0; e < kVec; ++e) sums[warp][lane + 32 * e] = x[e];
+    if (THREADS != 512) griddep_launch_dependents();
     __syncthreads();
     if (tid < D) {
         float y = 0.f, total = 0.f;
@@ -642,30 +661,34 @@ __global__ void __launch_bounds__(THREADS) s1_attention_paged_join_kernel(const 
     }
 }
 
-constexpr int kMaxCtas = 320;  // the workspace's share: two CTAs per SM of any sm_100 part
-static_assert(kMaxCtas <= 320, "the join looks at one piece a thread");
 
 size_t workspace_bytes_of(int head_dim) {
-    return sizeof(int4) * kMaxCtas + 2 * kMaxCtas * 2 * kCols * (sizeof(float2) + sizeof(float) * static_cast<size_t>(head_dim));
+    return sizeof(int4) * max_ctas(head_dim) + 2 * max_ctas(head_dim) * 2 * kCols * (sizeof(float2) + sizeof(float) * static_cast<size_t>(head_dim));
 }
 
-template <int D, int NT, int W>
+template <int D, int NT, int W, int P>
 int launch(s1_ctx* ctx, PagedParams p, int units) {
-    constexpr int smem = W * kRingBytes;
+    constexpr int smem = W * WarpPass<D, NT, W, P>::kRingBytes;
     static std::atomic<unsigned long long> told{0};  // one bit per device
     if (!(told.load(std::memory_order_relaxed) >> (ctx->device & 63) & 1)) {
-        S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        S1_CUDA_OK(ctx, cudaFuncSetAttribute(s1_attention_paged_kernel<D, NT, W, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         told.fetch_or(1ull << (ctx->device & 63), std::memory_order_relaxed);
     }
-    const int ctas = std::min({8 / W * ctx->sm_count, kMaxCtas, units});  // no more than the block tables could make units of
-    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D, NT, W>, static_cast<unsigned>(ctas), 1u, W * 32u, smem, p));
+    const int ctas = std::min({P * ctx->sm_count, max_ctas(D), units});  // no more than the block tables could make units of
+    const long long spans = static_cast<long long>(p.num_seqs) * p.spans_per_row;
+    // sixteen blocks of the join to every record: fewer records where there are fewer spans than CTAs (4 contexts of 66164 tokens, 64 heads on 4
+    // of 64: 44 us, by CTA 46; with up to 8 heads the few blocks would crowd on a few SMs, one of 131071 51 us and 49)
+    p.by_span = NT == 2 && spans <= ctas;
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D, NT, W, P>, static_cast<unsigned>(ctas), 1u, W * 32u, smem, p));
     ctx->launches += 1;
     // a span of one unit is never cut: block tables that hold no more than a unit leave nothing to join (one context of 17 tokens in a
     // table of 32: 7.3 us with the second kernel, 6.3 without)
-    if (static_cast<long long>(p.table_width) << p.shift <= WarpPass<D, NT, W>::kUnit) return S1_OK;
-    const bool many = static_cast<long long>(p.num_seqs) * p.spans_per_row >= ctas;
-    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, many ? s1_attention_paged_join_kernel<D, NT, 320> : s1_attention_paged_join_kernel<D, NT, 512>,
-                                      static_cast<unsigned>(ctas), static_cast<unsigned>(std::min(NT * kCols, p.group)), many ? 320u : 512u, 0, p));
+    if (static_cast<long long>(p.table_width) << p.shift <= WarpPass<D, NT, W, P>::kUnit) return S1_OK;
+    constexpr int kThreads = D == 256 ? 256 : 128;
+    const bool many = 4 * spans >= ctas;  // four pieces to a span at most, were all spans alike
+    S1_CUDA_OK(ctx, s1_launch_waiting(ctx, many ? s1_attention_paged_join_kernel<D, NT, kThreads> : s1_attention_paged_join_kernel<D, NT, 512>,
+                                      static_cast<unsigned>(p.by_span ? spans : ctas), static_cast<unsigned>(std::min(NT * kCols, p.group)),
+                                      many ? kThreads : 512u, 0, p));
     ctx->launches += 1;
     return S1_OK;
 }
@@ -673,8 +696,8 @@ int launch(s1_ctx* ctx, PagedParams p, int units) {
 template <int D>
 int launch(s1_ctx* ctx, const PagedParams& p, int units) {
     const bool wide = p.group > kCols, many = static_cast<long long>(p.num_seqs) * p.spans_per_row >= 3ll * ctx->sm_count;
-    if (wide) return many ? launch<D, 2, 4>(ctx, p, units) : launch<D, 2, 8>(ctx, p, units);
-    return many ? launch<D, 1, 4>(ctx, p, units) : launch<D, 1, 8>(ctx, p, units);
+    if (wide) return many ? launch<D, 2, 4, 2>(ctx, p, units) : launch<D, 2, 8, D == 64 ? 2 : 1>(ctx, p, units);
+    return many ? launch<D, 1, 4, D == 256 ? 2 : D == 128 ? 3 : 4>(ctx, p, units) : launch<D, 1, 8, D == 256 ? 1 : 2>(ctx, p, units);
 }
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -718,12 +741,12 @@ extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, lon
     // the costs of all spans, with the smaller units, have to fit 31 bits
     const long long spans = static_cast<long long>(num_seqs) * kv_heads * blocks, cost = static_cast<long long>(table_width) * page_size / (4 * kTile) + 5;
     if (spans > (1ll << 31) / cost - 1) return s1_fail(ctx, S1_EINVAL, "%s: rows x KV heads x (tokens of a block table) / 64 must be below 2^31", who);
-    float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * kMaxCtas);
+    float2* marks = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + sizeof(int4) * max_ctas(head_dim));
     PagedParams p{static_cast<const __nv_bfloat16*>(q), ldq, q_head_stride, static_cast<const __nv_bfloat16*>(k_cache),
                   static_cast<const __nv_bfloat16*>(v_cache), page_stride, token_stride, head_stride, num_pages, __builtin_ctz(page_size), tables, ldt,
                   table_width, lengths, num_seqs, heads, kv_heads, group, kv_heads * blocks, blocks, scale * 1.4426950408889634f,
                   static_cast<const __nv_bfloat16*>(gate), ldg, gate_head_stride, static_cast<__nv_bfloat16*>(out), ldo,
-                  reinterpret_cast<float*>(marks + 2 * kMaxCtas * 2 * kCols), marks, static_cast<int4*>(workspace), ctx->status_dev};
+                  reinterpret_cast<float*>(marks + 2 * max_ctas(head_dim) * 2 * kCols), marks, static_cast<int4*>(workspace), false, ctx->status_dev};
     const int units = static_cast<int>(std::min(spans * cost, 1ll << 30));
     return head_dim == 64 ? launch<64>(ctx, p, units) : head_dim == 128 ? launch<128>(ctx, p, units) : launch<256>(ctx, p, units);
 }

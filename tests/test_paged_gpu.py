@@ -302,6 +302,18 @@ def test_paged_attention_many_ragged_rows(ctx, rows, H, kv, dim, longest):
     _check_attention(got, q, kc, vc, tables, lens, gate)
 
 
+@pytest.mark.parametrize("rows,H,kv,dim,longest", [(200, 6, 3, 64, 200000), (230, 6, 2, 128, 150000), (100, 32, 2, 64, 100000), (3, 16, 1, 128, 90000), (250, 2, 2, 256, 60000)])
+def test_paged_attention_of_one_long_context_among_many(ctx, rows, H, kv, dim, longest):
+    """More pieces of one span than the join's threads, or than its warps, among spans that are never cut; few spans of many heads."""
+    lens = [int(n) for n in np.random.RandomState(9).randint(0, 60, rows)]
+    lens[rows // 2] = longest
+    q, kc, vc, tables, lengths, gate = _attention_case(lens, H, kv, dim, 64, 9)
+    got = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate)
+    ctx.sync()
+    _check_attention(got, q, kc, vc, tables, lens, gate)
+    assert torch.equal(got, paged.attention_paged(q, kc, vc, tables, lengths, gate=gate))
+
+
 @pytest.mark.parametrize("rows,kv,page,longest", [(3, 2, 16, 112), (3, 2, 16, 128), (70, 3, 16, 112), (1, 1, 64, 64), (250, 2, 16, 48), (250, 2, 16, 64), (600, 1, 2, 62)])
 @pytest.mark.parametrize("dim", [64, 256])
 def test_paged_attention_of_tables_about_a_unit_wide(ctx, rows, kv, page, longest, dim):
