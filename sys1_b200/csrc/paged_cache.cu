@@ -263,12 +263,13 @@ constexpr int kWriteThreads = 128, kWriteWarps = kWriteThreads / 32;
 
 // LPR lanes hold one head row, two pieces of 16 bytes each, the halves of the row. Streaming: every value is read and written once.
 // Where keys are only copied, a warp takes keys or values (every other warp): short, with two loads a lane on the way (16384 tokens x 4
-// heads of 256: 21.4 us = 6.3 TB/s; 1330 tokens x 8 heads 3.3; with keys and values of a row in one lane 21.4 and 4.0, with one piece a
-// lane and 32 lanes a row 27 and 4.0). With the norm, which costs 250 instructions a row and warp, a lane takes a row's key and value:
-// the value's way and the indices come free under the arithmetic (7799 tokens x 4 heads of 256, 32 rotated: 12.0 us = 5.1 TB/s; keys and
-// values in warps of their own 15.4, and 22.6 with 32 lanes a row, whose exchanges and square roots serve half as many columns).
+// heads of 256: 21.2 us = 6.3 TB/s, 1918 x 8 4.6; with 46 registers instead of 32 a thread 21.5 and 5.0, with keys and values of a row in
+// one lane 21.4 and 4.8, with one piece a lane and 32 lanes a row 27 and 5.5). With the norm, which costs 250 instructions a row and warp,
+// a lane takes a row's key and value: the value's way and the indices come free under the arithmetic (7799 tokens x 4 heads of 256, 32
+// rotated: 12.0 us = 5.1 TB/s; keys and values in warps of their own 15.4, and 22.6 with 32 lanes a row, whose exchanges and square roots
+// serve half as many columns).
 template <int LPR, bool NORM>
-__global__ void __launch_bounds__(kWriteThreads, NORM ? 9 : 1) s1_cache_write_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, NORM ? 9 : 16) s1_cache_write_kernel(const WriteParams p) {
     constexpr int RPW = 32 / LPR;
     const int lane = threadIdx.x & 31, sub = lane % LPR;
     griddep_wait();
