@@ -1,0 +1,44 @@
+"""Decoding from a cache where it is easy to be nearly right.
+
+A rounding to bf16 is off by at most 2^-8 of the value, and so is the output's. A softmax weight enters its product as two bf16 values, the
+first cut to eight bits and the rest rounded: 2^-15 of it. The f32 sums and exponentials stay below 2^-15 of the sums taken with |v|."""
+import pytest
+import torch
+
+from paged_model import attention_64
+from sys1_b200 import paged
+from test_paged_gpu import _attention_case
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ paged attention
+@pytest.mark.parametrize("lens,H,kv,dim,page", [([17], 8, 2, 256, 16), ([1, 2, 3, 700], 8, 2, 128, 16), ([40, 65, 0, 5], 6, 3, 64, 4), ([300, 33], 16, 1, 64, 16),
+                                                ([128, 2500], 32, 2, 256, 64), ([513], 9, 1, 128, 32), ([9 + i % 90 for i in range(450)], 4, 1, 256, 16),
+                                                ([1 + i % 70 for i in range(500)], 4, 2, 128, 16), ([3 + i % 50 for i in range(480)], 2, 2, 64, 8),
+                                                ([2 + i % 130 for i in range(450)], 16, 1, 256, 16), ([2 + i % 99 for i in range(450)], 12, 1, 128, 16),
+                                                ([2 + i % 99 for i in range(450)], 16, 1, 64, 16)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_paged_attention_keeps_its_weights(ctx, lens, H, kv, dim, page, gated):
+    q, kc, vc, tables, lengths, gate = _attention_case(lens, H, kv, dim, page, len(lens) + H, gated=gated)
+    got = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate)
+    ctx.sync()
+    ref, size = attention_64(q, kc, vc, tables, lens, gate, dim ** -0.5)
+    err = (got.double().unflatten(1, (-1, dim)) - ref).abs()
+    assert bool((err <= 2.0 ** -8 * ref.abs() + 2.0 ** -14 * size).all()), float((err - 2.0 ** -8 * ref.abs()).div(size + 1e-30).max())
+
+
+@pytest.mark.parametrize("lens,H,kv,dim", [([1, 16, 100], 4, 2, 128), ([5000, 3], 16, 1, 64), ([700], 8, 2, 256)])
+def test_paged_attention_of_infinite_values(ctx, lens, H, kv, dim):
+    """Weights that are all alike: one infinite value makes its column infinite, two of different sign make it no number."""
+    q, kc, vc, tables, lengths, _ = _attention_case(lens, H, kv, dim, 16, 3, gated=False, poison=False)
+    q.zero_()
+    for b, n in enumerate(lens):
+        for j, d, x in ((0, 1, "inf"), (n - 1, 2, "-inf"), (0, 3, "inf"), (n - 1, 3, "-inf"), (n // 2, 4, "nan")):
+            vc[tables[b, j // 16].long(), j % 16, :, d] = float(x)
+    got = paged.attention_paged(q, kc, vc, tables, lengths)
+    ctx.sync()
+    ref, _ = attention_64(q, kc, vc, tables, lens, None, dim ** -0.5)
+    got, special = got.float().unflatten(1, (-1, dim)), ~torch.isfinite(ref)
+    assert bool(special[:, :, 1:5].all()) and int(special.sum()) == 4 * len(lens) * H
+    assert torch.equal(got[special].nan_to_num(7.0), ref[special].float().nan_to_num(7.0)) and bool(torch.isfinite(got[~special]).all())
