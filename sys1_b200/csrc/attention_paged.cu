@@ -132,6 +132,11 @@ __device__ __forceinline__ float rcp_fast(float x) {  // relative error 2^-23, b
     return r;
 }
 __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.f + exp2_fast(-1.4426950408889634f * x)); }
+// The sum of a part of a span's weights (maximum, sum) in terms of the whole span's maximum. A part without a finite score counts only
+// where the whole has none: 0 if it had no key, else no number.
+__device__ __forceinline__ float weighed(float2 mark, float top) {
+    return mark.x != -INFINITY ? mark.y * exp2_fast(mark.x - top) : top == -INFINITY ? mark.y : 0.f;
+}
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory"); }
 
 // One warp's pass over its tiles of a span: keys first, first + 16 W, ..., 16 to a tile, below `end`. NT = 1: up to 8 query heads, held in registers;
@@ -240,6 +245,7 @@ struct WarpPass {
             l[t][0] = l[t][1] = 0.f;
         }
         int rslot = 0;
+        uint32_t seen = 0;  // whether any key was there
         // this lane's rows of the ldmatrix tiles: the 16-byte pieces 2 s + h of row r lie at r * 2 D + ((2 s + h) ^ (r & 7)) * 16, which is
         // one of four places and a multiple of 128 bytes
         uint32_t kat[4], vat[4];
@@ -259,6 +265,7 @@ struct WarpPass {
             wslot = wslot + 1 == kSlots ? 0 : wslot + 1;
             {
                 const uint32_t live = masks[rslot], slot = ring + rslot * kSlotBytes;
+                seen |= live;
                 float c[NT][kChains][4];
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -362,6 +369,11 @@ struct WarpPass {
                 l[t][0] += __shfl_xor_sync(0xffffffffu, l[t][0], o);
                 l[t][1] += __shfl_xor_sync(0xffffffffu, l[t][1], o);
             }
+        if (seen)  // keys whose scores are all -inf: the sum of their weights is no number, unless others have a finite score
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) l[t][e] = m[t][e] == -INFINITY ? __int_as_float(0x7fffffff) : l[t][e];
     }
 };
 
@@ -568,7 +580,7 @@ __global__ void __launch_bounds__(W * 32, P) s1_attention_paged_kernel(const Pag
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) high = fmaxf(high, marks[w][tid].x);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) sum += marks[w][tid].x == -INFINITY ? 0.f : marks[w][tid].y * exp2_fast(marks[w][tid].x - high);
+                for (int w = 0; w < kWarps; ++w) sum += weighed(marks[w][tid], high);
                 marks_all[tid] = make_float2(high, sum);
             }
         }
@@ -645,7 +657,7 @@ __global__ void __launch_bounds__(THREADS) s1_attention_paged_join_kernel(const 
     float sum = 0.f;
     auto weigh = [&](int i, const float2& m) {
         weights[i] = m.x == -INFINITY ? 0.f : exp2_fast(m.x - top);
-        sum += m.y * weights[i];
+        sum += weighed(m, top);
     };
     if (tid < pieces) weigh(tid, mark);
     for (int i = tid + THREADS; i < pieces; i += THREADS) weigh(i, p.marks[place(i)]);

@@ -7,7 +7,7 @@ import torch
 
 from paged_model import attention_64
 from sys1_b200 import paged
-from test_paged_gpu import _attention_case
+from test_paged_gpu import DEV, _attention_case, _refused
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,36 @@ def test_paged_attention_of_infinite_values(ctx, lens, H, kv, dim):
     got, special = got.float().unflatten(1, (-1, dim)), ~torch.isfinite(ref)
     assert bool(special[:, :, 1:5].all()) and int(special.sum()) == 4 * len(lens) * H
     assert torch.equal(got[special].nan_to_num(7.0), ref[special].float().nan_to_num(7.0)) and bool(torch.isfinite(got[~special]).all())
+
+
+def _blind(q, kc, tables, b, keys, page=16):
+    """Scores of -inf for these keys of row b, for every head."""
+    q[..., 0] = q[..., 0].abs() + 0.5
+    j = torch.tensor(list(keys), device=DEV, dtype=torch.long)
+    kc[tables[b].long()[j // page], j % page, :, 0] = float("-inf")
+
+
+@pytest.mark.parametrize("lens,H,kv,dim", [([20, 100, 33, 0], 4, 2, 128), ([5000, 9000, 300, 40], 8, 2, 256), ([9000, 6000, 100], 16, 1, 64), ([70] * 450, 2, 1, 64)])
+def test_paged_attention_of_scores_that_are_minus_infinity(ctx, lens, H, kv, dim):
+    """A row without a finite score is no number (softmax divides nothing by nothing); keys of -inf beside others weigh nothing, also where
+    they are all that a warp or a block sees. A row without a key stays zero."""
+    q, kc, vc, tables, lengths, gate = _attention_case(lens, H, kv, dim, 16, 11, poison=False)
+    _blind(q, kc, tables, 0, range(lens[0]))
+    _blind(q, kc, tables, 1, range(lens[1] - 1))          # only the last key is left
+    _blind(q, kc, tables, 2, range(1, lens[2]))           # only the first
+    got = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate)
+    ctx.sync()
+    ref, size = attention_64(q, kc, vc, tables, lens, gate, dim ** -0.5)
+    got = got.double().unflatten(1, (-1, dim))
+    assert bool(torch.isnan(ref[0]).all()) and bool(torch.isnan(got[0]).all())
+    assert bool(((got[1:] - ref[1:]).abs() <= 2.0 ** -8 * ref[1:].abs() + 2.0 ** -14 * size[1:]).all())
+
+
+def test_paged_attention_of_a_row_whose_pages_are_all_bad(ctx):
+    """Keys that are left out are no keys: zeros, and the report; a bad page beside keys of -inf does not hide them."""
+    q, kc, vc, tables, lengths, _ = _attention_case([40, 40], 2, 1, 64, 16, 5, gated=False, poison=False)
+    _blind(q, kc, tables, 1, range(40))
+    tables[0, :3], tables[1, 1] = -1, -1
+    got = paged.attention_paged(q, kc, vc, tables, lengths)
+    _refused(ctx, "names page -1")
+    assert bool((got[0] == 0).all()) and bool(torch.isnan(got[1]).all())
