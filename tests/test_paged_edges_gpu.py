@@ -2,6 +2,7 @@
 
 A rounding to bf16 is off by at most 2^-8 of the value, and so is the output's. A softmax weight enters its product as two bf16 values, the
 first cut to eight bits and the rest rounded: 2^-15 of it. The f32 sums and exponentials stay below 2^-15 of the sums taken with |v|."""
+import numpy as np
 import pytest
 import torch
 
@@ -75,3 +76,34 @@ def test_paged_attention_of_a_row_whose_pages_are_all_bad(ctx):
     got = paged.attention_paged(q, kc, vc, tables, lengths)
     _refused(ctx, "names page -1")
     assert bool((got[0] == 0).all()) and bool(torch.isnan(got[1]).all())
+
+
+@pytest.mark.parametrize("rows,H,kv,dim,longest", [(200, 6, 3, 64, 200000), (230, 6, 2, 128, 150000), (100, 32, 2, 64, 100000), (3, 16, 1, 128, 90000), (250, 2, 2, 256, 60000),
+                                                   (1, 8, 2, 256, 131071), (1, 4, 2, 128, 70001), (2, 4, 4, 64, 70001), (1, 32, 2, 256, 30001), (1, 64, 4, 64, 66164),
+                                                   (160, 12, 1, 256, 20001), (300, 12, 1, 128, 20001)])
+def test_paged_attention_counts_every_key_once(ctx, rows, H, kv, dim, longest):
+    """Scores that are all alike, values that are 1 at the keys that a column marks and 0 elsewhere: the column's output is how many of its
+    keys were seen over how many there are. A column marks at most 64 keys, so one missing or counted twice is off by 2^-6 of the
+    output, and what is allowed is 2^-8 (the output's rounding) and 2^-14. Every key is marked once; neighbours have different columns."""
+    lens = [int(n) for n in np.random.RandomState(9).randint(0, 60, rows)]
+    b = rows // 2
+    lens[b] = longest
+    q, kc, vc, tables, lengths, _ = _attention_case(lens, H, kv, dim, 64, 9, gated=False, poison=False)
+    kc.zero_()
+    j = torch.arange(longest, device=DEV)
+    page, at = tables[b].long()[j // 64], j % 64
+    which = torch.arange(kv, device=DEV)[:, None] * 7 + j  # the KV heads' columns are not alike
+    column, turn = which % dim, which // dim // 64
+    counts = 0
+    for t in range(int(turn.max()) + 1):
+        vc.zero_()
+        for h in range(kv):
+            mine = turn[h] == t
+            vc[page[mine], at[mine], h, column[h][mine]] = 1.0
+        want = torch.stack([torch.bincount(column[h][turn[h] == t], minlength=dim) for h in range(kv)]).double()
+        assert int(want.max()) <= 64
+        got = paged.attention_paged(q, kc, vc, tables, lengths)[b].double().view(kv, H // kv, dim) * longest
+        assert bool(((got - want[:, None]).abs() <= (2.0 ** -8 + 2.0 ** -14) * want[:, None]).all()), (t, float((got - want[:, None]).abs().max()))
+        counts += int(want.sum())
+    ctx.sync()
+    assert counts == kv * longest
