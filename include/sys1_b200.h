@@ -397,7 +397,7 @@ int s1_cache_write(s1_ctx* ctx, const void* k, long long ldk, long long k_head_s
  * product with v as two bf16 values each: 2^-15 of a weight.)
  * A row with lengths[b] <= 0 gets zeros, one whose scores are all -inf NaN. lengths: DEVICE int32; tables [num_seqs, ldt], of which
  * table_width entries a row may be used. A length beyond that is reported and its row gets zeros; a page outside the cache is reported
- * and its keys are left out.
+ * and its keys are left out. `scale` must be positive and below 2.35e38.
  * head_dim 64, 128 or 256; any group size; rows x KV heads x (tokens that a row's block table can hold) / 64 below 2^31. q, gate: as
  * for s1_attention_gqa; out: bf16 [num_seqs, heads * head_dim].
  * `workspace`: device memory, 16-byte aligned, of s1_attention_paged_workspace(head_dim) bytes whatever the batch. Calls that may

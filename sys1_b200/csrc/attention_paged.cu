@@ -745,7 +745,8 @@ extern "C" int s1_attention_paged(s1_ctx* ctx, const void* q, long long ldq, lon
     if (head_dim != 64 && head_dim != 128 && head_dim != 256)
         return s1_fail(ctx, S1_EINVAL, "%s: head_dim must be 64, 128 or 256 (got %d)", who, head_dim);
     if (num_seqs < 0 || kv_heads < 1 || heads < kv_heads || heads % kv_heads) return s1_fail(ctx, S1_EINVAL, "%s: heads must be a multiple of kv_heads", who);
-    if (!(scale > 0.f) || !(scale < 3.0e38f)) return s1_fail(ctx, S1_EINVAL, "%s: scale must be positive and finite", who);
+    // (scores are kept in units of log 2: the scale times log2(e) has to be finite too)
+    if (!(scale > 0.f) || !(scale < 2.35e38f)) return s1_fail(ctx, S1_EINVAL, "%s: scale must be positive and below 2.35e38", who);
     if (num_pages < 1 || page_size < 1 || page_size > 65536 || (page_size & (page_size - 1)))
         return s1_fail(ctx, S1_EINVAL, "%s: page_size must be a power of two up to 65536 (got %d)", who, page_size);
     if (static_cast<long long>(table_width) * page_size > (1ll << 30)) return s1_fail(ctx, S1_EINVAL, "%s: block tables of over 2^30 tokens a row", who);

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from paged_model import attention_64
-from sys1_b200 import paged
+from sys1_b200 import _lib, paged
 from test_paged_gpu import DEV, _attention_case, _refused
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +107,14 @@ def test_paged_attention_counts_every_key_once(ctx, rows, H, kv, dim, longest):
         counts += int(want.sum())
     ctx.sync()
     assert counts == kv * longest
+
+
+def test_paged_attention_refuses_a_scale_beyond_its_exponent(ctx):
+    """The scores are kept in units of log 2: a scale that is finite but not times log2(e) would make every score infinite or no number."""
+    q, kc, vc, tables, lengths, _ = _attention_case([20, 30], 4, 2, 64, 16, 1, gated=False)
+    with pytest.raises(_lib.S1Error, match="scale"):
+        paged.attention_paged(q, kc, vc, tables, lengths, scale=2.9e38)
+    q.zero_()
+    got = paged.attention_paged(q, kc, vc, tables, lengths, scale=2.3e38)
+    ctx.sync()
+    assert torch.equal(got, paged.attention_paged(q, kc, vc, tables, lengths))
