@@ -78,6 +78,10 @@ int64_t extent(int64_t n, const char* name) {
     return n;
 }
 
+// A dimension of size 1 has no stride: what a transposed or expanded tensor says there is of no account, and `otherwise` is used.
+bool next_to(const Tensor& t, int dim) { return t.stride(dim) == 1 || t.size(dim) == 1; }
+int64_t stride(const Tensor& t, int dim, int64_t otherwise) { return t.size(dim) == 1 ? otherwise : t.stride(dim); }
+
 template <typename T>
 T* address(const Tensor& t) {
     return static_cast<T*>(t.data_ptr());
@@ -95,9 +99,9 @@ struct Table {
     int width;
 };
 Table table(const Tensor& t, int dev, int64_t rows) {
-    if (!on(t, dev, at::kInt) || t.dim() != 2 || t.size(0) != rows || t.stride(1) != 1)
+    if (!on(t, dev, at::kInt) || t.dim() != 2 || t.size(0) != rows || !next_to(t, 1))
         throw Refused{"block tables must be an int32 CUDA tensor [" + std::to_string(rows) + ", pages] with contiguous rows"};
-    return {address<int32_t>(t), t.stride(0), static_cast<int>(extent(t.size(1), "the block table"))};
+    return {address<int32_t>(t), stride(t, 0, t.size(1)), static_cast<int>(extent(t.size(1), "the block table"))};
 }
 
 struct Heads {  // a tensor of head rows
@@ -109,15 +113,22 @@ Heads heads(const Tensor& t, int dev, std::initializer_list<int64_t> shape, cons
         throw Refused{std::string(name) + " must be a bf16 CUDA tensor [tokens, heads, head_dim] with contiguous head rows (no CPU fallback)"};
     if (!has_shape(t, shape)) throw Refused{std::string(name) + " must have shape " + shape_of(shape) + ", not " + shape_of(t.sizes())};
     if (t.stride(2) != 1) throw Refused{std::string(name) + " must have contiguous head rows"};
-    return {t.data_ptr(), t.stride(0), t.stride(1)};
+    const int64_t head = stride(t, 1, t.size(2));
+    return {t.data_ptr(), stride(t, 0, (t.size(1) - 1) * head + t.size(2)), head};
 }
 
-void caches(const Tensor& k, const Tensor& v, int dev) {
+struct Cache {
+    int64_t page, token, head;
+};
+Cache caches(const Tensor& k, const Tensor& v, int dev) {
     if (!on(k, dev, at::kBFloat16) || k.dim() != 4 || !on(v, dev, at::kBFloat16) || v.dim() != 4)
         throw Refused{"k_cache and v_cache must be bf16 CUDA tensors [pages, page_size, kv_heads, head_dim] with contiguous head rows (no CPU fallback)"};
-    if (k.sizes() != v.sizes() || k.strides() != v.strides() || k.stride(3) != 1)
+    bool alike = k.sizes() == v.sizes() && k.stride(3) == 1 && v.stride(3) == 1;
+    for (int i = 0; i < 3 && alike; ++i) alike = k.size(i) == 1 || k.stride(i) == v.stride(i);
+    if (!alike)
         throw Refused{"k_cache and v_cache must have the same shape and strides, and contiguous head rows"};
     for (int i = 0; i < 4; ++i) extent(k.size(i), "the cache");
+    return {stride(k, 0, k.size(3)), stride(k, 1, k.size(3)), stride(k, 2, k.size(3))};
 }
 
 PyObject* wrapped(const Tensor& t) { return THPVariable_Wrap(t); }
@@ -179,7 +190,7 @@ PyObject* cache_write(const Args& a) {
     s1_ctx* const ctx = a.context();
     const Tensor &k = a.tensor(1, "k"), &v = a.tensor(2, "v"), &kc = a.tensor(3, "k_cache"), &vc = a.tensor(4, "v_cache"), &slots = a.tensor(5, "slots");
     const int dev = gpu_of(k);
-    caches(kc, vc, dev);
+    const Cache cache = caches(kc, vc, dev);
     const int64_t kv = kc.size(2), dim = kc.size(3), T = k.dim() ? extent(k.size(0), "k") : 0;
     const Heads kh = heads(k, dev, {T, kv, dim}, "k"), vh = heads(v, dev, {T, kv, dim}, "v");
     const int32_t* sp = ints(slots, dev, T, "slots");
@@ -207,7 +218,7 @@ PyObject* cache_write(const Args& a) {
     return code(run([&] {
         return s1_cache_write(ctx, kh.at, kh.token, kh.head, vh.at, vh.token, vh.head, sp, static_cast<int>(T), static_cast<int>(kv), static_cast<int>(dim), weight,
                               eps, cos, sin, positions, rows, rotary, bf16_ops, kc.data_ptr(), vc.data_ptr(), static_cast<int>(kc.size(0)),
-                              static_cast<int>(kc.size(1)), kc.stride(0), kc.stride(1), kc.stride(2));
+                              static_cast<int>(kc.size(1)), cache.page, cache.token, cache.head);
     }));
 }
 
@@ -216,7 +227,7 @@ PyObject* attention_paged(const Args& a) {
     s1_ctx* const ctx = a.context();
     const Tensor &q = a.tensor(1, "q"), &kc = a.tensor(2, "k_cache"), &vc = a.tensor(3, "v_cache"), &tables = a.tensor(4, "block tables"), &lengths = a.tensor(5, "lengths");
     const int dev = gpu_of(q);
-    caches(kc, vc, dev);
+    const Cache cache = caches(kc, vc, dev);
     const int64_t kv = kc.size(2), dim = kc.size(3), B = q.dim() == 3 ? extent(q.size(0), "q") : 0, H = q.dim() == 3 ? extent(q.size(1), "q") : 0;
     const Heads qh = heads(q, dev, {B, H, dim}, "q");
     const Table t = table(tables, dev, B);
@@ -237,8 +248,8 @@ PyObject* attention_paged(const Args& a) {
     if (!on(ws, dev, at::kByte) || !ws.is_contiguous()) throw Refused{"the workspace must be a contiguous uint8 CUDA tensor"};
     const int rc = run([&] {
         return s1_attention_paged(ctx, qh.at, qh.token, qh.head, kc.data_ptr(), vc.data_ptr(), static_cast<int>(kc.size(0)), static_cast<int>(kc.size(1)),
-                                  kc.stride(0), kc.stride(1), kc.stride(2), t.at, t.ld, t.width, lp, static_cast<int>(B), static_cast<int>(H), static_cast<int>(kv),
-                                  static_cast<int>(dim), scale, gh.at, gh.token, gh.head, out.data_ptr(), out.stride(0), ws.data_ptr(),
+                                  cache.page, cache.token, cache.head, t.at, t.ld, t.width, lp, static_cast<int>(B), static_cast<int>(H), static_cast<int>(kv),
+                                  static_cast<int>(dim), scale, gh.at, gh.token, gh.head, out.data_ptr(), stride(out, 0, H * dim), ws.data_ptr(),
                                   static_cast<size_t>(ws.numel()));
     });
     return rc ? code(rc) : result(a, 8, out);
@@ -256,7 +267,7 @@ PyObject* gated_delta_rule_step(const Args& args) {
         throw Refused{"mixed must have " + std::to_string((2LL * key_heads + Hv) * 128) + " columns for " + std::to_string(key_heads) + " key and " + std::to_string(Hv) +
                       " value heads, not " + std::to_string(C)};
     auto check = [&](const Tensor& t, const char* name, at::ScalarType type, std::initializer_list<int64_t> shape, bool by_rows) {
-        if (!on(t, dev, type) || !has_shape(t, shape) || !(by_rows ? t.stride(-1) == 1 : t.is_contiguous()))
+        if (!on(t, dev, type) || !has_shape(t, shape) || !(by_rows ? next_to(t, 1) : t.is_contiguous()))
             throw Refused{std::string(name) + " must be a " + (by_rows ? "" : "contiguous ") +
                           (type == at::kBFloat16 ? "bfloat16" : type == at::kFloat ? "float32" : "int32") + " CUDA tensor " + shape_of(shape) +
                           (by_rows ? " with contiguous rows" : "") + " on the call's GPU (no CPU fallback)"};
@@ -287,8 +298,9 @@ PyObject* gated_delta_rule_step(const Args& args) {
     }
     if (rows == 0) return result(args, 15, out);
     const int rc = run([&] {
-        return s1_gated_delta_rule_step(ctx, x, mixed.stride(0), taps, positions, bp, ap, b.stride(0), dt_bias, decay, zp, z.stride(0), weight, eps, index,
-                                        static_cast<int>(states), cs, sp, static_cast<int>(rows), key_heads, static_cast<int>(Hv), out.data_ptr(), out.stride(0));
+        return s1_gated_delta_rule_step(ctx, x, stride(mixed, 0, C), taps, positions, bp, ap, stride(b, 0, Hv), dt_bias, decay, zp, stride(z, 0, inner), weight, eps,
+                                        index, static_cast<int>(states), cs, sp, static_cast<int>(rows), key_heads, static_cast<int>(Hv), out.data_ptr(),
+                                        stride(out, 0, inner));
     });
     return rc ? code(rc) : result(args, 15, out);
 }

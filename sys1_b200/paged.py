@@ -39,9 +39,9 @@ def _ints(t: torch.Tensor, dev: int, n: int, name: str) -> int:
 
 def _table(t: torch.Tensor, dev: int, rows: int):
     """Address, row stride and width of the block tables."""
-    if t.dtype is not _I32 or t.get_device() != dev or dev < 0 or t.dim() != 2 or t.shape[0] != rows or t.stride(1) != 1:
+    if t.dtype is not _I32 or t.get_device() != dev or dev < 0 or t.dim() != 2 or t.shape[0] != rows or (t.stride(1) != 1 and t.shape[1] != 1):
         raise ValueError(f"block tables must be an int32 CUDA tensor [{rows}, pages] with contiguous rows")
-    return t.data_ptr(), t.stride(0), t.shape[1]
+    return t.data_ptr(), t.shape[1] if rows == 1 else t.stride(0), t.shape[1]
 
 
 def _context(dev: int, ctx: Optional[device.Context]):

@@ -7,8 +7,8 @@ import pytest
 import torch
 
 from paged_model import attention_64
-from sys1_b200 import _lib, paged
-from test_paged_gpu import DEV, _attention_case, _refused
+from sys1_b200 import _lib, paged, qwen35
+from test_paged_gpu import DEV, _attention_case, _refused, _step_case, bf, gen, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,53 @@ def test_paged_attention_refuses_a_scale_beyond_its_exponent(ctx):
     got = paged.attention_paged(q, kc, vc, tables, lengths, scale=2.3e38)
     ctx.sync()
     assert torch.equal(got, paged.attention_paged(q, kc, vc, tables, lengths))
+
+
+# ------------------------------------------------------------------------------------------------ strides that mean nothing
+def _odd(t, dims, stride=3):
+    """The same values with another stride in dimensions of size 1."""
+    strides = list(t.stride())
+    for d in dims:
+        assert t.shape[d] == 1
+        strides[d] = stride
+    return t.as_strided(t.shape, strides)
+
+
+def test_strides_of_dimensions_of_size_one_are_of_no_account(ctx):
+    """One row, one head, one page or one token: whatever a transposed or expanded tensor leaves as the stride there."""
+    q, kc, vc, tables, lengths, gate = _attention_case([13], 4, 1, 128, 16, 2, poison=False)
+    want = paged.attention_paged(q, kc, vc, tables, lengths, gate=gate)
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)  # [1, 4, 128] of strides 128, 128: heads x rows turned round
+    assert turned.stride(0) == 128 and torch.equal(paged.attention_paged(turned, kc, vc, tables, lengths, gate=gate), want)
+    out = torch.empty(512, 1, dtype=torch.bfloat16, device=DEV).t()
+    paged.attention_paged(_odd(q, [0]), _odd(kc, [2]), _odd(vc, [2], 0), _odd(tables, [0], 1), lengths, gate=_odd(gate, [0], 1), out=out)
+    assert torch.equal(out, want)
+    one = [torch.zeros(1, 16, 1, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    k, v = bf(gen(3), 1, 1, 128), bf(gen(4), 1, 1, 128)
+    paged.cache_write(_odd(k, [0, 1], 1), _odd(v, [0, 1], 0), _odd(one[0], [0]), _odd(one[1], [0, 2], 0), ints([5]))
+    ctx.sync()
+    assert torch.equal(one[0][0, 5], k[0]) and torch.equal(one[1][0, 5], v[0]) and int((one[0] != 0).any(-1).sum()) == 1
+    small = [torch.zeros(3, 1, 2, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2)]  # pages of one token
+    k, v = bf(gen(3), 2, 2, 64), bf(gen(4), 2, 2, 64)
+    paged.cache_write(k, v, _odd(small[0], [1]), _odd(small[1], [1], 0), ints([2, 0]))
+    ctx.sync()
+    assert torch.equal(small[0][[2, 0], 0], k) and torch.equal(small[1][[2, 0], 0], v)
+    table = ints([[4, 7]])
+    r = paged.block_tables(ints([3]), _odd(table, [0], 1), ints([1, 2]), ints([2]), 4)
+    ctx.sync()
+    assert r.slots.tolist() == [19]
+    paged.release_blocks(ints([1]), r.lengths, _odd(table, [0], 1), ints([0, 0]), r.free_count.zero_(), 4)
+    ctx.sync()
+    assert r.lengths.tolist() == [-1] and r.free_count.tolist() == [1]
+
+
+def test_delta_step_of_one_row_of_any_stride(ctx):
+    c = _step_case(1, 2, 4, 8)
+    d = dict(c, state=c["state"].clone(), conv_state=c["conv_state"].clone())
+    want = qwen35.gated_delta_rule_step(**c)
+    for name in ("mixed", "b", "a", "z"):
+        d[name] = _odd(d[name], [0], 1)
+    out = torch.empty(512, 1, dtype=torch.bfloat16, device=DEV).t()
+    qwen35.gated_delta_rule_step(**d, out=out)
+    ctx.sync()
+    assert torch.equal(out, want) and torch.equal(c["state"], d["state"]) and torch.equal(c["conv_state"], d["conv_state"])
