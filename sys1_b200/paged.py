@@ -143,7 +143,10 @@ class PagedCache:
     `admit(n)` picks idle rows, `Decoder.prefill` fills them, `Decoder.step` adds a token to every active row, `release(rows)`
     gives their pages back. The bookkeeping lives on the GPU (`lengths`, `tables`, `free_pages`, `free_count`), so that a captured
     step can be replayed; `held` and `pages_left` mirror it on the host, where a request that does not fit is refused before
-    anything is launched. After replaying a captured step, tell the mirror with `advanced(steps)`."""
+    anything is launched. After replaying a captured step, tell the mirror with `advanced(steps)`.
+
+    A step that raises between its layers has moved the states of some and not of others. Its rows are then `unfinished`: no step is
+    taken until they have been released."""
 
     def __init__(self, cfg, rows: int, num_pages: int, page_size: int = 64, max_length: int = 8192, dev="cuda"):
         if rows < 1 or num_pages < 1 or max_length < 1 or page_size < 1 or page_size & (page_size - 1):
@@ -170,6 +173,7 @@ class PagedCache:
         self.free_count = torch.full((1,), num_pages, **i32)
         self.state_index = torch.full((rows,), -1, **i32)
         self.held = np.full(rows, -1, dtype=np.int64)
+        self.unfinished = np.zeros(rows, dtype=bool)
         self.pages_left = int(num_pages)
         channels = (2 * cfg.linear_num_key_heads + cfg.linear_num_value_heads) * 128
         self.layers: List = []
@@ -213,10 +217,10 @@ class PagedCache:
         start = np.where(added > 0, 0, -1).astype(np.int32)  # lengths that change: the new rows' only
         state = np.where(index, np.arange(self.rows), -1).astype(np.int32)
         added_dev, start_dev, state_dev = torch.from_numpy(np.stack([added, start, state])).to(self.device)
-        self.lengths.copy_(torch.maximum(self.lengths, start_dev))
+        # nothing of the cache changes before this call, and nothing fails after it
+        plan = block_tables(torch.maximum(self.lengths, start_dev), self.tables, self.free_pages, self.free_count, self.page_size, added=added_dev,
+                            max_tokens=int(sum(lengths)), lengths=self.lengths, free_count_out=self.free_count)
         self.state_index.copy_(state_dev)
-        plan = block_tables(self.lengths, self.tables, self.free_pages, self.free_count, self.page_size, added=added_dev, max_tokens=int(sum(lengths)),
-                            lengths=self.lengths, free_count_out=self.free_count)
         for r, n in zip(rows, lengths):
             self.held[r] = n
             self.pages_left -= self._pages(n)
@@ -224,22 +228,34 @@ class PagedCache:
 
     def extend(self) -> BlockTables:
         """One more token for every active row. Token r of the step belongs to row r; idle rows have slot -1."""
-        if not torch.cuda.is_current_stream_capturing():
-            self.advanced(1)
-        return block_tables(self.lengths, self.tables, self.free_pages, self.free_count, self.page_size, lengths=self.lengths,
+        eager = not torch.cuda.is_current_stream_capturing()
+        if eager:
+            self._refuse(1)
+        plan = block_tables(self.lengths, self.tables, self.free_pages, self.free_count, self.page_size, lengths=self.lengths,
                             free_count_out=self.free_count)
+        if eager:
+            self._advance(1)
+        return plan
 
     def fits(self, steps: int = 1) -> bool:
         """Whether every active row can grow by `steps` tokens."""
         live = self.held[self.held >= 0]
         need = sum(self._pages(n + steps) - self._pages(n) for n in live)
-        return need <= self.pages_left and (len(live) == 0 or int(live.max()) + steps <= self.max_length)
+        return not self.unfinished.any() and need <= self.pages_left and (len(live) == 0 or int(live.max()) + steps <= self.max_length)
 
     def advanced(self, steps: int = 1) -> None:
-        """Notes on the host that every active row has `steps` more tokens; refuses steps that do not fit. (`Decoder.step` calls it;
+        """Notes on the host that every active row has `steps` more tokens; refuses steps that do not fit. (`Decoder.step` does as much;
         call it yourself before replaying a captured step.)"""
+        self._refuse(steps)
+        self._advance(steps)
+
+    def _refuse(self, steps: int) -> None:
+        if self.unfinished.any():
+            raise ValueError(f"a call failed half-way and left rows {np.flatnonzero(self.unfinished).tolist()} with part of a token: release them")
         if not self.fits(steps):
             raise ValueError(f"{steps} more token(s) do not fit: {self.pages_left} pages left, rows of up to {self.max_length} tokens")
+
+    def _advance(self, steps: int) -> None:
         live = self.held >= 0
         self.pages_left -= sum(self._pages(n + steps) - self._pages(n) for n in self.held[live])
         self.held[live] += steps
@@ -253,8 +269,9 @@ class PagedCache:
         ended[rows] = 1
         index = np.where((self.held >= 0) & (ended == 0), np.arange(self.rows), -1).astype(np.int32)
         ended_dev, index_dev = torch.from_numpy(np.stack([ended, index])).to(self.device)
-        self.state_index.copy_(index_dev)
         release_blocks(ended_dev, self.lengths, self.tables, self.free_pages, self.free_count, self.page_size)
+        self.state_index.copy_(index_dev)
+        self.unfinished[rows] = False
         for r in rows:
             self.pages_left += self._pages(self.held[r])
             self.held[r] = -1

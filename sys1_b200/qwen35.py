@@ -473,6 +473,7 @@ class Decoder:
         for n in lengths:
             bounds.append(bounds[-1] + n)
         plan = cache.enter(rows, lengths)
+        cache.unfinished[rows] = True
         previous = getattr(ctx, "_plan", None)
         try:
             cu, index = torch.tensor([bounds, rows + [0]], dtype=torch.int32).to(ids.device)
@@ -486,25 +487,31 @@ class Decoder:
             raise
         finally:
             ctx.use_plan(previous)
+        cache.unfinished[rows] = False
         return x, rows
 
     def step(self, ids: torch.Tensor, cache: "paged.PagedCache") -> torch.Tensor:
         """One new token of every active row of the cache: `ids [cache.rows]` (CUDA; idle rows need an id of the vocabulary too,
         which is of no account). Returns the hidden states `[cache.rows, hidden]` after the final norm; the rows of idle requests mean nothing.
-        Can be captured into a CUDA graph and replayed (`cache.advanced` tells the host's mirror)."""
+        Can be captured into a CUDA graph and replayed (`cache.advanced` tells the host's mirror). A step that raises once its first kernel
+        is under way leaves its rows `cache.unfinished`: they have to be released."""
         if ids.dim() != 1 or not ids.is_cuda or ids.shape[0] != cache.rows:
             raise ValueError(f"ids must be a CUDA tensor [{cache.rows}], a token for every row of the cache (no CPU fallback)")
         self._check(cache, ids)
         if not torch.cuda.is_current_stream_capturing() and cache.held.max() >= self.max_positions:
             raise ValueError(f"a row has reached the decoder's {self.max_positions} positions")
+        live = (cache.held >= 0) & (not torch.cuda.is_current_stream_capturing())  # (what fails while it is captured has moved nothing)
         plan = cache.extend()
+        cache.unfinished |= live
         x = _norm.embedding(self.w["embed_tokens"], ids.to(torch.int32).contiguous())
         # a row that got no page (a replayed step that the host did not look after) has no slot, and keeps its states as they are
         index = torch.where(plan.slots < 0, plan.slots, cache.state_index)
         for layer, part in zip(self.layers, cache.layers):
             x = layer.step(x, Kept(part, plan.positions, plan.slots, index, tables=cache.tables, lengths=cache.lengths,
                                    workspace=cache.workspace), inplace=True)
-        return self.norm(x)
+        x = self.norm(x)
+        cache.unfinished &= ~live
+        return x
 
     def _check(self, cache, ids) -> None:
         if cache.device != ids.device or cache.device != self.w["embed_tokens"].device:

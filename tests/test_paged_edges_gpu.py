@@ -7,8 +7,8 @@ import pytest
 import torch
 
 from paged_model import attention_64
-from sys1_b200 import _lib, paged, qwen35
-from test_paged_gpu import DEV, _attention_case, _refused, _step_case, bf, gen, ints
+from sys1_b200 import _lib, device, paged, qwen35
+from test_paged_gpu import DEV, _attention_case, _decoder, _refused, _step_case, bf, gen, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +168,95 @@ def test_delta_step_of_one_row_of_any_stride(ctx):
     qwen35.gated_delta_rule_step(**d, out=out)
     ctx.sync()
     assert torch.equal(out, want) and torch.equal(c["state"], d["state"]) and torch.equal(c["conv_state"], d["conv_state"])
+
+
+# ------------------------------------------------------------------------------------------------ calls that fail half-way
+def _fails(*a, **k):
+    raise RuntimeError("no")
+
+
+def _device_matches(cache):
+    return cache.lengths.tolist() == cache.held.tolist() and cache.free_count.tolist() == [cache.pages_left]
+
+
+def test_a_step_that_fails_half_way_is_not_gone_on_from(ctx, monkeypatch):
+    """Some layers' states have the token and others do not: the rows are refused until they are released, others may come in, and nothing
+    of the failed step is left."""
+    cfg, w, dec = _decoder()
+    cache, other = (paged.PagedCache(cfg, rows=3, num_pages=16, page_size=16, max_length=64, dev=DEV) for _ in range(2))
+    ids = torch.randint(0, 500, (60,), generator=torch.Generator().manual_seed(3)).to(DEV)
+    tokens = ids[:3]
+    dec.prefill(ids[:47], [15, 32], cache)
+    for broken in (1, 3):  # a linear-attention layer, the full-attention layer
+        live = cache.active
+        with monkeypatch.context() as m:
+            m.setattr(dec.layers[broken].mlp, "forward", _fails)
+            with pytest.raises(RuntimeError, match="no"):
+                dec.step(tokens, cache)
+        ctx.sync()
+        assert _device_matches(cache) and not cache.fits()
+        with pytest.raises(ValueError, match="release"):
+            dec.step(tokens, cache)
+        with pytest.raises(ValueError, match="release"):
+            cache.advanced(1)
+        assert _device_matches(cache)
+        _, rows = dec.prefill(ids[47:], [13], cache)  # an idle row is none of its business
+        with pytest.raises(ValueError, match="release"):
+            dec.step(tokens, cache)
+        cache.release(live[:1])
+        if len(live) > 1:
+            with pytest.raises(ValueError, match="release"):
+                dec.step(tokens, cache)
+            cache.release(live[1:])
+        _, same = dec.prefill(ids[47:], [13], other)
+        got, want = dec.step(tokens, cache), dec.step(tokens[rows].repeat(3), other)
+        ctx.sync()
+        assert torch.equal(got[rows[0]], want[same[0]]) and _device_matches(cache)
+        other.release(same)
+    cache.release(cache.active)
+    ctx.sync()
+    assert sorted(cache.free_pages.tolist()) == list(range(16)) and cache.free_count.tolist() == [16]
+
+
+def test_a_capture_that_fails_has_moved_nothing(ctx, monkeypatch):
+    cfg, w, dec = _decoder(layers=2)
+    cache = paged.PagedCache(cfg, rows=2, num_pages=8, page_size=16, max_length=64, dev=DEV)
+    ids = torch.zeros(20, dtype=torch.int64, device=DEV)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        dec.prefill(ids, [20], cache)
+        dec.step(ids[:2], cache)
+        stream.synchronize()
+        with monkeypatch.context() as m:
+            m.setattr(dec.layers[1].mlp, "forward", _fails)
+            with pytest.raises(RuntimeError, match="no"):
+                with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+                    dec.step(ids[:2], cache)
+        assert cache.fits()
+        dec.step(ids[:2], cache)
+        stream.synchronize()
+        device.load(0).sync()
+    assert cache.held.tolist() == [22, -1] and _device_matches(cache)
+
+
+@pytest.mark.parametrize("call", ["prefill", "step", "release"])
+def test_bookkeeping_that_fails_changes_nothing(ctx, monkeypatch, call):
+    """The call itself is refused (no memory for its outputs, say): host and device stay as they were, and together."""
+    cfg, w, dec = _decoder(layers=1)
+    cache = paged.PagedCache(cfg, rows=3, num_pages=8, page_size=16, max_length=64, dev=DEV)
+    ids = torch.zeros(20, dtype=torch.int64, device=DEV)
+    dec.prefill(ids[:16], [16], cache)
+    before = [t.clone() for t in (cache.lengths, cache.state_index, cache.free_count, cache.free_pages, cache.tables)]
+    with monkeypatch.context() as m:
+        m.setattr(paged, "block_tables", _fails)
+        m.setattr(paged, "release_blocks", _fails)
+        with pytest.raises(RuntimeError, match="no"):
+            dict(prefill=lambda: dec.prefill(ids, [20], cache), step=lambda: dec.step(ids[:3], cache), release=lambda: cache.release([0]))[call]()
+    ctx.sync()
+    assert cache.held.tolist() == [16, -1, -1] and cache.pages_left == 7
+    for t, old in zip((cache.lengths, cache.state_index, cache.free_count, cache.free_pages, cache.tables), before):
+        assert torch.equal(t, old)
+    dec.step(ids[:3], cache)
+    ctx.sync()
+    assert cache.held.tolist() == [17, -1, -1] and _device_matches(cache)
