@@ -174,6 +174,7 @@ class PagedCache:
         self.state_index = torch.full((rows,), -1, **i32)
         self.held = np.full(rows, -1, dtype=np.int64)
         self.unfinished = np.zeros(rows, dtype=bool)
+        self.positions = self.max_length  # up to which rows may grow: those of a decoder whose step was captured, if it has fewer
         self.pages_left = int(num_pages)
         channels = (2 * cfg.linear_num_key_heads + cfg.linear_num_value_heads) * 128
         self.layers: List = []
@@ -241,7 +242,7 @@ class PagedCache:
         """Whether every active row can grow by `steps` tokens."""
         live = self.held[self.held >= 0]
         need = sum(self._pages(n + steps) - self._pages(n) for n in live)
-        return not self.unfinished.any() and need <= self.pages_left and (len(live) == 0 or int(live.max()) + steps <= self.max_length)
+        return not self.unfinished.any() and need <= self.pages_left and (len(live) == 0 or int(live.max()) + steps <= self.positions)
 
     def advanced(self, steps: int = 1) -> None:
         """Notes on the host that every active row has `steps` more tokens; refuses steps that do not fit. (`Decoder.step` does as much;
@@ -253,7 +254,7 @@ class PagedCache:
         if self.unfinished.any():
             raise ValueError(f"a call failed half-way and left rows {np.flatnonzero(self.unfinished).tolist()} with part of a token: release them")
         if not self.fits(steps):
-            raise ValueError(f"{steps} more token(s) do not fit: {self.pages_left} pages left, rows of up to {self.max_length} tokens")
+            raise ValueError(f"{steps} more token(s) do not fit: {self.pages_left} pages left, rows of up to {self.positions} tokens")
 
     def _advance(self, steps: int) -> None:
         live = self.held >= 0

@@ -498,9 +498,12 @@ class Decoder:
         if ids.dim() != 1 or not ids.is_cuda or ids.shape[0] != cache.rows:
             raise ValueError(f"ids must be a CUDA tensor [{cache.rows}], a token for every row of the cache (no CPU fallback)")
         self._check(cache, ids)
-        if not torch.cuda.is_current_stream_capturing() and cache.held.max() >= self.max_positions:
+        eager = not torch.cuda.is_current_stream_capturing()
+        if eager and cache.held.max() >= self.max_positions:
             raise ValueError(f"a row has reached the decoder's {self.max_positions} positions")
-        live = (cache.held >= 0) & (not torch.cuda.is_current_stream_capturing())  # (what fails while it is captured has moved nothing)
+        if not eager:
+            cache.positions = min(cache.positions, self.max_positions)  # replays have only the cache's own count to stop them
+        live = (cache.held >= 0) & eager  # (what fails while it is captured has moved nothing)
         plan = cache.extend()
         cache.unfinished |= live
         x = _norm.embedding(self.w["embed_tokens"], ids.to(torch.int32).contiguous())

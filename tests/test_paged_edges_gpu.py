@@ -260,3 +260,33 @@ def test_bookkeeping_that_fails_changes_nothing(ctx, monkeypatch, call):
     dec.step(ids[:3], cache)
     ctx.sync()
     assert cache.held.tolist() == [17, -1, -1] and _device_matches(cache)
+
+
+def test_replayed_steps_end_where_the_positions_do(ctx):
+    """A cache that could hold longer rows than the decoder has positions: what counts the replays of a captured step stops there."""
+    cfg, w, dec = _decoder(layers=1)
+    dec = qwen35.Decoder(dec.w, cfg, max_positions=24)
+    cache = paged.PagedCache(cfg, rows=2, num_pages=8, page_size=16, max_length=64, dev=DEV)
+    ids = torch.zeros(20, dtype=torch.int64, device=DEV)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        dec.prefill(ids, [20], cache)
+        dec.step(ids[:2], cache)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            dec.step(ids[:2], cache)
+        assert cache.fits(3) and not cache.fits(4)
+        with pytest.raises(ValueError, match="24"):
+            cache.advanced(4)
+        cache.advanced(3)
+        for _ in range(3):
+            graph.replay()
+        stream.synchronize()
+        device.load(0).sync()
+        with pytest.raises(ValueError, match="24"):
+            cache.advanced(1)
+        with pytest.raises(ValueError, match="24 positions"):
+            dec.step(ids[:2], cache)
+    assert cache.held.tolist() == [24, -1] and cache.lengths.tolist() == [24, -1]
