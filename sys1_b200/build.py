@@ -3,14 +3,14 @@
 Takes the place of the reference's `build.rs:51-83` (which concatenates `src/kernels/*.cu` and emits generic
 PTX for whatever compute capability it finds): here there is exactly one target, `sm_100a`, and the output is
 a shared library exporting the C ABI declared in `include/sys1_b200.h`. Beside it goes `_binding.so`, the Python side of the
-decode-step calls (`csrc/binding.cpp`, g++), built against this interpreter and its PyTorch.
+decode-step calls (`csrc/binding.cpp`, g++), built against this interpreter and its PyTorch; where there is no PyTorch (a host that
+only links the C ABI) it is left out.
 
 Run as `python -m sys1_b200.build` (add `-v` for the ptxas resource report).
 """
 from __future__ import annotations
 
 import hashlib
-import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -39,9 +39,14 @@ NVCC_FLAGS = [
 BINDING = PKG / "_binding.so"
 
 
-def _binding_command() -> list:
+def _pytorch():
+    """Folder of this interpreter's PyTorch, or None."""
+    spec = importlib.util.find_spec("torch")
+    return Path(spec.submodule_search_locations[0]) if spec is not None and spec.submodule_search_locations else None
+
+
+def _binding_command(torch_dir: Path) -> list:
     """g++ on the Python side of the decode-step calls, against this interpreter's and its PyTorch's headers and the library beside it."""
-    torch_dir = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
     inc = [sysconfig.get_paths()["include"], torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include"]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", *(f"-I{p}" for p in inc),
             str(CSRC / "binding.cpp"), "-o", str(BINDING), "-L", str(PKG), "-l:libsys1_b200.so", "-L", str(torch_dir / "lib"),
@@ -69,7 +74,10 @@ def _fingerprint() -> str:
     for f in sorted([*CSRC.glob("*.cu"), *CSRC.glob("*.cpp")]):
         h.update(f.name.encode())
         h.update(f.read_bytes())
-    h.update((importlib.metadata.version("torch") + sys.version).encode())  # the binding is built against these
+    torch_dir = _pytorch()
+    if torch_dir is not None:  # the binding is built against these
+        version = torch_dir / "version.py"
+        h.update((version.read_bytes() if version.exists() else b"") + sys.version.encode())
     return h.hexdigest()
 
 
@@ -77,8 +85,8 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     """Compile the library if sources changed since the last build; returns the path of the .so. Each `.cu` file is
     compiled to an object of its own (in parallel, and only if it or a header changed), then the objects are linked."""
     from concurrent.futures import ThreadPoolExecutor
-    fp = _fingerprint()
-    if not force and LIB.exists() and BINDING.exists() and STAMP.exists() and STAMP.read_text().strip() == fp:
+    fp, torch_dir = _fingerprint(), _pytorch()
+    if not force and LIB.exists() and (BINDING.exists() or torch_dir is None) and STAMP.exists() and STAMP.read_text().strip() == fp:
         return LIB
     nvcc = _nvcc()
     OBJ.mkdir(exist_ok=True)
@@ -111,10 +119,13 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("linking libsys1_b200.so failed")
-    res = subprocess.run(_binding_command(), capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("building _binding.so failed")
+    if torch_dir is None:
+        sys.stderr.write(f"{BINDING.name} is left out: there is no PyTorch here to build it against (the C ABI does not need it)\n")
+    else:
+        res = subprocess.run(_binding_command(torch_dir), capture_output=True, text=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("building _binding.so failed")
     STAMP.write_text(fp)
     return LIB
 
