@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 2) s1_delta_step_kernel(const StepPa
             const __nv_bfloat16* ring = p.conv_state + r.slot * kTaps * C + c;
 #pragma unroll
             for (int back = 1; back < kTaps; ++back) in.past[back - 1] = back <= r.pos ? *reinterpret_cast<const uint32_t*>(ring + ((r.pos - back) & 3) * C) : 0u;
-            in.w = __ldg(reinterpret_cast<const uint4*>(p.conv_w + static_cast<long long>(c) * kTaps));
+            in.w = *reinterpret_cast<const uint4*>(p.conv_w + static_cast<long long>(c) * kTaps);
         } else if (tid == kConv) {
             in.x = __bfloat16_as_ushort(p.b[r.row * p.ldba + r.head]);
             in.past[0] = __bfloat16_as_ushort(p.a[r.row * p.ldba + r.head]);
@@ -157,8 +157,11 @@ __global__ void __launch_bounds__(kThreads, 2) s1_delta_step_kernel(const StepPa
         const Inputs in_next = fetch(next);
         const bool last_warp = warp == turn;  // writes this pair's output
         turn = turn + 1 == kWarps ? 0 : turn + 1;
-        uint2 zr = make_uint2(0, 0);
-        if (last_warp && there(now)) zr = *reinterpret_cast<const uint2*>(p.z + now.row * p.ldz + now.head * kDim + 4 * lane);
+        uint2 zr = make_uint2(0, 0), wr = zr;
+        if (last_warp && there(now)) {
+            zr = *reinterpret_cast<const uint2*>(p.z + now.row * p.ldz + now.head * kDim + 4 * lane);
+            wr = *reinterpret_cast<const uint2*>(p.norm_w + 4 * lane);
+        }
         // ---- conv + SiLU of this head's 384 channels, the gates
         bool bad = now.slot >= p.num_states || (now.slot >= 0 && now.pos < 0);
         if (p.index && now.slot >= 0) {  // a state that a row before this one has
@@ -234,7 +237,6 @@ __global__ void __launch_bounds__(kThreads, 2) s1_delta_step_kernel(const StepPa
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = rq * fmaf(sm.d[4 * lane + e], kq, keep * sm.sq[4 * lane + e]);
                 const float r = 1.f / sqrtf(warp_sum(o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3]) * (1.f / kDim) + p.eps);
-                const uint2 wr = __ldg(reinterpret_cast<const uint2*>(p.norm_w + 4 * lane));
                 const float z[4] = {lo_of(zr.x), hi_of(zr.x), lo_of(zr.y), hi_of(zr.y)}, w[4] = {lo_of(wr.x), hi_of(wr.x), lo_of(wr.y), hi_of(wr.y)};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] *= r * w[e] * z[e] * sigmoid(z[e]);

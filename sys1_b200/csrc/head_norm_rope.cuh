@@ -34,13 +34,22 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
+// Weights and tables: by the read-only path where the kernel is launched after its operands are complete (FIXED), by plain loads where it
+// may be resident before (the read-only path says that the data does not change in the kernel's life, so that the compiler may move such a
+// load ahead of the wait for the kernel before).
+template <bool FIXED, typename T>
+__device__ __forceinline__ T operand(const T* p) {
+    return FIXED ? __ldg(p) : *p;
+}
+
 // The cosines and sines of lane `sub` of a head (its 8 columns of the rotated span, `rot / 16` lanes to each half).
+template <bool FIXED>
 __device__ __forceinline__ void load_rotation(const float* cos_t, const float* sin_t, int pos, int rot, int sub, float (&c)[8], float (&sn)[8]) {
     const long long tb = static_cast<long long>(pos) * (rot / 2) + (sub & (rot / 16 - 1)) * 8;  // rot / 16 is a power of two
-    *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cos_t + tb));
-    *reinterpret_cast<float4*>(c + 4) = __ldg(reinterpret_cast<const float4*>(cos_t + tb) + 1);
-    *reinterpret_cast<float4*>(sn) = __ldg(reinterpret_cast<const float4*>(sin_t + tb));
-    *reinterpret_cast<float4*>(sn + 4) = __ldg(reinterpret_cast<const float4*>(sin_t + tb) + 1);
+    *reinterpret_cast<float4*>(c) = operand<FIXED>(reinterpret_cast<const float4*>(cos_t + tb));
+    *reinterpret_cast<float4*>(c + 4) = operand<FIXED>(reinterpret_cast<const float4*>(cos_t + tb) + 1);
+    *reinterpret_cast<float4*>(sn) = operand<FIXED>(reinterpret_cast<const float4*>(sin_t + tb));
+    *reinterpret_cast<float4*>(sn + 4) = operand<FIXED>(reinterpret_cast<const float4*>(sin_t + tb) + 1);
 }
 
 // The steps of bf16(x / sqrt(mean(x^2) + eps) * (1 + w)) and of the rotation, on 8 columns.
@@ -84,7 +93,7 @@ template <int LPR>
 __device__ __forceinline__ uint4 head_norm_rope(const uint4& raw, const __nv_bfloat16* w, float eps, const float (&c)[8], const float (&sn)[8],
                                                 bool rotate, int sub, int halfc, int bf16_ops) {
     const float rstd = 1.f / sqrtf(group_sum<LPR>(sum_squares8(raw)) * (1.f / static_cast<float>(8 * LPR)) + eps);
-    const uint4 normed = norm8(raw, rstd, __ldg(reinterpret_cast<const uint4*>(w + sub * 8)));
+    const uint4 normed = norm8(raw, rstd, operand<true>(reinterpret_cast<const uint4*>(w + sub * 8)));
     const uint4 other = shfl_xor4(normed, halfc);  // the partner half of the rotated span sits rot / 16 lanes away
     return rotate ? rotate8(normed, other, c, sn, sub < halfc, bf16_ops) : normed;
 }
@@ -96,7 +105,7 @@ __device__ __forceinline__ void head_norm_rope(uint4 (&x)[2], const __nv_bfloat1
                                                int sub, int halfc, int bf16_ops) {
     const float rstd = 1.f / sqrtf(group_sum<LPR>(sum_squares8(x[0]) + sum_squares8(x[1])) * (1.f / static_cast<float>(16 * LPR)) + eps);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] = norm8(x[i], rstd, __ldg(reinterpret_cast<const uint4*>(w + (sub + i * LPR) * 8)));
+    for (int i = 0; i < 2; ++i) x[i] = norm8(x[i], rstd, operand<false>(reinterpret_cast<const uint4*>(w + (sub + i * LPR) * 8)));
     if (halfc == LPR) {  // the whole head is rotated: a lane's pieces are each other's partners
         const uint4 lo = x[0], hi = x[1];
         if (rotate) x[0] = rotate8(lo, hi, c, sn, true, bf16_ops), x[1] = rotate8(hi, lo, c, sn, false, bf16_ops);

@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256) s1_head_norm_rope_kernel(__nv_bfloat16* _
     const bool pos_ok = pos >= 0 && pos < max_pos;
     float c[8], sn[8];
     if (rotates && pos_ok) {
-        load_rotation(cos_t, sin_t, pos, rot, sub, c, sn);
+        load_rotation<true>(cos_t, sin_t, pos, rot, sub, c, sn);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f;

@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kWriteThreads, NORM ? 9 : 16) s1_cache_write_k
         const int halfc = p.rot / 16;
         const bool rotates = live && sub < 2 * halfc, pos_ok = pos >= 0 && pos < p.max_pos;
         float c[8], sn[8];
-        load_rotation(p.cos_t, p.sin_t, pos_ok ? pos : 0, p.rot, sub, c, sn);  // (whatever the slot says, which may still be on its way)
+        load_rotation<false>(p.cos_t, p.sin_t, pos_ok ? pos : 0, p.rot, sub, c, sn);  // (whatever the slot says, which may still be on its way)
         head_norm_rope<LPR>(k, p.norm_w, p.eps, c, sn, rotates && pos_ok, sub, halfc, p.bf16_ops);
         if (rotates && !pos_ok) report(p.status, 102, t, pos);
     }

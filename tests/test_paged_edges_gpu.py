@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from paged_model import attention_64
-from sys1_b200 import _lib, device, paged, qwen35
+from sys1_b200 import _lib, device, norm, paged, qwen35
 from test_paged_gpu import DEV, _attention_case, _decoder, _refused, _step_case, bf, gen, ints
 
 pytestmark = pytest.mark.gpu
@@ -290,3 +290,44 @@ def test_replayed_steps_end_where_the_positions_do(ctx):
         with pytest.raises(ValueError, match="24 positions"):
             dec.step(ids[:2], cache)
     assert cache.held.tolist() == [24, -1] and cache.lengths.tolist() == [24, -1]
+
+
+# ------------------------------------------------------------------------------------------------ operands that the call before has written
+def test_weights_that_the_call_before_writes(ctx):
+    """A norm weight that lies in a page and is written there by the cache write just before: the kernels overlap, and the second one's
+    loads wait all the same."""
+    g = gen(6)
+    T, dim = 4096, 256
+    kc, vc = (torch.zeros(T // 16 + 1, 16, 1, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    cos, sin = torch.ones(1, 8, device=DEV), torch.zeros(1, 8, device=DEV)
+    last, slots, zeros = ints([T]), torch.arange(T, device=DEV, dtype=torch.int32), torch.zeros(T, dtype=torch.int32, device=DEV)
+    k = bf(g, T, 1, dim)
+    weights = [bf(g, 1, 1, dim) for _ in range(6)]
+    got = []
+    for w in weights:
+        paged.cache_write(w, w, kc, vc, last)
+        paged.cache_write(k, k, kc, vc, slots, norm_weight=kc[-1, 0, 0], cos=cos, sin=sin, positions=zeros, rotary_dim=16)
+        got.append(kc[:-1].clone())
+    for w, x in zip(weights, got):
+        want = k[:, 0].clone()
+        norm.head_norm_rope_(want, 1, dim, dim, w[0, 0], 1e-6, cos, sin, zeros, 16)
+        assert torch.equal(x.view(T, dim), want)
+    ctx.sync()
+
+
+def test_step_weights_that_the_call_before_writes(ctx):
+    """The same for the delta rule's step: its norm weight and its conv taps come out of a page that is written just before."""
+    c = _step_case(40, 1, 1, 12)
+    kc, vc = (torch.zeros(8, 1, 1, 256, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    for seed in range(6):
+        g = gen(seed)
+        taps, w = bf(g, 384, 4, s=0.3), 1 + bf(g, 128, s=0.1)
+        rows = torch.cat([taps.flatten(), w, w]).view(7, 1, 256)  # six rows of taps, one of two norm weights
+        c = dict(c, conv_weight=taps, norm_weight=w)
+        d = dict(c, state=c["state"].clone(), conv_state=c["conv_state"].clone(), conv_weight=kc[:6].view(384, 4), norm_weight=kc[6].view(256)[:128])
+        want = qwen35.gated_delta_rule_step(**c)
+        ctx.sync()
+        paged.cache_write(rows, rows, kc, vc, ints(range(7)))
+        got = qwen35.gated_delta_rule_step(**d)
+        assert torch.equal(got, want) and torch.equal(c["state"], d["state"])
+    ctx.sync()
