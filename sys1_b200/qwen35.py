@@ -221,6 +221,10 @@ class LinearAttention:
             conv, state, pos = *kept.layer, kept.positions
             if state.shape[1:] != (self.value_heads, 128, 128) or conv.shape[1:] != (4, pre.shape[1]) or conv.shape[0] != state.shape[0]:
                 raise ValueError(f"the states are those of other heads: {list(conv.shape)} and {list(state.shape)}")
+            for name, t, dtype, least in (("positions", pos, torch.int32, T), ("cu_seqlens", kept.cu_seqlens, torch.int32, len(cu)),
+                                          ("state_index", kept.state_index, torch.int32, len(cu) - 1), ("conv", conv, torch.bfloat16, 0), ("state", state, torch.float32, 0)):
+                if t.dtype != dtype or t.device != x.device or not t.is_contiguous() or t.numel() < least:
+                    raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor on the GPU of x" + (f" with {least} values at least" if least else ""))
             rc = ctx._lib.s1_gated_delta_rule_prefill(ctx.handle, P(pre), pre.stride(0), P(self.conv_taps), P(pos), *tail, P(kept.cu_seqlens),
                                                       P(kept.state_index), state.shape[0], P(conv), P(state))
         elif self.fuse_conv:

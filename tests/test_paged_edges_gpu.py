@@ -8,7 +8,7 @@ import torch
 
 from paged_model import attention_64
 from sys1_b200 import _lib, device, norm, paged, qwen35
-from test_paged_gpu import DEV, _attention_case, _decoder, _refused, _step_case, bf, gen, ints
+from test_paged_gpu import DEV, _attention_case, _decoder, _linear_attention, _refused, _step_case, bf, gen, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -331,3 +331,22 @@ def test_step_weights_that_the_call_before_writes(ctx):
         got = qwen35.gated_delta_rule_step(**d)
         assert torch.equal(got, want) and torch.equal(c["state"], d["state"])
     ctx.sync()
+
+
+@pytest.mark.parametrize("name,change", [("cu_seqlens", lambda t: t[:-1]), ("cu_seqlens", lambda t: t.long()), ("cu_seqlens", lambda t: t.cpu()),
+                                         ("state_index", lambda t: t[:1]), ("state_index", lambda t: t.long()), ("state_index", lambda t: t.repeat(2)[::2]),
+                                         ("positions", lambda t: t[:-1]), ("positions", lambda t: t.long()), ("state", lambda t: t.to(torch.bfloat16)),
+                                         ("state", lambda t: t.transpose(2, 3)), ("conv", lambda t: t.float()), ("conv", lambda t: t[::2]), ("conv", lambda t: t.cpu())])
+def test_prefill_refuses_what_its_kernels_would_misread(ctx, name, change):
+    """Arrays too short for the batch, of other types, elsewhere, or with gaps: before any kernel sees them."""
+    m, lens = _linear_attention(7), [70, 5]
+    x, cu = bf(gen(3), 75, 256), np.cumsum([0] + lens).astype(np.int32)
+    pos = ints(np.concatenate([np.arange(n) for n in lens]))
+    parts = dict(conv=torch.zeros(4, 4, 1024, dtype=torch.bfloat16, device=DEV), state=torch.zeros(4, 4, 128, 128, device=DEV), positions=pos,
+                 state_index=ints([2, 0]), cu_seqlens=ints(cu))
+    kept = lambda p: qwen35.Kept(paged.DeltaState(p["conv"], p["state"]), p["positions"], pos, p["state_index"], cu_seqlens=p["cu_seqlens"])  # noqa: E731
+    with pytest.raises(ValueError, match="state|conv|positions|cu_seqlens"):
+        m.mix(x, cu, pos, kept({**parts, name: change(parts[name])}))
+    assert torch.equal(m.mix(x, cu, pos, kept(parts)), m.mix(x, cu, pos))
+    ctx.sync()
+    assert bool((parts["state"][[0, 2]] != 0).any(-1).any(-1).all()) and not parts["state"][[1, 3]].any()
