@@ -282,6 +282,7 @@ inline bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintpt
 
 int s1_conv_state_launch(s1_ctx* ctx, const void* mixed, long long ldm, const int32_t* cu_seqlens, int num_seqs, int total_tokens, const int32_t* index,
                          int num_states, int channels, void* conv_state) {
+    if (num_seqs == 0) return S1_OK;
     s1_conv_state_kernel<<<dim3(num_seqs, kTaps), 256, 0, ctx->stream>>>(static_cast<const __nv_bfloat16*>(mixed), ldm, cu_seqlens, index, num_states,
                                                                          total_tokens, channels, static_cast<__nv_bfloat16*>(conv_state));
     S1_CUDA_OK(ctx, cudaGetLastError());

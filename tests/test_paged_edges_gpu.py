@@ -350,3 +350,12 @@ def test_prefill_refuses_what_its_kernels_would_misread(ctx, name, change):
     assert torch.equal(m.mix(x, cu, pos, kept(parts)), m.mix(x, cu, pos))
     ctx.sync()
     assert bool((parts["state"][[0, 2]] != 0).any(-1).any(-1).all()) and not parts["state"][[1, 3]].any()
+
+
+def test_prefill_of_a_batch_without_sequences(ctx):
+    """Only tokens behind the last sequence: no sequence leaves a state, and that is no error."""
+    m, x = _linear_attention(7), bf(gen(3), 8, 256)
+    conv, state, pos = torch.ones(2, 4, 1024, dtype=torch.bfloat16, device=DEV), torch.ones(2, 4, 128, 128, device=DEV), ints([0] * 8)
+    m.mix(x, np.zeros(1, np.int32), pos, qwen35.Kept(paged.DeltaState(conv, state), pos, pos, ints([0]), cu_seqlens=ints([0])))
+    ctx.sync()
+    assert bool((conv == 1).all()) and bool((state == 1).all())
