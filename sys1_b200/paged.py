@@ -26,11 +26,8 @@ class BlockTables(NamedTuple):
     free_count: torch.Tensor
 
 
-_I32, _BF16 = torch.int32, torch.bfloat16
-
-
 def _ints(t: torch.Tensor, dev: int, n: int, name: str) -> int:
-    if t.dtype is not _I32 or t.get_device() != dev or dev < 0 or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.get_device() != dev or dev < 0 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor on the call's GPU (no CPU fallback)")
     if t.shape != (n,):
         raise ValueError(f"{name} must have shape [{n}], not {list(t.shape)}")
@@ -39,7 +36,7 @@ def _ints(t: torch.Tensor, dev: int, n: int, name: str) -> int:
 
 def _table(t: torch.Tensor, dev: int, rows: int):
     """Address, row stride and width of the block tables."""
-    if t.dtype is not _I32 or t.get_device() != dev or dev < 0 or t.dim() != 2 or t.shape[0] != rows or (t.stride(1) != 1 and t.shape[1] != 1):
+    if t.dtype is not torch.int32 or t.get_device() != dev or dev < 0 or t.dim() != 2 or t.shape[0] != rows or (t.stride(1) != 1 and t.shape[1] != 1):
         raise ValueError(f"block tables must be an int32 CUDA tensor [{rows}, pages] with contiguous rows")
     return t.data_ptr(), t.shape[1] if rows == 1 else t.stride(0), t.shape[1]
 
@@ -77,11 +74,8 @@ def release_blocks(ended: torch.Tensor, lengths: torch.Tensor, tables: torch.Ten
     ep, lp, fp, np_ = (_ints(ended, dev, rows, "ended"), _ints(lengths, dev, rows, "lengths"), _ints(free_pages, dev, pool, "free_pages"),
                        _ints(free_count, dev, 1, "free_count"))
     tp, ldt, width = _table(tables, dev, rows)
-    if ctx is None:
-        ctx = device.load(dev)
-    elif ctx.ordinal != dev:
-        raise ValueError(f"the tensors are on GPU {dev}, the context on GPU {ctx.ordinal}")
-    ctx.check(ctx._lib.s1_release_blocks(ctx._h, ep, rows, page_size, lp, tp, ldt, width, fp, pool, np_))
+    ctx, handle = _context(dev, ctx)
+    ctx.check(ctx._lib.s1_release_blocks(handle, ep, rows, page_size, lp, tp, ldt, width, fp, pool, np_))
 
 
 def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
