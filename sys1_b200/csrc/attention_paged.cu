@@ -7,24 +7,25 @@
 // the group size. So the kernel is built around the loads:
 //  * work is cut into units of kUnit keys of one (row, KV head, 8 or 16 of its query heads) - a "span" is all units of one such triple -
 //    and the units of the whole batch, in order, are dealt out in contiguous ranges of equal cost, one to each CTA of the grid; a
-//    span's beginning is counted too, as so many units (kStart; without it 32 short contexts beside 30 of 8192 tokens took 340 us,
-//    with it 209). The CTAs find their ranges from the lengths in device memory, so that nothing of a step depends on the host and
+//    span's beginning is counted too, as so many units (kStart; without it 32 contexts of 128 tokens beside 30 of 8192 take 254 us,
+//    with it 161). The CTAs find their ranges from the lengths in device memory, so that nothing of a step depends on the host and
 //    the balance holds for one long context and for many ragged ones alike. A span that crosses from one CTA to the next leaves
 //    partial results (maximum, sum, unnormalised output in f32) in the workspace, at most two per CTA; and a second
 //    kernel joins them, in the order of the units: results do not depend on timing. (Joined by the CTA that finds all pieces of a
-//    span there, without the second kernel, the pieces were one CTA's work: 32 contexts up to 2048 took 27 us instead of 21.)
+//    span there, without the second kernel, the pieces were one CTA's work: an earlier form of this kernel, 21 us for 32 contexts up to
+//    2048, took 27 that way.)
 //  * inside a CTA the warps take tiles of 16 keys in turn, each through a ring of its own in shared memory (cp.async, 192 KB an SM in
 //    flight or in use): no warp waits for another until its span is done. The next span's first keys are fetched into
 //    L2 and its queries into registers while the warps' results are put together.
 //  * the products run on mma.sync m16n8k16 with the operands turned round - S^T = K Q^T, O^T = V^T P^T - so that the 16 rows are
 //    keys and head dimensions, which there are enough of, and the 8 columns the query heads of the group. tcgen05 would want 64 or
-//    128 rows of queries where there are 1 to 16; at the rate that HBM delivers keys, mma.sync is a fifth busy.
-// Measured: 62 contexts of 100 .. 8192 tokens, 24 query and 4 KV heads of 256: 168 us = 6.3 TB/s; one of 131071 tokens, 8 and 2 heads:
-// 49 us = 5.4 TB/s; 31 of 1 .. 2048 tokens: 19.6 us; one of 17: 6 us.
+//    128 rows of queries where there are 1 to 16; at the rate that HBM delivers keys, the tensor pipe is 15 % busy.
+// Measured: 62 contexts of 100 .. 8192 tokens, 24 query and 4 KV heads of 256: 169 us = 6.2 TB/s; one of 131071 tokens, 8 and 2 heads:
+// 50 us = 5.4 TB/s; 31 of 1 .. 2048 tokens: 19.6 us; one of 17: 6.5 us.
 // Scores, maxima, sums and outputs are f32. For the second product a weight is split into two bf16 values, its first eight bits and
 // what they leave (rounded: an error of 2^-15 of the weight, where one bf16 value would be 2^-8 off); their sum over the keys is that of
-// the f32 weights. The product with the rest costs 168.5 -> 169.7 us
-// at the first size above, 19.4 -> 19.5 at the third (captured, both sides in turn).
+// the f32 weights. The product with the rest costs 1 % at the first size above and at the third, up to 5 % elsewhere (16 heads to a KV head
+// of 64, 450 contexts of 900 tokens: 35.7 -> 37.6 us).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -388,7 +389,7 @@ struct Segment {     // the part of one span that lies in the range
     int end;             // keys u0 * kUnit .. end - 1
 };
 
-// P CTAs of W warps per SM. W = 8 and as many CTAs as the registers allow, one at a head dim of 256 and two below (head dim 128, 28 contexts
+// P CTAs of W warps per SM (both sides of each pair measured with weights of one part). W = 8 and as many CTAs as the registers allow, one at a head dim of 256 and two below (head dim 128, 28 contexts
 // of up to 61259 tokens, 4 heads on 2: 161 us, with one 163; head dim 64, 4 of 66164, 64 on 4: 37 and 44) but one at head dim 128 with NT
 // = 2, which would spill (94 of 3443, 64 on 4: 92 us, with two 114). Where there are many spans, W = 4: one's keys come while another puts
 // its results together (head dim 256: 512 contexts of 100 tokens 40 us with W = 8, 35 with 4; with few and long ones the larger units
@@ -708,7 +709,8 @@ int launch(s1_ctx* ctx, PagedParams p, int units) {
     S1_CUDA_OK(ctx, s1_launch_waiting(ctx, s1_attention_paged_kernel<D, NT, W, P>, static_cast<unsigned>(ctas), 1u, W * 32u, smem, p));
     ctx->launches += 1;
     // a span of one unit is never cut: block tables that hold no more than a unit leave nothing to join (one context of 17 tokens in a
-    // table of 32: 7.3 us with the second kernel, 6.3 without)
+    // table of 32: 7.3 us with the second kernel, 6.3 without). Callers that cut their tables to what is used have this; those of a
+    // `PagedCache` are as wide as its longest row may get.
     if (static_cast<long long>(p.table_width) << p.shift <= WarpPass<D, NT, W, P>::kUnit) return S1_OK;
     constexpr int kThreads = D == 256 ? 256 : 128;
     const bool many = 4 * spans >= ctas;  // four pieces to a span at most, were all spans alike

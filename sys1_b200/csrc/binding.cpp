@@ -1,7 +1,8 @@
 // The Python side of the decode-step calls (module sys1_b200._binding): arguments checked, outputs allocated, the C ABI called. From
 // Python itself the checks of up to 14 tensors, at 0.1 us an attribute, and the conversion of up to 27 arguments took longer than
-// the kernels of a small step. Measured, calls one after the other: block tables 14.1 -> 6.7 us, cache write 11.2 -> 4.2, attention
-// 16.0 -> 7.8, delta step 15.0 -> 5.6; what is left is the launches (3.3 us one, 5.6 the attention's two) and the outputs.
+// the kernels of a small step. Measured, calls one after the other: block tables 14.1 -> 6.8 us, cache write 11.2 -> 4.0, attention
+// 16.0 -> 7.0, delta step 15.0 -> 5.5 (a tenth more where the host is busy); what is left is the launches (3.3 us one, 5.6 the
+// attention's two) and the outputs.
 // Every function takes a context's handle, then the arguments of the Python function of the same name in its order (None where one is
 // left out), and returns its result, or the error code of the C call as an int. Bad arguments raise ValueError.
 #include <torch/csrc/Exceptions.h>

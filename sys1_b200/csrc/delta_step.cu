@@ -10,7 +10,7 @@
 // arithmetic. With
 //     S^T k and S^T q taken over the old S,   o = e^g (S^T q) + d (k . q),
 // both sums over the key rows come from the same pass and one exchange between the warps, and S leaves as it is updated. Measured: 64
-// rows x 48 heads 72 us = 5.6 TB/s (one block of 512 threads a pair 115 us, one such block an SM with three S in its ring 93), one
+// rows x 48 heads 71 us = 5.7 TB/s (one block of 512 threads a pair 115 us, one such block an SM with three S in its ring 93), one
 // row x 16 heads 5 us.
 // Sums, norms and state are f32 throughout (the prompt form rounds the conv tap by tap to bf16, as the reference's kernel does; a
 // step keeps it in f32). The conv's history is a ring of four rows by position mod 4: the new row's place is one that no conv of
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 2) s1_delta_step_kernel(const StepPa
         parity ^= 1;
     }
     // (not earlier: the next kernel's blocks would be placed two to an SM on what this grid leaves free - 37 rows of 6 heads 7.6 us
-    // instead of 6.9 in a row of steps)
+    // instead of 6.9 in a row of steps, when this was tried)
     s1::griddep_launch_dependents();
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }

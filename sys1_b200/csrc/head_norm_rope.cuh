@@ -87,7 +87,8 @@ __device__ __forceinline__ uint4 shfl_xor4(const uint4& v, int mask) {
 }
 
 // bf16(x / sqrt(mean(x^2) + eps) * (1 + w)) over the 8 * LPR columns of the head, then the rotation of its first `16 * halfc`
-// columns where `rotate`. bf16_ops = 1: each product and the sum are bf16 values (src/archs/qwen35_text.rs:302); 0: products and
+// columns where `rotate`. The rotation starts from the norm rounded to bf16, as the norm's own output is in the reference and in
+// s1_norm followed by s1_rope, whose bits these are (2^-8 of a value more than one rounding in all). bf16_ops = 1: each product and the sum are bf16 values (src/archs/qwen35_text.rs:302); 0: products and
 // sum in f32, rounded once. Every lane of the warp takes part in the exchanges, also those without a live row.
 template <int LPR>
 __device__ __forceinline__ uint4 head_norm_rope(const uint4& raw, const __nv_bfloat16* w, float eps, const float (&c)[8], const float (&sn)[8],
