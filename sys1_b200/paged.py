@@ -158,7 +158,8 @@ class PagedCache:
         self.device = dev
         i32 = dict(dtype=torch.int32, device=dev)
         width = -(-max_length // page_size)
-        spans = rows * cfg.num_key_value_heads * -(-cfg.num_attention_heads // (8 * cfg.num_key_value_heads))  # s1_attention_paged's limit
+        group = cfg.num_attention_heads // cfg.num_key_value_heads
+        spans = rows * cfg.num_key_value_heads * (1 if group <= 8 else -(-group // 16))  # s1_attention_paged's limit
         if (spans + 1) * (width * page_size // 64 + 5) > 1 << 31:
             raise ValueError("rows x KV heads x max_length / 64 must be below 2^31")
         self.tables = torch.zeros((rows, width), **i32)

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import oracle
 from paged_model import attention_64
 from sys1_b200 import _lib, device, norm, paged, qwen35
 from test_paged_gpu import DEV, _attention_case, _decoder, _linear_attention, _refused, _step_case, bf, gen, ints
@@ -359,3 +360,19 @@ def test_prefill_of_a_batch_without_sequences(ctx):
     m.mix(x, np.zeros(1, np.int32), pos, qwen35.Kept(paged.DeltaState(conv, state), pos, pos, ints([0]), cu_seqlens=ints([0])))
     ctx.sync()
     assert bool((conv == 1).all()) and bool((state == 1).all())
+
+
+def test_the_cache_takes_every_size_that_its_kernels_do(ctx):
+    """16 query heads to a KV head are one span: 8192 rows of up to 2^21 tokens are within the attention's limit, and so within the cache's."""
+    cfg = oracle.DecoderConfig(vocab_size=16, hidden_size=64, intermediate_size=64, num_hidden_layers=1, num_attention_heads=64, num_key_value_heads=4,
+                               head_dim=256, full_attention_interval=1)
+    cache = paged.PagedCache(cfg, rows=8192, num_pages=1, page_size=65536, max_length=1 << 21, dev=DEV)
+    cache.lengths[:2] = ints([1, 3])
+    k, v = cache.layers[0]
+    k[0, :3], v[0, :3] = 0, bf(gen(1), 3, 4, 256)
+    got = paged.attention_paged(torch.zeros(8192, 64, 256, dtype=torch.bfloat16, device=DEV), k, v, cache.tables, cache.lengths, workspace=cache.workspace)
+    ctx.sync()
+    want = torch.stack([v[0, 0].float(), v[0, :3].float().mean(0)])[:, :, None].expand(2, 4, 16, 256).reshape(2, 64 * 256)
+    assert bool(((got[:2].float() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14).all()) and not got[2:].any()
+    with pytest.raises(ValueError, match="below 2.31"):
+        paged.PagedCache(cfg, rows=8192, num_pages=1, page_size=65536, max_length=1 << 22, dev=DEV)
